@@ -598,6 +598,93 @@ int mx_nbit_forward_nobag(const uint8_t* dev_weights, const int64_t* weights_off
                           int32_t fp8_exponent_bits, int32_t fp8_exponent_bias, void* out,
                           void* stream);
 
+/* ---- attention over packed sequences (no fbgemm counterpart) -------------
+ * Softmax attention of the lists that offsets cut a packed tensor into (the
+ * rows and offsets a sequence lookup gives), with grouped key-value heads.
+ * List b has queries q_offsets[b] .. q_offsets[b + 1] - 1 and keys k_offsets[b]
+ * .. k_offsets[b + 1] - 1 (the same array for self-attention); with `causal`,
+ * query i of Lq sees key j of Lk if j <= i + Lk - Lq, so that a list's last
+ * query sees every key.  A query that sees no key, and a query row of no list,
+ * gives zeros and lse = -inf; a key row of no list gets zero gradients.  Rows
+ * of other lists are never read into a list's result.  fp16 or bf16, D a
+ * multiple of 8 up to MX_ATTENTION_MAX_D, H a multiple of Hkv (query head h
+ * reads key-value head h / (H / Hkv)). */
+#define MX_ATTENTION_MAX_D 128
+
+/* A [rows, heads, D] operand: strides in elements (multiples of 8; of a row at
+ * least D and at most 2^23), the last dimension contiguous, 16-byte aligned. */
+typedef struct mx_attention_tensor {
+  const void* data;
+  int64_t row_stride;
+  int64_t head_stride;
+} mx_attention_tensor;
+
+typedef struct mx_attention_problem {
+  int32_t dtype;          /* MX_DTYPE_F16 or MX_DTYPE_BF16 */
+  int32_t index_bytes;    /* of the offsets: 4 or 8 */
+  const void* q_offsets;  /* [B + 1], non-decreasing */
+  const void* k_offsets;  /* [B + 1] */
+  int64_t B, Nq, Nk;      /* lists, query rows, key rows */
+  int32_t H, Hkv, D;
+  int32_t causal;
+  float scale;            /* of the scores; positive */
+} mx_attention_problem;
+
+/* out: contiguous [Nq, H, D] of the inputs' type; lse (natural logarithm of
+ * each query's sum, may be NULL): [H, Nq] fp32. */
+int mx_jagged_attention_forward(const mx_attention_problem* p, const mx_attention_tensor* q,
+                                const mx_attention_tensor* k, const mx_attention_tensor* v,
+                                void* out, float* lse, void* stream);
+
+/* Gradients of the above from its out and lse: contiguous [Nq, H, D] and twice
+ * [Nk, Hkv, D], the same bits for the same inputs.  Without dk and dv (both
+ * NULL) dq alone. */
+size_t mx_jagged_attention_backward_workspace_bytes(int64_t Nq, int32_t H);
+int mx_jagged_attention_backward(const mx_attention_problem* p, const mx_attention_tensor* q,
+                                 const mx_attention_tensor* k, const mx_attention_tensor* v,
+                                 const mx_attention_tensor* out,
+                                 const mx_attention_tensor* grad_out, const float* lse, void* dq,
+                                 void* dk, void* dv, void* workspace, size_t workspace_bytes,
+                                 void* stream);
+
+/* ---- paged key-value cache (no fbgemm counterpart) -----------------------
+ * Keys and values of a batch's sequences in pages of page_size tokens: token t
+ * of sequence b is in slot t % page_size of page table[b, t / page_size].
+ * Strides in elements (multiples of 8), a head's D values contiguous, pointers
+ * 16-byte aligned.  An entry outside [0, pages) is never followed: an append
+ * drops its rows, the attention takes its tokens as absent; entries past a
+ * sequence's length are not read. */
+typedef struct mx_paged_cache {
+  void* k;
+  void* v;
+  int64_t k_page_stride, k_slot_stride, k_head_stride;
+  int64_t v_page_stride, v_slot_stride, v_head_stride;
+  int64_t pages;
+  int32_t page_size;
+  const int32_t* table;      /* [B, table_width] */
+  int64_t table_row_stride;  /* entries */
+  int64_t table_width;
+} mx_paged_cache;
+
+/* Writes rows offsets[b] .. offsets[b + 1] - 1 of k and v (strided [N, Hkv, D])
+ * to tokens starts[b], starts[b] + 1, ... of sequence b.  Rows of no list, and
+ * tokens past the table's width, are dropped. */
+int mx_paged_cache_append(const mx_paged_cache* cache, int32_t dtype, int32_t Hkv, int32_t D,
+                          const mx_attention_tensor* k, const mx_attention_tensor* v, int64_t N,
+                          int64_t B, const void* offsets, int32_t offsets_bytes,
+                          const void* starts, int32_t starts_bytes, void* stream);
+
+/* Attention of one query per sequence (q [B, H, D], strided) over its first
+ * lengths[b] tokens (at most table_width * page_size): out contiguous
+ * [B, H, D]; zeros where there is no token.  The same bits for the same
+ * inputs. */
+size_t mx_paged_cache_attention_workspace_bytes(const mx_paged_cache* cache, int64_t B, int32_t H,
+                                                int32_t Hkv, int32_t D);
+int mx_paged_cache_attention(const mx_paged_cache* cache, int32_t dtype,
+                             const mx_attention_tensor* q, int64_t B, int32_t H, int32_t Hkv,
+                             int32_t D, const void* lengths, int32_t lengths_bytes, float scale,
+                             void* out, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

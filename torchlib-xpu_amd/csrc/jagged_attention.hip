@@ -1,0 +1,685 @@
+// Attention over packed (jagged) sequences, forward and backward, for fp16 and
+// bf16 with grouped key-value heads.
+//
+// List b has queries i in [0, Lq) and keys j in [0, Lk); query i sees key j if
+// !causal or j <= i + Lk - Lq (the last query sees every key).  Over the
+// visible keys
+//   s_ij = scale q_i.k_j,  lse_i = log sum_j exp(s_ij),  p_ij = exp(s_ij - lse_i),
+//   o_i = sum_j p_ij v_j;   a query that sees no key has o_i = 0, lse_i = -inf.
+#include "attention_common.h"
+
+namespace mx {
+namespace attn {
+namespace {
+
+struct FwdArgs {
+  const char *q, *k, *v;           // bytes
+  int64_t q_row, q_head;           // strides in bytes
+  int64_t k_row, k_head, v_row, v_head;
+  const void *q_offsets, *k_offsets;
+  int64_t B, Nq, Nk;
+  int32_t H, G, D;                 // G query heads per key-value head
+  int32_t causal;
+  float scale;
+  void* out;                       // [Nq, H, D]
+  float* lse;                      // [H, Nq] or null
+};
+
+// Which head and tile slot a block works on.  Blocks go to the 8 XCDs in turn:
+// with a multiple of 8 heads each XCD keeps H / 8 neighbouring heads (which
+// share keys) and takes all their tiles, so its L2 holds few keys and the
+// causal tiles, unequal in length, spread evenly.  Later tiles first: they are
+// a list's longest under the causal mask.
+__device__ __forceinline__ void head_and_slot(int64_t bid, int H, int64_t slots, int* head,
+                                              int64_t* slot) {
+  if (H % 8 == 0) {
+    const int per = H / 8;
+    const int64_t x = bid % 8, y = bid / 8;
+    *head = static_cast<int>(x * per + y % per);
+    *slot = slots - 1 - y / per;
+  } else {
+    *head = static_cast<int>(bid % H);
+    *slot = slots - 1 - bid / H;
+  }
+}
+
+// Writes one lane's row of a transposed result: column l of acc is a row of
+// `out`, its values scaled and rounded to the output's type.
+template <typename T, int DP>
+__device__ __forceinline__ void store_columns(T* out, const f32x16* acc, float scale, int D, int h) {
+  typedef T x4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const int col = 32 * d + 8 * (i / 4) + 4 * h;
+      x4 w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = static_cast<T>(acc[d][i + e] * scale);
+      if (col < D) *reinterpret_cast<x4*>(out + col) = w;
+    }
+}
+
+// Row l of a 32-row tile as the B operand: 8 columns per step.
+template <typename X8, int KS>
+__device__ __forceinline__ void load_rows(X8* f, const char* base, int rows, int64_t stride, int D,
+                                          int l, int h) {
+  const __amdgpu_buffer_rsrc_t r = make_rsrc(base, span_bytes(rows, static_cast<uint32_t>(stride), D * 2));
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int c = 2 * s + h;
+    const uint32_t off = c * 8 < D ? static_cast<uint32_t>(l) * static_cast<uint32_t>(stride) + c * 16 : kOutside;
+    f[s] = __builtin_bit_cast(X8, load16(r, off));
+  }
+}
+
+constexpr int kBN = 64;  // keys per tile
+
+// One block: NW waves, 32 queries each, of one list and head.  Tiles of 64 keys
+// and values go to LDS, the next one while this one is worked on.  Per tile a
+// wave computes K Q^T (a query per lane), the running maximum and sum of its
+// queries in registers, and adds V^T P^T to its outputs, which are rescaled
+// only when a maximum has grown by more than 2^8.  Probabilities are rounded to
+// the input type for the second product; sums, maxima and outputs are fp32.
+template <typename T, typename I, int DP, int NW>
+__global__ void __launch_bounds__(NW * 64, 2) fwd_kernel(const FwdArgs a, int64_t slots) {
+  using E = Elem<T>;
+  using X8 = typename E::x8;
+  using Ti = Tile<DP>;
+  constexpr int KS = DP / 16, DB = DP / 32, BM = NW * 32;
+  constexpr int kTileBytes = kBN * DP * 2;
+  __shared__ __attribute__((aligned(1024))) char lds[4 * kTileBytes];  // K0 V0 K1 V1
+
+  int head;
+  int64_t slot, tile;
+  head_and_slot(blockIdx.x, a.H, slots, &head, &slot);
+  const I* qo = static_cast<const I*>(a.q_offsets);
+  const I* ko = static_cast<const I*>(a.k_offsets);
+  constexpr int kShift = NW == 1 ? 5 : NW == 2 ? 6 : NW == 4 ? 7 : 8;
+  const int64_t list = find_list(qo, a.B, a.Nq, kShift, slot, &tile);
+  const Span sq = list_span(qo, a.B, a.Nq, list);
+  if (tile * BM >= sq.len) return;
+  Span sk{0, 0};
+  if (list > 0 && list <= a.B) sk = list_span(ko, a.B, a.Nk, list);
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63, l = lane & 31, h = lane >> 5;
+  const int64_t row0 = uniform64(tile * BM + wave * 32);  // the wave's first query in the list
+  const int64_t q_base = uniform64(sq.start + row0);
+  const int rows = static_cast<int>(sq.len - row0 < 32 ? (sq.len > row0 ? sq.len - row0 : 0) : 32);
+  const int64_t Lk = uniform64(sk.len);
+  const int64_t shift = uniform64(Lk - sq.len);  // query i sees keys 0 .. i + shift
+  // Keys that a query of the block, and one of the wave, sees at most.
+  int64_t blk_end = Lk, wave_end = Lk;
+  if (a.causal) {
+    const int64_t last = (tile + 1) * BM < sq.len ? (tile + 1) * BM : sq.len;
+    blk_end = last + shift < Lk ? last + shift : Lk;
+    wave_end = row0 + rows + shift;
+  }
+  if (rows == 0) wave_end = 0;
+  const int tiles = blk_end > 0 ? static_cast<int>((blk_end + kBN - 1) / kBN) : 0;
+
+  // Queries: the B operand of K Q^T.
+  X8 qf[KS];
+  load_rows<X8, KS>(qf, a.q + q_base * a.q_row + head * a.q_head, rows, a.q_row, a.D, l, h);
+
+  typename Ti::template Loader<kBN, NW * 64> lk, lv;
+  lk.init(tid, static_cast<uint32_t>(a.k_row), a.D / 8);
+  lv.init(tid, static_cast<uint32_t>(a.v_row), a.D / 8);
+  const char* kp = a.k + uniform64(sk.start) * a.k_row + (head / a.G) * a.k_head;
+  const char* vp = a.v + uniform64(sk.start) * a.v_row + (head / a.G) * a.v_head;
+  f32x16 o[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) o[d] = f32x16{};
+  float m = -INFINITY, sum = 0.0f;
+  const float c2 = a.scale * kLog2e;
+
+  // LDS places of this lane's operands.
+  const int t16 = lane & 15, g16 = (lane >> 4) & 1;
+  const int vrow = 4 * h + (t16 >> 2);
+
+  // The restrict pointers tell the compiler that the copies into the next
+  // tiles' LDS do not meet this tile's reads (it would wait for them).
+  auto load_tile = [&](int j, char* __restrict__ dst) __attribute__((always_inline)) {
+    const int64_t left = Lk - static_cast<int64_t>(j) * kBN;
+    const int n = left < kBN ? static_cast<int>(left) : kBN;
+    lk.load(make_rsrc(kp + static_cast<int64_t>(j) * kBN * a.k_row,
+                      span_bytes(n, static_cast<uint32_t>(a.k_row), a.D * 2)), dst, wave);
+    lv.load(make_rsrc(vp + static_cast<int64_t>(j) * kBN * a.v_row,
+                      span_bytes(n, static_cast<uint32_t>(a.v_row), a.D * 2)),
+            dst + kTileBytes, wave);
+  };
+  auto work = [&](int j, const char* __restrict__ kt, char* __restrict__ next) __attribute__((always_inline)) {
+    if (j + 1 < tiles) load_tile(j + 1, next);
+    const int64_t k0 = static_cast<int64_t>(j) * kBN;
+    if (k0 >= wave_end) return;
+    const char* vt = kt + kTileBytes;
+
+    f32x16 s[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      s[b] = f32x16{};
+#pragma unroll
+      for (int x = 0; x < KS; ++x)
+        s[b] = E::mfma32(lds_read16<X8>(kt + Ti::at(32 * b + l, 2 * x + h)), qf[x], s[b]);
+    }
+
+    // Mask: only where the tile reaches past a query's last key.
+    const int64_t end0 = a.causal ? row0 + shift + 1 : Lk;  // of the wave's first query
+    if (k0 + kBN > end0 || k0 + kBN > Lk) {
+      const int64_t mine = a.causal ? row0 + l + shift + 1 : Lk;
+      const int last = static_cast<int>((mine < Lk ? mine : Lk) - k0 < kBN ? (mine < Lk ? mine : Lk) - k0 : kBN);
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (32 * b + 8 * (i / 4) + 4 * h + i % 4 >= last) s[b][i] = -INFINITY;
+    }
+
+    float top = s[0][0];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+    top = fmaxf(top, other_half(top));
+    if (__any((top - m) * c2 > 8.0f)) {
+      const float m2 = fmaxf(m, top);
+      const float r = m2 == -INFINITY ? 1.0f : exp2_hw((m - m2) * c2);
+      sum *= r;
+#pragma unroll
+      for (int d = 0; d < DB; ++d) o[d] *= r;
+      m = m2;
+    }
+    const float mc = m == -INFINITY ? 0.0f : m * c2;
+
+    X8 p[4];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float e = exp2_hw(__builtin_fmaf(s[b][i], c2, -mc));
+        sum += e;
+        p[2 * b + i / 8][i % 8] = static_cast<T>(e);
+      }
+
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const int chunk = 4 * d + 2 * g16 + ((t16 & 3) >> 1);
+        const char* p0 = vt + Ti::at(16 * x + vrow, chunk) + (t16 & 1) * 8;
+        const char* p1 = vt + Ti::at(16 * x + 8 + vrow, chunk) + (t16 & 1) * 8;
+        o[d] = E::mfma32(join<X8>(lds_read_tr(p0), lds_read_tr(p1)), p[x], o[d]);
+      }
+  };
+
+  if (tiles > 0) load_tile(0, lds);
+  for (int j = 0; j < tiles; ++j) {
+    wait_lds_loads();
+    __syncthreads();
+    work(j, lds + (j & 1) * 2 * kTileBytes, lds + ((j + 1) & 1) * 2 * kTileBytes);
+  }
+
+  sum += other_half(sum);
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  if (l >= rows) return;
+  store_columns<T, DP>(static_cast<T*>(a.out) + ((q_base + l) * a.H + head) * a.D, o, inv, a.D, h);
+  if (a.lse != nullptr && h == 0)
+    a.lse[head * a.Nq + q_base + l] = sum == 0.0f ? -INFINITY : m * a.scale + __logf(sum);
+}
+
+// ---------------------------------------------------------------------------
+// Backward
+// ---------------------------------------------------------------------------
+// With delta_i = dO_i.o_i and dP_ij = dO_i.v_j:
+//   dS_ij = p_ij (dP_ij - delta_i),
+//   dQ_i = scale sum_j dS_ij k_j,  dK_j = scale sum_i dS_ij q_i,  dV_j = sum_i p_ij dO_i,
+// the last two also over the query heads that share the key-value head.  Two
+// launches, each of which owns what it writes (no atomics: the same bits every
+// time): the first has the queries' tiles and leaves each query's delta and
+// base-2 lse for the second, which has the keys' tiles.  Scores are computed
+// in both, seven products where five would do, which is less than what summing
+// dQ over key tiles through memory costs.
+
+struct BwdArgs {
+  const char *q, *k, *v, *out, *grad;  // bytes; out and grad with q's shape
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, g_row, g_head;
+  const void *q_offsets, *k_offsets;
+  int64_t B, Nq, Nk;
+  int32_t H, Hkv, G, D;
+  int32_t causal;
+  float scale;
+  const float* lse;                    // [H, Nq]
+  float *lse2, *delta;                 // [H, Nq], workspace
+  void *dq, *dk, *dv;                  // contiguous
+};
+
+template <typename T, typename I, int DP, int NW>
+__global__ void __launch_bounds__(NW * 64, 2) bwd_q_kernel(const BwdArgs a, int64_t slots) {
+  using E = Elem<T>;
+  using X8 = typename E::x8;
+  using Ti = Tile<DP>;
+  constexpr int KS = DP / 16, DB = DP / 32, BM = NW * 32;
+  constexpr int kTileBytes = kBN * DP * 2;
+  __shared__ __attribute__((aligned(1024))) char lds[4 * kTileBytes];
+
+  int head;
+  int64_t slot, tile;
+  head_and_slot(blockIdx.x, a.H, slots, &head, &slot);
+  const I* qo = static_cast<const I*>(a.q_offsets);
+  const I* ko = static_cast<const I*>(a.k_offsets);
+  constexpr int kShift = NW == 1 ? 5 : NW == 2 ? 6 : NW == 4 ? 7 : 8;
+  const int64_t list = find_list(qo, a.B, a.Nq, kShift, slot, &tile);
+  const Span sq = list_span(qo, a.B, a.Nq, list);
+  if (tile * BM >= sq.len) return;
+  Span sk{0, 0};
+  if (list > 0 && list <= a.B) sk = list_span(ko, a.B, a.Nk, list);
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63, l = lane & 31, h = lane >> 5;
+  const int64_t row0 = uniform64(tile * BM + wave * 32);
+  const int64_t q_base = uniform64(sq.start + row0);
+  const int rows = static_cast<int>(sq.len - row0 < 32 ? (sq.len > row0 ? sq.len - row0 : 0) : 32);
+  const int64_t Lk = uniform64(sk.len);
+  const int64_t shift = uniform64(Lk - sq.len);
+  int64_t blk_end = Lk, wave_end = Lk;
+  if (a.causal) {
+    const int64_t last = (tile + 1) * BM < sq.len ? (tile + 1) * BM : sq.len;
+    blk_end = last + shift < Lk ? last + shift : Lk;
+    wave_end = row0 + rows + shift;
+  }
+  if (rows == 0) wave_end = 0;
+  const int tiles = blk_end > 0 ? static_cast<int>((blk_end + kBN - 1) / kBN) : 0;
+
+  X8 qf[KS], gf[KS];
+  load_rows<X8, KS>(qf, a.q + q_base * a.q_row + head * a.q_head, rows, a.q_row, a.D, l, h);
+  load_rows<X8, KS>(gf, a.grad + q_base * a.g_row + head * a.g_head, rows, a.g_row, a.D, l, h);
+  float delta = 0.0f, lse2 = 0.0f;
+  {
+    X8 of[KS];
+    load_rows<X8, KS>(of, a.out + q_base * a.o_row + head * a.o_head, rows, a.o_row, a.D, l, h);
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        delta = __builtin_fmaf(static_cast<float>(of[s][e]), static_cast<float>(gf[s][e]), delta);
+    delta += other_half(delta);
+    if (l < rows) {
+      const int64_t at = head * a.Nq + q_base + l;
+      lse2 = a.lse[at] * kLog2e;
+      if (h == 0) {
+        a.lse2[at] = lse2;
+        a.delta[at] = delta;
+      }
+    }
+  }
+
+  typename Ti::template Loader<kBN, NW * 64> lk, lv;
+  lk.init(tid, static_cast<uint32_t>(a.k_row), a.D / 8);
+  lv.init(tid, static_cast<uint32_t>(a.v_row), a.D / 8);
+  const char* kp = a.k + uniform64(sk.start) * a.k_row + (head / a.G) * a.k_head;
+  const char* vp = a.v + uniform64(sk.start) * a.v_row + (head / a.G) * a.v_head;
+
+  f32x16 dq[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) dq[d] = f32x16{};
+  const float c2 = a.scale * kLog2e;
+  const int t16 = lane & 15, g16 = (lane >> 4) & 1;
+  const int trow = 4 * h + (t16 >> 2);
+
+  auto load_tile = [&](int j, char* __restrict__ dst) __attribute__((always_inline)) {
+    const int64_t left = Lk - static_cast<int64_t>(j) * kBN;
+    const int n = left < kBN ? static_cast<int>(left) : kBN;
+    lk.load(make_rsrc(kp + static_cast<int64_t>(j) * kBN * a.k_row,
+                      span_bytes(n, static_cast<uint32_t>(a.k_row), a.D * 2)), dst, wave);
+    lv.load(make_rsrc(vp + static_cast<int64_t>(j) * kBN * a.v_row,
+                      span_bytes(n, static_cast<uint32_t>(a.v_row), a.D * 2)),
+            dst + kTileBytes, wave);
+  };
+  auto work = [&](int j, const char* __restrict__ kt, char* __restrict__ next) __attribute__((always_inline)) {
+    if (j + 1 < tiles) load_tile(j + 1, next);
+    const char* vt = kt + kTileBytes;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int64_t k0 = static_cast<int64_t>(j) * kBN + 32 * b;
+      if (k0 >= wave_end) return;
+      f32x16 s{}, dp{};
+#pragma unroll
+      for (int x = 0; x < KS; ++x) {
+        s = E::mfma32(lds_read16<X8>(kt + Ti::at(32 * b + l, 2 * x + h)), qf[x], s);
+        dp = E::mfma32(lds_read16<X8>(vt + Ti::at(32 * b + l, 2 * x + h)), gf[x], dp);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = exp2_hw(__builtin_fmaf(s[i], c2, -lse2));
+      const int64_t end0 = a.causal ? row0 + shift + 1 : Lk;
+      if (k0 + 32 > end0 || k0 + 32 > Lk) {
+        const int64_t mine = a.causal ? row0 + l + shift + 1 : Lk;
+        const int64_t lim = (mine < Lk ? mine : Lk) - k0;
+        const int last = lim < 32 ? (lim > 0 ? static_cast<int>(lim) : 0) : 32;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const bool hidden = 8 * (i / 4) + 4 * h + i % 4 >= last;
+          s[i] = hidden ? 0.0f : s[i];
+          dp[i] = hidden ? 0.0f : dp[i];
+        }
+      }
+      X8 ds[2];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) ds[i / 8][i % 8] = static_cast<T>(s[i] * (dp[i] - delta));
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          const int chunk = 4 * d + 2 * g16 + ((t16 & 3) >> 1);
+          const char* p0 = kt + Ti::at(32 * b + 16 * x + trow, chunk) + (t16 & 1) * 8;
+          const char* p1 = kt + Ti::at(32 * b + 16 * x + 8 + trow, chunk) + (t16 & 1) * 8;
+          dq[d] = E::mfma32(join<X8>(lds_read_tr(p0), lds_read_tr(p1)), ds[x], dq[d]);
+        }
+    }
+  };
+
+  if (tiles > 0) load_tile(0, lds);
+  for (int j = 0; j < tiles; ++j) {
+    wait_lds_loads();
+    __syncthreads();
+    work(j, lds + (j & 1) * 2 * kTileBytes, lds + ((j + 1) & 1) * 2 * kTileBytes);
+  }
+  if (l >= rows) return;
+  store_columns<T, DP>(static_cast<T*>(a.dq) + ((q_base + l) * a.H + head) * a.D, dq, a.scale, a.D, h);
+}
+
+// The keys' launch: a wave owns 32 keys and their sums over every query head of
+// the group and every query that sees them.  Queries and dO go through LDS in
+// tiles of 64 with their lse and delta; scores come out with a key per lane.
+template <typename T, typename I, int DP, int NW>
+__global__ void __launch_bounds__(NW * 64, 1) bwd_kv_kernel(const BwdArgs a, int64_t slots) {
+  using E = Elem<T>;
+  using X8 = typename E::x8;
+  using Ti = Tile<DP>;
+  constexpr int KS = DP / 16, DB = DP / 32, BM = NW * 32, BQ = 64;
+  constexpr int kTileBytes = BQ * DP * 2;
+  constexpr int kStat = BQ * 4;
+  constexpr int kBuf = 2 * kTileBytes + 2 * kStat;  // Q, dO, lse2, delta
+  __shared__ __attribute__((aligned(1024))) char lds[2 * kBuf];
+
+  int kvh;
+  int64_t slot, tile;
+  head_and_slot(blockIdx.x, a.Hkv, slots, &kvh, &slot);
+  const I* qo = static_cast<const I*>(a.q_offsets);
+  const I* ko = static_cast<const I*>(a.k_offsets);
+  constexpr int kShift = NW == 1 ? 5 : NW == 2 ? 6 : NW == 4 ? 7 : 8;
+  const int64_t list = find_list(ko, a.B, a.Nk, kShift, slots - 1 - slot, &tile);
+  const Span sk = list_span(ko, a.B, a.Nk, list);
+  if (tile * BM >= sk.len) return;
+  Span sq{0, 0};
+  if (list > 0 && list <= a.B) sq = list_span(qo, a.B, a.Nq, list);
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63, l = lane & 31, h = lane >> 5;
+  const int64_t key0 = uniform64(tile * BM + wave * 32);
+  const int64_t k_base = uniform64(sk.start + key0);
+  const int keys = static_cast<int>(sk.len - key0 < 32 ? (sk.len > key0 ? sk.len - key0 : 0) : 32);
+  const int64_t Lq = uniform64(sq.len);
+  const int64_t shift = uniform64(sk.len - sq.len);
+  // First query that sees a key of the block, to a whole tile.
+  int64_t first = 0;
+  if (a.causal) first = tile * BM - shift > 0 ? tile * BM - shift : 0;
+  const int64_t t0 = first / BQ;
+  const int64_t t1 = (Lq + BQ - 1) / BQ;
+  const int per = t1 > t0 ? static_cast<int>(t1 - t0) : 0;
+  const int steps = per * a.G;
+
+  X8 kf[KS], vf[KS];
+  load_rows<X8, KS>(kf, a.k + k_base * a.k_row + kvh * a.k_head, keys, a.k_row, a.D, l, h);
+  load_rows<X8, KS>(vf, a.v + k_base * a.v_row + kvh * a.v_head, keys, a.v_row, a.D, l, h);
+
+  typename Ti::template Loader<BQ, NW * 64> lq, lg;
+  lq.init(tid, static_cast<uint32_t>(a.q_row), a.D / 8);
+  lg.init(tid, static_cast<uint32_t>(a.g_row), a.D / 8);
+  const int64_t qs = uniform64(sq.start);
+
+  f32x16 dk[DB], dv[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) dk[d] = dv[d] = f32x16{};
+  const float c2 = a.scale * kLog2e;
+  const int t16 = lane & 15, g16 = (lane >> 4) & 1;
+  const int trow = 4 * h + (t16 >> 2);
+
+  auto load_tile = [&](int g, int t, char* __restrict__ dst) __attribute__((always_inline)) {
+    const int head = kvh * a.G + g;
+    const int64_t i0 = (t0 + t) * BQ;
+    const int n = Lq - i0 < BQ ? static_cast<int>(Lq - i0) : BQ;
+    lq.load(make_rsrc(a.q + (qs + i0) * a.q_row + head * a.q_head,
+                      span_bytes(n, static_cast<uint32_t>(a.q_row), a.D * 2)), dst, wave);
+    lg.load(make_rsrc(a.grad + (qs + i0) * a.g_row + head * a.g_head,
+                      span_bytes(n, static_cast<uint32_t>(a.g_row), a.D * 2)),
+            dst + kTileBytes, wave);
+    if (wave < 2) {
+      const float* st = (wave == 0 ? a.lse2 : a.delta) + head * a.Nq + qs + i0;
+      load4_to_lds(make_rsrc(st, n * 4), dst + 2 * kTileBytes + wave * kStat, lane * 4);
+    }
+  };
+  auto work = [&](int t, const char* __restrict__ qt, char* __restrict__ next, int gn, int tn,
+                  bool more) __attribute__((always_inline)) {
+    if (more) load_tile(gn, tn, next);
+    const char* gt = qt + kTileBytes;
+    const char* st = qt + 2 * kTileBytes;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int64_t i0 = (t0 + t) * BQ + 32 * b;
+      if (keys == 0 || i0 >= Lq) return;
+      if (a.causal && key0 > i0 + 31 + shift) continue;
+      f32x16 s{}, dp{};
+#pragma unroll
+      for (int x = 0; x < KS; ++x) {
+        s = E::mfma32(lds_read16<X8>(qt + Ti::at(32 * b + l, 2 * x + h)), kf[x], s);
+        dp = E::mfma32(lds_read16<X8>(gt + Ti::at(32 * b + l, 2 * x + h)), vf[x], dp);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const f32x4 ls = *reinterpret_cast<const f32x4*>(st + (32 * b + 8 * u + 4 * h) * 4);
+        const f32x4 de = *reinterpret_cast<const f32x4*>(st + kStat + (32 * b + 8 * u + 4 * h) * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[4 * u + e] = exp2_hw(__builtin_fmaf(s[4 * u + e], c2, -ls[e]));
+          dp[4 * u + e] -= de[e];
+        }
+      }
+      if (a.causal && key0 + 31 > i0 + shift) {
+        // Query i0 + r sees key0 + l if r >= key0 + l - shift - i0.
+        const int64_t lim = key0 + l - shift - i0;
+        const int from = lim > 0 ? (lim < 32 ? static_cast<int>(lim) : 32) : 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const bool hidden = 8 * (i / 4) + 4 * h + i % 4 < from;
+          s[i] = hidden ? 0.0f : s[i];
+          dp[i] = hidden ? 0.0f : dp[i];
+        }
+      }
+      X8 p[2], ds[2];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        p[i / 8][i % 8] = static_cast<T>(s[i]);
+        ds[i / 8][i % 8] = static_cast<T>(s[i] * dp[i]);
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          const int chunk = 4 * d + 2 * g16 + ((t16 & 3) >> 1);
+          const int o0 = Ti::at(32 * b + 16 * x + trow, chunk) + (t16 & 1) * 8;
+          const int o1 = Ti::at(32 * b + 16 * x + 8 + trow, chunk) + (t16 & 1) * 8;
+          dv[d] = E::mfma32(join<X8>(lds_read_tr(gt + o0), lds_read_tr(gt + o1)), p[x], dv[d]);
+          dk[d] = E::mfma32(join<X8>(lds_read_tr(qt + o0), lds_read_tr(qt + o1)), ds[x], dk[d]);
+        }
+    }
+  };
+
+  if (steps > 0) load_tile(0, 0, lds);
+  int g = 0, t = 0;
+  for (int i = 0; i < steps; ++i) {
+    const int tn = t + 1 < per ? t + 1 : 0, gn = t + 1 < per ? g : g + 1;
+    wait_lds_loads();
+    __syncthreads();
+    work(t, lds + (i & 1) * kBuf, lds + ((i + 1) & 1) * kBuf, gn, tn, i + 1 < steps);
+    t = tn;
+    g = gn;
+  }
+  if (l >= keys) return;
+  const int64_t at = ((k_base + l) * a.Hkv + kvh) * a.D;
+  store_columns<T, DP>(static_cast<T*>(a.dk) + at, dk, a.scale, a.D, h);
+  store_columns<T, DP>(static_cast<T*>(a.dv) + at, dv, 1.0f, a.D, h);
+}
+
+// ---------------------------------------------------------------------------
+// Launches
+// ---------------------------------------------------------------------------
+
+template <typename T, typename I, int DP>
+int launch_fwd(const FwdArgs& a, hipStream_t stream) {
+  constexpr int NW = 4;
+  const int64_t slots = tile_slots(a.Nq, a.B, NW * 32);
+  MX_REQUIRE(slots * a.H < (1ll << 31), "too many query tiles: %lld", (long long)(slots * a.H));
+  fwd_kernel<T, I, DP, NW><<<dim3(static_cast<unsigned>(slots * a.H)), NW * 64, 0, stream>>>(a, slots);
+  MX_LAUNCH_CHECK();
+  return MX_OK;
+}
+
+template <typename T, typename I, int DP>
+int launch_bwd(const BwdArgs& a, hipStream_t stream) {
+  constexpr int NW = 4;
+  const int64_t qslots = tile_slots(a.Nq, a.B, NW * 32), kslots = tile_slots(a.Nk, a.B, NW * 32);
+  MX_REQUIRE(qslots * a.H < (1ll << 31) && kslots * a.Hkv < (1ll << 31), "too many tiles: %lld",
+             (long long)(qslots * a.H));
+  if (a.Nq > 0)
+    bwd_q_kernel<T, I, DP, NW><<<dim3(static_cast<unsigned>(qslots * a.H)), NW * 64, 0, stream>>>(a, qslots);
+  if (a.Nk > 0 && a.dk != nullptr)
+    bwd_kv_kernel<T, I, DP, NW><<<dim3(static_cast<unsigned>(kslots * a.Hkv)), NW * 64, 0, stream>>>(a, kslots);
+  MX_LAUNCH_CHECK();
+  return MX_OK;
+}
+
+// The instance of a call: element type, index type, and the head width rounded
+// up to 32 (zeros fill the rest of a tile's rows).
+#define MX_ATTN_DISPATCH(LAUNCH, T, args, index_bytes, stream)                          \
+  (index_bytes == 8 ? ((args).D <= 32   ? LAUNCH<T, int64_t, 32>(args, stream)          \
+                       : (args).D <= 64 ? LAUNCH<T, int64_t, 64>(args, stream)          \
+                       : (args).D <= 96 ? LAUNCH<T, int64_t, 96>(args, stream)          \
+                                        : LAUNCH<T, int64_t, 128>(args, stream))        \
+                    : ((args).D <= 32   ? LAUNCH<T, int32_t, 32>(args, stream)          \
+                       : (args).D <= 64 ? LAUNCH<T, int32_t, 64>(args, stream)          \
+                       : (args).D <= 96 ? LAUNCH<T, int32_t, 96>(args, stream)          \
+                                        : LAUNCH<T, int32_t, 128>(args, stream)))
+
+// One strided [N, heads, D] operand: its strides in bytes, checked for what
+// the kernels assume (16-byte rows; 64 rows of a tile within a descriptor).
+int check_operand(const char* name, const mx_attention_tensor* t, int32_t D, int64_t N) {
+  MX_REQUIRE(t != nullptr && (N == 0 || t->data != nullptr), "%s is null", name);
+  MX_REQUIRE(reinterpret_cast<uintptr_t>(t->data) % 16 == 0 && t->row_stride % 8 == 0 &&
+                 t->head_stride % 8 == 0,
+             "%s: rows and heads must start at multiples of 16 bytes", name);
+  MX_REQUIRE(t->row_stride >= D || N <= 1, "%s: row stride %lld below D = %d", name,
+             (long long)t->row_stride, D);
+  MX_REQUIRE(t->row_stride <= (1ll << 23), "%s: row stride %lld above 2^23 elements", name,
+             (long long)t->row_stride);
+  MX_REQUIRE(t->head_stride >= 0, "%s: negative head stride", name);
+  return MX_OK;
+}
+
+int check_problem(const mx_attention_problem* p) {
+  MX_REQUIRE(p != nullptr, "problem is null");
+  MX_REQUIRE(p->dtype == MX_DTYPE_F16 || p->dtype == MX_DTYPE_BF16, "dtype %d is not fp16 or bf16", p->dtype);
+  MX_REQUIRE(p->index_bytes == 4 || p->index_bytes == 8, "index_bytes %d", p->index_bytes);
+  MX_REQUIRE(p->B >= 0 && p->Nq >= 0 && p->Nk >= 0, "negative size");
+  MX_REQUIRE(p->H > 0 && p->Hkv > 0 && p->H % p->Hkv == 0,
+             "%d query heads are no multiple of %d key-value heads", p->H, p->Hkv);
+  MX_REQUIRE(p->D > 0 && p->D <= MX_ATTENTION_MAX_D && p->D % 8 == 0,
+             "head width %d is no multiple of 8 up to %d", p->D, MX_ATTENTION_MAX_D);
+  MX_REQUIRE(std::isfinite(p->scale) && p->scale > 0.0f, "scale must be positive and finite");
+  MX_REQUIRE(p->B == 0 || (p->q_offsets != nullptr && p->k_offsets != nullptr), "offsets are null");
+  return MX_OK;
+}
+
+}  // namespace
+}  // namespace attn
+}  // namespace mx
+
+extern "C" int mx_jagged_attention_forward(const mx_attention_problem* p, const mx_attention_tensor* q,
+                                           const mx_attention_tensor* k, const mx_attention_tensor* v,
+                                           void* out, float* lse, void* stream) {
+  using namespace mx::attn;
+  mx::clear_error();
+  if (int rc = check_problem(p)) return rc;
+  if (int rc = check_operand("q", q, p->D, p->Nq)) return rc;
+  if (int rc = check_operand("k", k, p->D, p->Nk)) return rc;
+  if (int rc = check_operand("v", v, p->D, p->Nk)) return rc;
+  if (p->Nq == 0) return MX_OK;
+  MX_REQUIRE(out != nullptr && reinterpret_cast<uintptr_t>(out) % 16 == 0, "out must be 16-byte aligned");
+  FwdArgs a{};
+  a.q = static_cast<const char*>(q->data);
+  a.k = static_cast<const char*>(k->data);
+  a.v = static_cast<const char*>(v->data);
+  a.q_row = q->row_stride * 2, a.q_head = q->head_stride * 2;
+  a.k_row = k->row_stride * 2, a.k_head = k->head_stride * 2;
+  a.v_row = v->row_stride * 2, a.v_head = v->head_stride * 2;
+  a.q_offsets = p->q_offsets, a.k_offsets = p->k_offsets;
+  a.B = p->B, a.Nq = p->Nq, a.Nk = p->Nk;
+  a.H = p->H, a.G = p->H / p->Hkv, a.D = p->D;
+  a.causal = p->causal, a.scale = p->scale;
+  a.out = out, a.lse = lse;
+  const hipStream_t s = mx::as_stream(stream);
+  return p->dtype == MX_DTYPE_BF16 ? MX_ATTN_DISPATCH(launch_fwd, __bf16, a, p->index_bytes, s)
+                                   : MX_ATTN_DISPATCH(launch_fwd, _Float16, a, p->index_bytes, s);
+}
+
+extern "C" size_t mx_jagged_attention_backward_workspace_bytes(int64_t Nq, int32_t H) {
+  return Nq > 0 && H > 0 ? static_cast<size_t>(Nq) * H * 2 * sizeof(float) : 0;
+}
+
+extern "C" int mx_jagged_attention_backward(const mx_attention_problem* p, const mx_attention_tensor* q,
+                                            const mx_attention_tensor* k, const mx_attention_tensor* v,
+                                            const mx_attention_tensor* out,
+                                            const mx_attention_tensor* grad_out, const float* lse,
+                                            void* dq, void* dk, void* dv, void* workspace,
+                                            size_t workspace_bytes, void* stream) {
+  using namespace mx::attn;
+  mx::clear_error();
+  if (int rc = check_problem(p)) return rc;
+  if (int rc = check_operand("q", q, p->D, p->Nq)) return rc;
+  if (int rc = check_operand("k", k, p->D, p->Nk)) return rc;
+  if (int rc = check_operand("v", v, p->D, p->Nk)) return rc;
+  if (int rc = check_operand("out", out, p->D, p->Nq)) return rc;
+  if (int rc = check_operand("grad_out", grad_out, p->D, p->Nq)) return rc;
+  MX_REQUIRE(p->Nq == 0 || (dq != nullptr && lse != nullptr), "dq or lse is null");
+  MX_REQUIRE((dk == nullptr) == (dv == nullptr), "dk and dv: both or neither");
+  for (const void* x : {dq, dk, dv})
+    MX_REQUIRE(reinterpret_cast<uintptr_t>(x) % 16 == 0, "gradients must be 16-byte aligned");
+  const size_t need = mx_jagged_attention_backward_workspace_bytes(p->Nq, p->H);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return mx::set_error(MX_EWORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  BwdArgs a{};
+  a.q = static_cast<const char*>(q->data);
+  a.k = static_cast<const char*>(k->data);
+  a.v = static_cast<const char*>(v->data);
+  a.out = static_cast<const char*>(out->data);
+  a.grad = static_cast<const char*>(grad_out->data);
+  a.q_row = q->row_stride * 2, a.q_head = q->head_stride * 2;
+  a.k_row = k->row_stride * 2, a.k_head = k->head_stride * 2;
+  a.v_row = v->row_stride * 2, a.v_head = v->head_stride * 2;
+  a.o_row = out->row_stride * 2, a.o_head = out->head_stride * 2;
+  a.g_row = grad_out->row_stride * 2, a.g_head = grad_out->head_stride * 2;
+  a.q_offsets = p->q_offsets, a.k_offsets = p->k_offsets;
+  a.B = p->B, a.Nq = p->Nq, a.Nk = p->Nk;
+  a.H = p->H, a.Hkv = p->Hkv, a.G = p->H / p->Hkv, a.D = p->D;
+  a.causal = p->causal, a.scale = p->scale;
+  a.lse = lse;
+  a.lse2 = static_cast<float*>(workspace);
+  a.delta = a.lse2 + p->Nq * p->H;
+  a.dq = dq, a.dk = dk, a.dv = dv;
+  const hipStream_t s = mx::as_stream(stream);
+  return p->dtype == MX_DTYPE_BF16 ? MX_ATTN_DISPATCH(launch_bwd, __bf16, a, p->index_bytes, s)
+                                   : MX_ATTN_DISPATCH(launch_bwd, _Float16, a, p->index_bytes, s);
+}

@@ -23,6 +23,7 @@
 
 #include <algorithm>
 #include <array>
+#include <cmath>
 #include <cstring>
 #include <mutex>
 #include <vector>
@@ -1923,6 +1924,301 @@ Tensor expand_into_jagged_permute(const Tensor& permute, const Tensor& input_off
   return out;
 }
 
+// ---------------------------------------------------------------------------
+// Attention over packed sequences and its paged cache
+// ---------------------------------------------------------------------------
+
+bool attention_ready(const Tensor& t) {
+  const int64_t rows = t.size(0), heads = t.size(1), D = t.size(2);
+  return t.stride(2) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
+         (rows <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= D && t.stride(0) <= (1ll << 23))) &&
+         (heads <= 1 || (t.stride(1) % 8 == 0 && t.stride(1) >= 0));
+}
+
+// A [rows, heads, D] tensor as the kernels take it: in place if its rows and
+// heads start at 16-byte boundaries (views of a fused projection do), else
+// through a copy kept in `keep`.
+mx_attention_tensor attention_operand(const Tensor& t, Tensor& keep) {
+  keep = attention_ready(t) ? t : t.clone(at::MemoryFormat::Contiguous);
+  const int64_t D = keep.size(2), heads = keep.size(1);
+  return {keep.data_ptr(), keep.size(0) > 1 ? keep.stride(0) : heads * D, heads > 1 ? keep.stride(1) : D};
+}
+
+void check_rows(const Tensor& t, const Tensor& like, const char* name) {
+  check_arg(t, like, name, false);
+  TORCH_CHECK(t.dim() == 3, name, " must be [rows, heads, D], got ", t.sizes());
+  TORCH_CHECK(t.scalar_type() == like.scalar_type(), name, " is ", t.scalar_type(), " but expected ",
+              like.scalar_type());
+}
+
+int32_t attention_dtype(const Tensor& t, const char* name) {
+  TORCH_CHECK(t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16, name,
+              " must be float16 or bfloat16, got ", t.scalar_type());
+  return mx_dtype_of(t.scalar_type());
+}
+
+void check_head_width(int64_t D) {
+  TORCH_CHECK(D >= 8 && D <= MX_ATTENTION_MAX_D && D % 8 == 0,
+              "the head width must be a multiple of 8 up to ", MX_ATTENTION_MAX_D, ", got ", D);
+}
+
+float attention_scale(std::optional<double> scale, int64_t D) {
+  const double s = scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(D));
+  TORCH_CHECK(std::isfinite(s) && s > 0.0 && static_cast<float>(s) > 0.0f && std::isfinite(static_cast<float>(s)),
+              "scale must be positive and finite, got ", s);
+  return static_cast<float>(s);
+}
+
+struct AttentionCall {
+  mx_attention_problem p{};
+  mx_attention_tensor q{}, k{}, v{};
+  std::array<Tensor, 5> keep;  // operands and offsets
+};
+
+void pack_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_offsets,
+                    const std::optional<Tensor>& k_offsets, bool causal,
+                    std::optional<double> scale, AttentionCall& c) {
+  check_rows(q, q, "q");
+  check_rows(k, q, "k");
+  check_rows(v, q, "v");
+  c.p.dtype = attention_dtype(q, "q");
+  const int64_t D = q.size(2);
+  check_head_width(D);
+  TORCH_CHECK(k.sizes() == v.sizes(), "k ", k.sizes(), " and v ", v.sizes(), " must have one shape");
+  TORCH_CHECK(k.size(2) == D, "k has head width ", k.size(2), " but q has ", D);
+  TORCH_CHECK(q.size(1) > 0 && k.size(1) > 0 && q.size(1) % k.size(1) == 0, "q has ", q.size(1),
+              " heads, which is no multiple of the ", k.size(1), " key-value heads");
+  TORCH_CHECK(q.size(1) < (1 << 20), "too many heads: ", q.size(1));
+  const Tensor& ko = k_offsets.has_value() && k_offsets->defined() ? *k_offsets : q_offsets;
+  for (const Tensor* o : {&q_offsets, &ko}) {
+    const char* name = o == &q_offsets ? "q_offsets" : "k_offsets";
+    check_arg(*o, q, name, false);
+    TORCH_CHECK(o->dim() == 1 && o->numel() >= 1, name, " must be 1-D with at least one entry");
+  }
+  c.p.index_bytes = index_bytes_of(q_offsets, "q_offsets");
+  TORCH_CHECK(index_bytes_of(ko, "k_offsets") == c.p.index_bytes, "q_offsets and k_offsets must share one dtype");
+  TORCH_CHECK(ko.numel() == q_offsets.numel(), "q_offsets has ", q_offsets.numel(),
+              " entries but k_offsets ", ko.numel());
+  TORCH_CHECK(k_offsets.has_value() || k.size(0) == q.size(0), "without k_offsets, k must have q's ",
+              q.size(0), " rows, got ", k.size(0));
+  c.keep[3] = q_offsets.contiguous();
+  c.keep[4] = ko.contiguous();
+  c.p.q_offsets = c.keep[3].data_ptr();
+  c.p.k_offsets = c.keep[4].data_ptr();
+  c.p.B = q_offsets.numel() - 1;
+  c.p.Nq = q.size(0);
+  c.p.Nk = k.size(0);
+  c.p.H = static_cast<int32_t>(q.size(1));
+  c.p.Hkv = static_cast<int32_t>(k.size(1));
+  c.p.D = static_cast<int32_t>(D);
+  c.p.causal = causal ? 1 : 0;
+  c.p.scale = attention_scale(scale, D);
+  c.q = attention_operand(q, c.keep[0]);
+  c.k = attention_operand(k, c.keep[1]);
+  c.v = attention_operand(v, c.keep[2]);
+}
+
+Tensor run_jagged_attention(const Tensor& q, const Tensor& k, const Tensor& v,
+                            const Tensor& q_offsets, const std::optional<Tensor>& k_offsets,
+                            bool causal, std::optional<double> scale, Tensor* lse) {
+  check_gpu(q, "q");
+  c10::OptionalDeviceGuard guard(q.device());
+  AttentionCall c;
+  pack_attention(q, k, v, q_offsets, k_offsets, causal, scale, c);
+  Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+  if (lse != nullptr) *lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
+  MX_CALL(mx_jagged_attention_forward(&c.p, &c.q, &c.k, &c.v, out.data_ptr(),
+                                      lse != nullptr ? lse->data_ptr<float>() : nullptr, stream_of(q)));
+  return out;
+}
+
+Tensor jagged_attention_plain(const Tensor& q, const Tensor& k, const Tensor& v,
+                              const Tensor& q_offsets, const std::optional<Tensor>& k_offsets,
+                              bool causal, std::optional<double> scale) {
+  return run_jagged_attention(q, k, v, q_offsets, k_offsets, causal, scale, nullptr);
+}
+
+std::tuple<Tensor, Tensor> jagged_attention_forward(const Tensor& q, const Tensor& k, const Tensor& v,
+                                                    const Tensor& q_offsets,
+                                                    const std::optional<Tensor>& k_offsets,
+                                                    bool causal, std::optional<double> scale) {
+  Tensor lse;
+  Tensor out = run_jagged_attention(q, k, v, q_offsets, k_offsets, causal, scale, &lse);
+  return {out, lse};
+}
+
+// (dq, dk, dv); dk and dv undefined unless `need_kv`.
+std::tuple<Tensor, Tensor, Tensor> run_jagged_attention_backward(
+    const Tensor& grad_output, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out,
+    const Tensor& lse, const Tensor& q_offsets, const std::optional<Tensor>& k_offsets, bool causal,
+    std::optional<double> scale, bool need_kv) {
+  check_gpu(q, "q");
+  c10::OptionalDeviceGuard guard(q.device());
+  AttentionCall c;
+  pack_attention(q, k, v, q_offsets, k_offsets, causal, scale, c);
+  check_rows(out, q, "out");
+  check_rows(grad_output, q, "grad_output");
+  TORCH_CHECK(out.sizes() == q.sizes(), "out ", out.sizes(), " must have q's shape ", q.sizes());
+  TORCH_CHECK(grad_output.sizes() == q.sizes(), "grad_output ", grad_output.sizes(),
+              " must have q's shape ", q.sizes());
+  check_arg(lse, q, "lse", true);
+  TORCH_CHECK(lse.scalar_type() == at::kFloat && lse.dim() == 2 && lse.size(0) == q.size(1) &&
+                  lse.size(1) == q.size(0),
+              "lse must be float32 [", q.size(1), ", ", q.size(0), "]");
+  Tensor keep_out, keep_grad;
+  const mx_attention_tensor o = attention_operand(out, keep_out);
+  const mx_attention_tensor g = attention_operand(grad_output, keep_grad);
+  const auto opts = q.options().memory_format(at::MemoryFormat::Contiguous);
+  Tensor dq = at::empty(q.sizes(), opts), dk, dv;
+  if (need_kv) {
+    dk = at::empty(k.sizes(), opts);
+    dv = at::empty(k.sizes(), opts);
+  }
+  const size_t ws_bytes = mx_jagged_attention_backward_workspace_bytes(q.size(0), c.p.H);
+  Tensor ws = at::empty({static_cast<int64_t>(ws_bytes)}, q.options().dtype(at::kByte));
+  MX_CALL(mx_jagged_attention_backward(
+      &c.p, &c.q, &c.k, &c.v, &o, &g, lse.data_ptr<float>(), dq.data_ptr(),
+      need_kv ? dk.data_ptr() : nullptr, need_kv ? dv.data_ptr() : nullptr, ws.data_ptr(), ws_bytes,
+      stream_of(q)));
+  return {dq, dk, dv};
+}
+
+std::tuple<Tensor, Tensor, Tensor> jagged_attention_backward(
+    const Tensor& grad_output, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out,
+    const Tensor& lse, const Tensor& q_offsets, const std::optional<Tensor>& k_offsets, bool causal,
+    std::optional<double> scale) {
+  return run_jagged_attention_backward(grad_output, q, k, v, out, lse, q_offsets, k_offsets, causal,
+                                       scale, true);
+}
+
+class JaggedAttention : public torch::autograd::Function<JaggedAttention> {
+ public:
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
+                        const Tensor& q_offsets, const std::optional<Tensor>& k_offsets,
+                        bool causal, std::optional<double> scale) {
+    at::AutoDispatchBelowADInplaceOrView g;
+    Tensor lse;
+    Tensor out = run_jagged_attention(q, k, v, q_offsets, k_offsets, causal, scale, &lse);
+    ctx->save_for_backward({q, k, v, out, lse, q_offsets,
+                            k_offsets.has_value() && k_offsets->defined() ? *k_offsets : q_offsets});
+    ctx->saved_data["causal"] = causal;
+    ctx->saved_data["scale"] = static_cast<double>(attention_scale(scale, q.size(2)));
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(),
+                "jagged_attention has no second derivative (backward ran with create_graph=True)");
+    variable_list r(7);  // q, k, v, q_offsets, k_offsets, causal, scale
+    if (!grads[0].defined()) return r;
+    const auto s = ctx->get_saved_variables();
+    const bool need_kv = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
+    auto [dq, dk, dv] = run_jagged_attention_backward(
+        grads[0], s[0], s[1], s[2], s[3], s[4], s[5], s[6], ctx->saved_data["causal"].toBool(),
+        ctx->saved_data["scale"].toDouble(), need_kv);
+    if (ctx->needs_input_grad(0)) r[0] = dq;
+    if (ctx->needs_input_grad(1)) r[1] = dk;
+    if (ctx->needs_input_grad(2)) r[2] = dv;
+    return r;
+  }
+};
+
+Tensor jagged_attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v,
+                                 const Tensor& q_offsets, const std::optional<Tensor>& k_offsets,
+                                 bool causal, std::optional<double> scale) {
+  if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
+    return JaggedAttention::apply(q, k, v, q_offsets, k_offsets, causal, scale);
+  at::AutoDispatchBelowADInplaceOrView g;
+  return jagged_attention_plain(q, k, v, q_offsets, k_offsets, causal, scale);
+}
+
+mx_paged_cache pack_cache(const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table) {
+  check_gpu(k_cache, "k_cache");
+  check_arg(v_cache, k_cache, "v_cache", false);
+  check_arg(page_table, k_cache, "page_table", false);
+  attention_dtype(k_cache, "k_cache");
+  TORCH_CHECK(k_cache.dim() == 4, "k_cache must be [pages, page_size, heads, D], got ", k_cache.sizes());
+  TORCH_CHECK(k_cache.sizes() == v_cache.sizes() && k_cache.scalar_type() == v_cache.scalar_type(),
+              "k_cache and v_cache must have one shape and type");
+  check_head_width(k_cache.size(3));
+  TORCH_CHECK(k_cache.size(1) >= 1 && k_cache.size(1) < (1ll << 31) && k_cache.size(2) >= 1,
+              "page_size and heads must be positive, got ", k_cache.sizes());
+  for (const Tensor* t : {&k_cache, &v_cache})
+    TORCH_CHECK(t->stride(3) == 1 && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0 &&
+                    t->stride(0) % 8 == 0 && t->stride(1) % 8 == 0 && t->stride(2) % 8 == 0,
+                "the caches' rows must be contiguous and start at multiples of 16 bytes, got strides ",
+                t->strides());
+  TORCH_CHECK(page_table.scalar_type() == at::kInt && page_table.dim() == 2 &&
+                  (page_table.size(1) <= 1 || page_table.stride(1) == 1),
+              "page_table must be int32 [sequences, pages of a sequence] with contiguous rows");
+  mx_paged_cache c{};
+  c.k = k_cache.data_ptr();
+  c.v = v_cache.data_ptr();
+  c.k_page_stride = k_cache.stride(0), c.k_slot_stride = k_cache.stride(1), c.k_head_stride = k_cache.stride(2);
+  c.v_page_stride = v_cache.stride(0), c.v_slot_stride = v_cache.stride(1), c.v_head_stride = v_cache.stride(2);
+  c.pages = k_cache.size(0);
+  c.page_size = static_cast<int32_t>(k_cache.size(1));
+  c.table = page_table.data_ptr<int32_t>();
+  c.table_row_stride = page_table.stride(0);
+  c.table_width = page_table.size(1);
+  return c;
+}
+
+void paged_cache_append(const Tensor& k, const Tensor& v, const Tensor& offsets, const Tensor& starts,
+                        const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table) {
+  check_gpu(k, "k");
+  c10::OptionalDeviceGuard guard(k.device());
+  check_arg(k_cache, k, "k_cache", false);
+  const mx_paged_cache c = pack_cache(k_cache, v_cache, page_table);
+  check_rows(k, k_cache, "k");
+  check_rows(v, k_cache, "v");
+  TORCH_CHECK(k.sizes() == v.sizes(), "k ", k.sizes(), " and v ", v.sizes(), " must have one shape");
+  TORCH_CHECK(k.size(1) == k_cache.size(2) && k.size(2) == k_cache.size(3), "k is ", k.sizes(),
+              " but the cache holds ", k_cache.size(2), " heads of ", k_cache.size(3));
+  check_arg(offsets, k, "offsets", true);
+  check_arg(starts, k, "starts", true);
+  const int64_t B = page_table.size(0);
+  TORCH_CHECK(offsets.dim() == 1 && offsets.numel() == B + 1, "offsets must have ", B + 1, " entries, got ",
+              offsets.sizes());
+  TORCH_CHECK(starts.dim() == 1 && starts.numel() == B, "starts must have ", B, " entries, got ", starts.sizes());
+  Tensor kk, kv;
+  const mx_attention_tensor ko = attention_operand(k, kk), vo = attention_operand(v, kv);
+  MX_CALL(mx_paged_cache_append(&c, mx_dtype_of(k.scalar_type()), static_cast<int32_t>(k.size(1)),
+                                static_cast<int32_t>(k.size(2)), &ko, &vo, k.size(0), B,
+                                offsets.data_ptr(), index_bytes_of(offsets, "offsets"),
+                                starts.data_ptr(), index_bytes_of(starts, "starts"), stream_of(k)));
+}
+
+Tensor paged_cache_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache,
+                             const Tensor& page_table, const Tensor& lengths,
+                             std::optional<double> scale) {
+  check_gpu(q, "q");
+  c10::OptionalDeviceGuard guard(q.device());
+  check_arg(k_cache, q, "k_cache", false);
+  const mx_paged_cache c = pack_cache(k_cache, v_cache, page_table);
+  check_rows(q, k_cache, "q");
+  const int64_t B = q.size(0), H = q.size(1), D = q.size(2), Hkv = k_cache.size(2);
+  TORCH_CHECK(D == k_cache.size(3), "q has head width ", D, " but the cache ", k_cache.size(3));
+  TORCH_CHECK(H > 0 && H % Hkv == 0 && H < (1 << 20), "q has ", H, " heads, which is no multiple of the ", Hkv,
+              " key-value heads");
+  TORCH_CHECK(page_table.size(0) == B, "page_table has ", page_table.size(0), " rows but q ", B);
+  check_arg(lengths, q, "lengths", true);
+  TORCH_CHECK(lengths.dim() == 1 && lengths.numel() == B, "lengths must have ", B, " entries, got ",
+              lengths.sizes());
+  Tensor keep;
+  const mx_attention_tensor qo = attention_operand(q, keep);
+  Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+  const size_t ws_bytes = mx_paged_cache_attention_workspace_bytes(
+      &c, B, static_cast<int32_t>(H), static_cast<int32_t>(Hkv), static_cast<int32_t>(D));
+  Tensor ws;
+  if (ws_bytes > 0) ws = at::empty({static_cast<int64_t>(ws_bytes)}, q.options().dtype(at::kByte));
+  MX_CALL(mx_paged_cache_attention(&c, mx_dtype_of(q.scalar_type()), &qo, B, static_cast<int32_t>(H),
+                                   static_cast<int32_t>(Hkv), static_cast<int32_t>(D),
+                                   lengths.data_ptr(), index_bytes_of(lengths, "lengths"),
+                                   attention_scale(scale, D), out.data_ptr(),
+                                   ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, stream_of(q)));
+  return out;
+}
+
 }  // namespace mx_ops
 
 TORCH_LIBRARY_FRAGMENT(fbgemm, m) {
@@ -2167,4 +2463,27 @@ TORCH_LIBRARY(mx_fbgemm, m) {
   m.def("test_force_wide_sort_words(bool enable) -> ()", &mx_ops::test_force_wide_sort_words);
   m.def("test_force_workspace_counters(bool enable) -> ()",
         &mx_ops::test_force_workspace_counters);
+  m.def("jagged_attention(Tensor q, Tensor k, Tensor v, Tensor q_offsets, Tensor? k_offsets=None, "
+        "bool causal=True, float? scale=None) -> Tensor");
+  m.def("jagged_attention_forward(Tensor q, Tensor k, Tensor v, Tensor q_offsets, "
+        "Tensor? k_offsets=None, bool causal=True, float? scale=None) -> (Tensor, Tensor)");
+  m.def("jagged_attention_backward(Tensor grad_output, Tensor q, Tensor k, Tensor v, Tensor out, "
+        "Tensor lse, Tensor q_offsets, Tensor? k_offsets=None, bool causal=True, "
+        "float? scale=None) -> (Tensor, Tensor, Tensor)");
+  m.def("paged_cache_append(Tensor k, Tensor v, Tensor offsets, Tensor starts, "
+        "Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor page_table) -> ()");
+  m.def("paged_cache_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor page_table, "
+        "Tensor lengths, float? scale=None) -> Tensor");
+}
+
+TORCH_LIBRARY_IMPL(mx_fbgemm, CUDA, m) {
+  m.impl("jagged_attention", TORCH_FN(mx_ops::jagged_attention_plain));
+  m.impl("jagged_attention_forward", TORCH_FN(mx_ops::jagged_attention_forward));
+  m.impl("jagged_attention_backward", TORCH_FN(mx_ops::jagged_attention_backward));
+  m.impl("paged_cache_append", TORCH_FN(mx_ops::paged_cache_append));
+  m.impl("paged_cache_attention", TORCH_FN(mx_ops::paged_cache_attention));
+}
+
+TORCH_LIBRARY_IMPL(mx_fbgemm, Autograd, m) {
+  m.impl("jagged_attention", TORCH_FN(mx_ops::jagged_attention_autograd));
 }
