@@ -610,6 +610,7 @@ int mx_nbit_forward_nobag(const uint8_t* dev_weights, const int64_t* weights_off
  * multiple of 8 up to MX_ATTENTION_MAX_D, H a multiple of Hkv (query head h
  * reads key-value head h / (H / Hkv)). */
 #define MX_ATTENTION_MAX_D 128
+#define MX_ATTENTION_MAX_ROWS 0x3fffff00 /* of queries, and of keys */
 
 /* A [rows, heads, D] operand: strides in elements (multiples of 8; of a row at
  * least D and at most 2^23), the last dimension contiguous, 16-byte aligned. */

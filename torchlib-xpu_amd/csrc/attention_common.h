@@ -65,6 +65,13 @@ __device__ __forceinline__ float other_half(float v) {
   return __uint_as_float(lane_id() < 32 ? r[1] : r[0]);
 }
 
+// The smaller, and a row count left of at most `most`.
+__device__ __forceinline__ int min_of(int a, int b) { return a < b ? a : b; }
+__device__ __forceinline__ int rows_left(int len, int from, int most) {
+  const int n = len - from;
+  return n < 0 ? 0 : min_of(n, most);
+}
+
 // A buffer descriptor of `bytes` bytes from a wave-uniform base: loads past
 // them return zeros.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* base, uint32_t bytes) {
@@ -75,7 +82,19 @@ __device__ __forceinline__ i32x4 load16(__amdgpu_buffer_rsrc_t r, uint32_t off) 
   return __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0);
 }
 
-// An offset no descriptor of ours covers.
+// v, of which the compiler knows nothing: what is computed from it in a loop
+// stays there instead of taking registers through the loop.
+__device__ __forceinline__ uint32_t opaque(uint32_t v) {
+  asm("" : "+v"(v));
+  return v;
+}
+
+// The lane's number, counted anew where it is needed.
+__device__ __forceinline__ uint32_t lane_again() {
+  return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, opaque(0)));
+}
+
+// An offset no descriptor of ours covers (also after a tile's steps).
 constexpr uint32_t kOutside = 0x80000000u;
 
 // Bytes of `rows` rows of `width` bytes at a stride, for a descriptor.
@@ -95,22 +114,36 @@ __device__ __forceinline__ void load4_to_lds(__amdgpu_buffer_rsrc_t r, char* to,
 }
 
 // A tile of ROWS x DP 16-bit values in LDS: rows of C = DP / 8 chunks of 16
-// bytes, chunk c of row r at place c ^ f(r).  f spreads both kinds of reads
-// over the banks: the row reads (lane l: chunk c of row l) and the transposing
-// reads (16 lanes: 4 consecutive rows x 2 chunks).
+// bytes, chunk c of row r at place c ^ f(r).  LDS serves 256 bytes over 64 banks
+// at a time: 16 lanes of a row read (lane l: chunk c of row l) and 32 of a
+// transposing read (4 rows x 4 chunks).  f makes both meet every bank once.
 template <int DP>
 struct Tile {
   static constexpr int C = DP / 8;
   static constexpr int kRow = DP * 2;  // bytes
 
   static __device__ __forceinline__ int f(int r) {
-    if constexpr (C == 16) return ((r & 7) << 1) | ((r >> 3) & 1);
-    else if constexpr (C == 8) return ((r & 3) << 1) | ((r >> 2) & 1);
-    else return (((r >> 1) & 1) << 1) | ((r >> 2) & 1);  // 4 and 12: rows 2i and 2i + 1 differ by 64 bytes
+    if constexpr (C == 16) return ((r & 3) << 2) | ((r >> 2) & 3);
+    else if constexpr (C == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+    else return (r >> 2) & 3;  // 4 and 12: rows 0..3 fall into different quarters anyway
   }
 
   // Byte offset of chunk c of row r.
   static __device__ __forceinline__ int at(int r, int c) { return r * kRow + ((c ^ f(r)) << 4); }
+
+  // The offset of chunk c + 2 x, and of chunk c + 4 d, of the same row from that
+  // of chunk c (c < 2, c < 4): one instruction, no register kept per x or d.
+  static __device__ __forceinline__ uint32_t step2(uint32_t at_c, int x) {
+    return C == 12 ? (at_c ^ ((x & 1) << 5)) + (x >> 1) * 64 : at_c ^ (x << 5);
+  }
+  static __device__ __forceinline__ uint32_t step4(uint32_t at_c, int d) {
+    return C == 12 ? at_c + d * 64 : at_c ^ (d << 6);
+  }
+
+  // The same chunk 8 rows on (from a row r with r & 8 == 0).
+  static __device__ __forceinline__ uint32_t next8(uint32_t at_c) {
+    return (at_c ^ 32) + 8 * kRow;
+  }
 
   // Copies a tile of ROWS rows from global memory into LDS, without passing
   // through registers: THREADS threads, 16 bytes per lane and instruction, the
@@ -121,11 +154,16 @@ struct Tile {
     static constexpr int kAll = ROWS * C;  // 16-byte places
     static constexpr int kPer = kAll / THREADS;
     static_assert(kAll % THREADS == 0, "whole instructions");
-    uint32_t off[kPer];
+    // With a power of two of chunks, an instruction's rows follow the last
+    // one's by a fixed number and f repeats: one offset serves all.
+    static constexpr bool kOne = THREADS % (16 * C) == 0;
+    uint32_t off[kOne ? 1 : kPer];
+    uint32_t step;
 
     __device__ __forceinline__ void init(int tid, uint32_t stride, int d_chunks) {
+      step = stride * (THREADS / C);
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
+      for (int i = 0; i < (kOne ? 1 : kPer); ++i) {
         const int u = i * THREADS + tid;
         const int r = u / C, c = (u % C) ^ f(r);
         off[i] = c < d_chunks ? static_cast<uint32_t>(r) * stride + c * 16 : kOutside;
@@ -133,10 +171,28 @@ struct Tile {
     }
 
     __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, char* lds, int wave) const {
+      uint32_t o = off[0];
+      if constexpr (kOne && kPer > 1) o = opaque(o);
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) load16_to_lds(r, lds + (i * THREADS + wave * 64) * 16, off[i]);
+      for (int i = 0; i < kPer; ++i)
+        load16_to_lds(r, lds + (i * THREADS + wave * 64) * 16, kOne ? o + i * step : off[kOne ? 0 : i]);
     }
   };
+};
+
+// A lane's places in a tile, from row r0 (a multiple of 16) on: its row's first
+// chunk, and its piece of the transposing reads of rows 0..7 of each 16 (8
+// columns of the 32 of a block).
+template <int DP>
+struct Places {
+  uint32_t row, tr;
+  __device__ __forceinline__ Places(int lane, int r0) {
+    using Ti = Tile<DP>;
+    const int t = lane & 15, h = lane >> 5;
+    const int r = 4 * h + (t >> 2), c = 2 * ((lane >> 4) & 1) + ((t & 3) >> 1);
+    row = r0 * Ti::kRow + Ti::at(lane & 31, h);
+    tr = r0 * Ti::kRow + Ti::at(r, c) + (t & 1) * 8;
+  }
 };
 
 template <typename X8>
@@ -173,8 +229,14 @@ __device__ __forceinline__ void wait_lds_loads() { __builtin_amdgcn_s_waitcnt(0x
 
 struct Span {
   int64_t start;
-  int64_t len;  // >= 0
+  int32_t len;  // >= 0 (rows are below 2^31)
 };
+
+__device__ __forceinline__ int64_t uniform64(int64_t v) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(v));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(v >> 32));
+  return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
+}
 
 template <typename I>
 __device__ __forceinline__ int64_t list_start(const I* offsets, int64_t B, int64_t N, int64_t i) {
@@ -187,19 +249,13 @@ __device__ __forceinline__ int64_t list_start(const I* offsets, int64_t B, int64
 template <typename I>
 __device__ __forceinline__ Span list_span(const I* offsets, int64_t B, int64_t N, int64_t i) {
   const int64_t s = list_start(offsets, B, N, i), e = list_start(offsets, B, N, i + 1);
-  return {s, e > s ? e - s : 0};
-}
-
-__device__ __forceinline__ int64_t uniform64(int64_t v) {
-  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(v));
-  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(v >> 32));
-  return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
+  return {uniform64(s), __builtin_amdgcn_readfirstlane(static_cast<int32_t>(e > s ? e - s : 0))};
 }
 
 // The list (0..B+1) that owns tile slot `slot`, and the tile's number in it.
 template <typename I>
 __device__ __forceinline__ int64_t find_list(const I* offsets, int64_t B, int64_t N, int bm_shift,
-                                             int64_t slot, int64_t* tile) {
+                                             int64_t slot, int32_t* tile) {
   int64_t lo = 0, n = B + 2;
   int64_t key = 0;
   while (n > 1) {
@@ -212,8 +268,65 @@ __device__ __forceinline__ int64_t find_list(const I* offsets, int64_t B, int64_
     n = n - at < step ? n - at : step;
   }
   key = (list_start(offsets, B, N, lo) >> bm_shift) + lo;
-  *tile = uniform64(slot - key);
+  *tile = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(slot - key));
   return uniform64(lo);
+}
+
+// The same for a causal call of up to 62 lists, by rank: tiles with more work
+// come first, across all lists (a block's time is its tile's length: the longest
+// must not start last).  Lane i holds list i with n tiles; tile t of them has
+// work t + 1 + c (QUERIES, c the keys before its queries in tiles) or n - t + c
+// (keys: the queries from its first one on).  There are F(w) tiles of work w or
+// more, so rank r has the largest w with F(w) > r and is the (r - F(w + 1))-th
+// list that has a tile of work w.  False if there are no more tiles.
+template <bool QUERIES, typename I>
+__device__ __forceinline__ bool find_ranked(const I* own, const I* other, int64_t B, int64_t N,
+                                            int64_t Nother, int bm_shift, int64_t rank, int64_t* list,
+                                            int32_t* tile) {
+  const int i = lane_id();
+  int n = 0, c = 0;
+  if (i < B + 2) {
+    const int64_t s = list_start(own, B, N, i), e = list_start(own, B, N, i + 1);
+    const int len = static_cast<int>(e > s ? e - s : 0);
+    n = (len + (1 << bm_shift) - 1) >> bm_shift;
+    if (QUERIES && i > 0 && i <= B) {
+      const int64_t os = list_start(other, B, Nother, i), oe = list_start(other, B, Nother, i + 1);
+      const int more = static_cast<int>(oe > os ? oe - os : 0) - len;
+      c = more > 0 ? more >> bm_shift : 0;
+    }
+  }
+  auto lane_count = [&](int w) {  // tiles of this list with work w or more
+    const int k = n + c - (w - 1);
+    return k < 0 ? 0 : (k < n ? k : n);
+  };
+  auto total = [&](int w) {
+    int v = lane_count(w);
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+    return __builtin_amdgcn_readfirstlane(v);
+  };
+  int lo = 0, hi = n + c + 1;  // F(lo) > rank >= F(hi)
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) {
+    const int v = __shfl_xor(hi, m, 64);
+    hi = v > hi ? v : hi;
+  }
+  hi = __builtin_amdgcn_readfirstlane(hi);
+  if (rank >= total(1)) return false;
+  lo = 1;
+  while (hi - lo > 1) {
+    const int mid = lo + (hi - lo) / 2;
+    if (total(mid) > rank) lo = mid;
+    else hi = mid;
+  }
+  const int k = static_cast<int>(rank) - total(lo + 1);
+  const bool has = lane_count(lo) > lane_count(lo + 1);
+  const uint64_t set = __ballot(has);
+  const bool me = has && __popcll(set & ((1ull << i) - 1)) == static_cast<unsigned>(k);
+  const int at = __builtin_ctzll(__ballot(me));
+  *list = at;
+  *tile = __builtin_amdgcn_readfirstlane(__shfl(QUERIES ? lo - 1 - c : n + c - lo, at, 64));
+  return true;
 }
 
 inline int64_t tile_slots(int64_t N, int64_t B, int bm) { return N / bm + B + 2; }

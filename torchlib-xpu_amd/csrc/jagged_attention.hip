@@ -20,26 +20,25 @@ struct FwdArgs {
   int64_t B, Nq, Nk;
   int32_t H, G, D;                 // G query heads per key-value head
   int32_t causal;
+  int32_t ranked;                  // find_ranked finds the tiles
   float scale;
   void* out;                       // [Nq, H, D]
   float* lse;                      // [H, Nq] or null
 };
 
-// Which head and tile slot a block works on.  Blocks go to the 8 XCDs in turn:
-// with a multiple of 8 heads each XCD keeps H / 8 neighbouring heads (which
-// share keys) and takes all their tiles, so its L2 holds few keys and the
-// causal tiles, unequal in length, spread evenly.  Later tiles first: they are
-// a list's longest under the causal mask.
-__device__ __forceinline__ void head_and_slot(int64_t bid, int H, int64_t slots, int* head,
-                                              int64_t* slot) {
+// Which head a block works on, and which of its tiles (the 0th first).  Blocks
+// go to the 8 XCDs in turn: with a multiple of 8 heads each XCD keeps H / 8
+// neighbouring heads (which share keys) and takes all their tiles, so its L2
+// holds few keys and the causal tiles, unequal in length, spread evenly.
+__device__ __forceinline__ void head_and_turn(int64_t bid, int H, int* head, int64_t* turn) {
   if (H % 8 == 0) {
     const int per = H / 8;
     const int64_t x = bid % 8, y = bid / 8;
     *head = static_cast<int>(x * per + y % per);
-    *slot = slots - 1 - y / per;
+    *turn = y / per;
   } else {
     *head = static_cast<int>(bid % H);
-    *slot = slots - 1 - bid / H;
+    *turn = bid / H;
   }
 }
 
@@ -91,12 +90,18 @@ __global__ void __launch_bounds__(NW * 64, 2) fwd_kernel(const FwdArgs a, int64_
   __shared__ __attribute__((aligned(1024))) char lds[4 * kTileBytes];  // K0 V0 K1 V1
 
   int head;
-  int64_t slot, tile;
-  head_and_slot(blockIdx.x, a.H, slots, &head, &slot);
+  int64_t turn;
+  int tile;
+  head_and_turn(blockIdx.x, a.H, &head, &turn);
   const I* qo = static_cast<const I*>(a.q_offsets);
   const I* ko = static_cast<const I*>(a.k_offsets);
-  constexpr int kShift = NW == 1 ? 5 : NW == 2 ? 6 : NW == 4 ? 7 : 8;
-  const int64_t list = find_list(qo, a.B, a.Nq, kShift, slot, &tile);
+  constexpr int kShift = NW == 1 ? 5 : NW == 2 ? 6 : 7;
+  int64_t list;
+  if (a.ranked) {
+    if (!find_ranked<true>(qo, ko, a.B, a.Nq, a.Nk, kShift, turn, &list, &tile)) return;
+  } else {  // a list's last tiles first: the causal mask makes them its longest
+    list = find_list(qo, a.B, a.Nq, kShift, slots - 1 - turn, &tile);
+  }
   const Span sq = list_span(qo, a.B, a.Nq, list);
   if (tile * BM >= sq.len) return;
   Span sk{0, 0};
@@ -105,20 +110,18 @@ __global__ void __launch_bounds__(NW * 64, 2) fwd_kernel(const FwdArgs a, int64_
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, l = lane & 31, h = lane >> 5;
-  const int64_t row0 = uniform64(tile * BM + wave * 32);  // the wave's first query in the list
-  const int64_t q_base = uniform64(sq.start + row0);
-  const int rows = static_cast<int>(sq.len - row0 < 32 ? (sq.len > row0 ? sq.len - row0 : 0) : 32);
-  const int64_t Lk = uniform64(sk.len);
-  const int64_t shift = uniform64(Lk - sq.len);  // query i sees keys 0 .. i + shift
-  // Keys that a query of the block, and one of the wave, sees at most.
-  int64_t blk_end = Lk, wave_end = Lk;
-  if (a.causal) {
-    const int64_t last = (tile + 1) * BM < sq.len ? (tile + 1) * BM : sq.len;
-    blk_end = last + shift < Lk ? last + shift : Lk;
-    wave_end = row0 + rows + shift;
-  }
-  if (rows == 0) wave_end = 0;
-  const int tiles = blk_end > 0 ? static_cast<int>((blk_end + kBN - 1) / kBN) : 0;
+  const int row0 = tile * BM + wave * 32;  // the wave's first query in the list
+  const int64_t q_base = sq.start + row0;
+  const int rows = rows_left(sq.len, row0, 32);
+  const int Lk = sk.len;
+  const int shift = Lk - sq.len;  // query i sees keys 0 .. i + shift
+  // Keys that a query of the block, and one of the wave, sees at most; keys that
+  // every query of the wave sees.
+  const int blk_end = a.causal ? min_of(tile * BM + BM, sq.len) + shift : Lk;
+  const int wave_end = rows == 0 ? 0 : a.causal ? row0 + rows + shift : Lk;
+  const int all_end = a.causal ? min_of(row0 + shift + 1, Lk) : Lk;
+  const int tiles = blk_end > 0 ? (blk_end + kBN - 1) / kBN : 0;
+  const int mine = a.causal ? min_of(row0 + l + shift + 1, Lk) : Lk;  // this lane's query sees
 
   // Queries: the B operand of K Q^T.
   X8 qf[KS];
@@ -127,34 +130,32 @@ __global__ void __launch_bounds__(NW * 64, 2) fwd_kernel(const FwdArgs a, int64_
   typename Ti::template Loader<kBN, NW * 64> lk, lv;
   lk.init(tid, static_cast<uint32_t>(a.k_row), a.D / 8);
   lv.init(tid, static_cast<uint32_t>(a.v_row), a.D / 8);
-  const char* kp = a.k + uniform64(sk.start) * a.k_row + (head / a.G) * a.k_head;
-  const char* vp = a.v + uniform64(sk.start) * a.v_row + (head / a.G) * a.v_head;
+  const char* kp = a.k + sk.start * a.k_row + (head / a.G) * a.k_head;
+  const char* vp = a.v + sk.start * a.v_row + (head / a.G) * a.v_head;
   f32x16 o[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) o[d] = f32x16{};
   float m = -INFINITY, sum = 0.0f;
   const float c2 = a.scale * kLog2e;
 
-  // LDS places of this lane's operands.
-  const int t16 = lane & 15, g16 = (lane >> 4) & 1;
-  const int vrow = 4 * h + (t16 >> 2);
+  const Places<DP> at(lane, 0);
 
   // The restrict pointers tell the compiler that the copies into the next
   // tiles' LDS do not meet this tile's reads (it would wait for them).
   auto load_tile = [&](int j, char* __restrict__ dst) __attribute__((always_inline)) {
-    const int64_t left = Lk - static_cast<int64_t>(j) * kBN;
-    const int n = left < kBN ? static_cast<int>(left) : kBN;
+    const int n = rows_left(Lk, j * kBN, kBN);
     lk.load(make_rsrc(kp + static_cast<int64_t>(j) * kBN * a.k_row,
                       span_bytes(n, static_cast<uint32_t>(a.k_row), a.D * 2)), dst, wave);
     lv.load(make_rsrc(vp + static_cast<int64_t>(j) * kBN * a.v_row,
                       span_bytes(n, static_cast<uint32_t>(a.v_row), a.D * 2)),
             dst + kTileBytes, wave);
   };
-  auto work = [&](int j, const char* __restrict__ kt, char* __restrict__ next) __attribute__((always_inline)) {
+  auto work = [&](int j, const char* __restrict__ cur, uint32_t buf,
+                  char* __restrict__ next) __attribute__((always_inline)) {
     if (j + 1 < tiles) load_tile(j + 1, next);
-    const int64_t k0 = static_cast<int64_t>(j) * kBN;
+    const int k0 = j * kBN;
     if (k0 >= wave_end) return;
-    const char* vt = kt + kTileBytes;
+    const uint32_t ra = opaque(at.row + buf);
 
     f32x16 s[2];
 #pragma unroll
@@ -162,19 +163,16 @@ __global__ void __launch_bounds__(NW * 64, 2) fwd_kernel(const FwdArgs a, int64_
       s[b] = f32x16{};
 #pragma unroll
       for (int x = 0; x < KS; ++x)
-        s[b] = E::mfma32(lds_read16<X8>(kt + Ti::at(32 * b + l, 2 * x + h)), qf[x], s[b]);
+        s[b] = E::mfma32(lds_read16<X8>(cur + 32 * b * Ti::kRow + Ti::step2(ra, x)), qf[x], s[b]);
     }
 
-    // Mask: only where the tile reaches past a query's last key.
-    const int64_t end0 = a.causal ? row0 + shift + 1 : Lk;  // of the wave's first query
-    if (k0 + kBN > end0 || k0 + kBN > Lk) {
-      const int64_t mine = a.causal ? row0 + l + shift + 1 : Lk;
-      const int last = static_cast<int>((mine < Lk ? mine : Lk) - k0 < kBN ? (mine < Lk ? mine : Lk) - k0 : kBN);
+    if (k0 + kBN > all_end) {  // the tile reaches past a query's last key
+      const int last = mine - k0 - 4 * h;
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (32 * b + 8 * (i / 4) + 4 * h + i % 4 >= last) s[b][i] = -INFINITY;
+          if (32 * b + 8 * (i / 4) + i % 4 >= last) s[b][i] = -INFINITY;
     }
 
     float top = s[0][0];
@@ -203,14 +201,14 @@ __global__ void __launch_bounds__(NW * 64, 2) fwd_kernel(const FwdArgs a, int64_
         p[2 * b + i / 8][i % 8] = static_cast<T>(e);
       }
 
+    const uint32_t t0 = opaque(at.tr + buf), t1 = Ti::next8(t0);
 #pragma unroll
     for (int x = 0; x < 4; ++x)
 #pragma unroll
       for (int d = 0; d < DB; ++d) {
-        const int chunk = 4 * d + 2 * g16 + ((t16 & 3) >> 1);
-        const char* p0 = vt + Ti::at(16 * x + vrow, chunk) + (t16 & 1) * 8;
-        const char* p1 = vt + Ti::at(16 * x + 8 + vrow, chunk) + (t16 & 1) * 8;
-        o[d] = E::mfma32(join<X8>(lds_read_tr(p0), lds_read_tr(p1)), p[x], o[d]);
+        const char* f = cur + kTileBytes + 16 * x * Ti::kRow;
+        o[d] = E::mfma32(join<X8>(lds_read_tr(f + Ti::step4(t0, d)), lds_read_tr(f + Ti::step4(t1, d))),
+                         p[x], o[d]);
       }
   };
 
@@ -218,7 +216,7 @@ __global__ void __launch_bounds__(NW * 64, 2) fwd_kernel(const FwdArgs a, int64_
   for (int j = 0; j < tiles; ++j) {
     wait_lds_loads();
     __syncthreads();
-    work(j, lds + (j & 1) * 2 * kTileBytes, lds + ((j + 1) & 1) * 2 * kTileBytes);
+    work(j, lds, (j & 1) * 2 * kTileBytes, lds + ((j + 1) & 1) * 2 * kTileBytes);
   }
 
   sum += other_half(sum);
@@ -249,6 +247,7 @@ struct BwdArgs {
   int64_t B, Nq, Nk;
   int32_t H, Hkv, G, D;
   int32_t causal;
+  int32_t ranked;                  // find_ranked finds the tiles
   float scale;
   const float* lse;                    // [H, Nq]
   float *lse2, *delta;                 // [H, Nq], workspace
@@ -265,12 +264,18 @@ __global__ void __launch_bounds__(NW * 64, 2) bwd_q_kernel(const BwdArgs a, int6
   __shared__ __attribute__((aligned(1024))) char lds[4 * kTileBytes];
 
   int head;
-  int64_t slot, tile;
-  head_and_slot(blockIdx.x, a.H, slots, &head, &slot);
+  int64_t turn;
+  int tile;
+  head_and_turn(blockIdx.x, a.H, &head, &turn);
   const I* qo = static_cast<const I*>(a.q_offsets);
   const I* ko = static_cast<const I*>(a.k_offsets);
-  constexpr int kShift = NW == 1 ? 5 : NW == 2 ? 6 : NW == 4 ? 7 : 8;
-  const int64_t list = find_list(qo, a.B, a.Nq, kShift, slot, &tile);
+  constexpr int kShift = NW == 1 ? 5 : NW == 2 ? 6 : 7;
+  int64_t list;
+  if (a.ranked) {
+    if (!find_ranked<true>(qo, ko, a.B, a.Nq, a.Nk, kShift, turn, &list, &tile)) return;
+  } else {  // a list's last tiles first: the causal mask makes them its longest
+    list = find_list(qo, a.B, a.Nq, kShift, slots - 1 - turn, &tile);
+  }
   const Span sq = list_span(qo, a.B, a.Nq, list);
   if (tile * BM >= sq.len) return;
   Span sk{0, 0};
@@ -279,19 +284,18 @@ __global__ void __launch_bounds__(NW * 64, 2) bwd_q_kernel(const BwdArgs a, int6
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, l = lane & 31, h = lane >> 5;
-  const int64_t row0 = uniform64(tile * BM + wave * 32);
-  const int64_t q_base = uniform64(sq.start + row0);
-  const int rows = static_cast<int>(sq.len - row0 < 32 ? (sq.len > row0 ? sq.len - row0 : 0) : 32);
-  const int64_t Lk = uniform64(sk.len);
-  const int64_t shift = uniform64(Lk - sq.len);
-  int64_t blk_end = Lk, wave_end = Lk;
-  if (a.causal) {
-    const int64_t last = (tile + 1) * BM < sq.len ? (tile + 1) * BM : sq.len;
-    blk_end = last + shift < Lk ? last + shift : Lk;
-    wave_end = row0 + rows + shift;
-  }
-  if (rows == 0) wave_end = 0;
-  const int tiles = blk_end > 0 ? static_cast<int>((blk_end + kBN - 1) / kBN) : 0;
+  const int row0 = tile * BM + wave * 32;  // the wave's first query in the list
+  const int64_t q_base = sq.start + row0;
+  const int rows = rows_left(sq.len, row0, 32);
+  const int Lk = sk.len;
+  const int shift = Lk - sq.len;  // query i sees keys 0 .. i + shift
+  // Keys that a query of the block, and one of the wave, sees at most; keys that
+  // every query of the wave sees.
+  const int blk_end = a.causal ? min_of(tile * BM + BM, sq.len) + shift : Lk;
+  const int wave_end = rows == 0 ? 0 : a.causal ? row0 + rows + shift : Lk;
+  const int all_end = a.causal ? min_of(row0 + shift + 1, Lk) : Lk;
+  const int tiles = blk_end > 0 ? (blk_end + kBN - 1) / kBN : 0;
+  const int mine = a.causal ? min_of(row0 + l + shift + 1, Lk) : Lk;  // this lane's query sees
 
   X8 qf[KS], gf[KS];
   load_rows<X8, KS>(qf, a.q + q_base * a.q_row + head * a.q_head, rows, a.q_row, a.D, l, h);
@@ -319,63 +323,58 @@ __global__ void __launch_bounds__(NW * 64, 2) bwd_q_kernel(const BwdArgs a, int6
   typename Ti::template Loader<kBN, NW * 64> lk, lv;
   lk.init(tid, static_cast<uint32_t>(a.k_row), a.D / 8);
   lv.init(tid, static_cast<uint32_t>(a.v_row), a.D / 8);
-  const char* kp = a.k + uniform64(sk.start) * a.k_row + (head / a.G) * a.k_head;
-  const char* vp = a.v + uniform64(sk.start) * a.v_row + (head / a.G) * a.v_head;
+  const char* kp = a.k + sk.start * a.k_row + (head / a.G) * a.k_head;
+  const char* vp = a.v + sk.start * a.v_row + (head / a.G) * a.v_head;
 
   f32x16 dq[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) dq[d] = f32x16{};
   const float c2 = a.scale * kLog2e;
-  const int t16 = lane & 15, g16 = (lane >> 4) & 1;
-  const int trow = 4 * h + (t16 >> 2);
+  const Places<DP> at(lane, 0);
 
   auto load_tile = [&](int j, char* __restrict__ dst) __attribute__((always_inline)) {
-    const int64_t left = Lk - static_cast<int64_t>(j) * kBN;
-    const int n = left < kBN ? static_cast<int>(left) : kBN;
+    const int n = rows_left(Lk, j * kBN, kBN);
     lk.load(make_rsrc(kp + static_cast<int64_t>(j) * kBN * a.k_row,
                       span_bytes(n, static_cast<uint32_t>(a.k_row), a.D * 2)), dst, wave);
     lv.load(make_rsrc(vp + static_cast<int64_t>(j) * kBN * a.v_row,
                       span_bytes(n, static_cast<uint32_t>(a.v_row), a.D * 2)),
             dst + kTileBytes, wave);
   };
-  auto work = [&](int j, const char* __restrict__ kt, char* __restrict__ next) __attribute__((always_inline)) {
+  auto work = [&](int j, const char* __restrict__ cur, uint32_t buf,
+                  char* __restrict__ next) __attribute__((always_inline)) {
     if (j + 1 < tiles) load_tile(j + 1, next);
-    const char* vt = kt + kTileBytes;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      const int64_t k0 = static_cast<int64_t>(j) * kBN + 32 * b;
+      const int k0 = j * kBN + 32 * b;
       if (k0 >= wave_end) return;
+      const uint32_t ra = opaque(at.row + buf), t0 = opaque(at.tr + buf), t1 = Ti::next8(t0);
+      const char* kt = cur + 32 * b * Ti::kRow;
+      const char* vt = kt + kTileBytes;
       f32x16 s{}, dp{};
 #pragma unroll
       for (int x = 0; x < KS; ++x) {
-        s = E::mfma32(lds_read16<X8>(kt + Ti::at(32 * b + l, 2 * x + h)), qf[x], s);
-        dp = E::mfma32(lds_read16<X8>(vt + Ti::at(32 * b + l, 2 * x + h)), gf[x], dp);
+        s = E::mfma32(lds_read16<X8>(kt + Ti::step2(ra, x)), qf[x], s);
+        dp = E::mfma32(lds_read16<X8>(vt + Ti::step2(ra, x)), gf[x], dp);
       }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = exp2_hw(__builtin_fmaf(s[i], c2, -lse2));
-      const int64_t end0 = a.causal ? row0 + shift + 1 : Lk;
-      if (k0 + 32 > end0 || k0 + 32 > Lk) {
-        const int64_t mine = a.causal ? row0 + l + shift + 1 : Lk;
-        const int64_t lim = (mine < Lk ? mine : Lk) - k0;
-        const int last = lim < 32 ? (lim > 0 ? static_cast<int>(lim) : 0) : 32;
+      for (int i = 0; i < 16; ++i)
+        s[i] = exp2_hw(__builtin_fmaf(s[i], c2, -lse2)) * (dp[i] - delta);
+      if (k0 + 32 > all_end) {
+        const int last = mine - k0 - 4 * h;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const bool hidden = 8 * (i / 4) + 4 * h + i % 4 >= last;
-          s[i] = hidden ? 0.0f : s[i];
-          dp[i] = hidden ? 0.0f : dp[i];
-        }
+        for (int i = 0; i < 16; ++i)
+          if (8 * (i / 4) + i % 4 >= last) s[i] = 0.0f;
       }
       X8 ds[2];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) ds[i / 8][i % 8] = static_cast<T>(s[i] * (dp[i] - delta));
+      for (int i = 0; i < 16; ++i) ds[i / 8][i % 8] = static_cast<T>(s[i]);
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
-          const int chunk = 4 * d + 2 * g16 + ((t16 & 3) >> 1);
-          const char* p0 = kt + Ti::at(32 * b + 16 * x + trow, chunk) + (t16 & 1) * 8;
-          const char* p1 = kt + Ti::at(32 * b + 16 * x + 8 + trow, chunk) + (t16 & 1) * 8;
-          dq[d] = E::mfma32(join<X8>(lds_read_tr(p0), lds_read_tr(p1)), ds[x], dq[d]);
+          const char* f = kt + 16 * x * Ti::kRow;
+          dq[d] = E::mfma32(join<X8>(lds_read_tr(f + Ti::step4(t0, d)), lds_read_tr(f + Ti::step4(t1, d))),
+                            ds[x], dq[d]);
         }
     }
   };
@@ -384,33 +383,44 @@ __global__ void __launch_bounds__(NW * 64, 2) bwd_q_kernel(const BwdArgs a, int6
   for (int j = 0; j < tiles; ++j) {
     wait_lds_loads();
     __syncthreads();
-    work(j, lds + (j & 1) * 2 * kTileBytes, lds + ((j + 1) & 1) * 2 * kTileBytes);
+    work(j, lds, (j & 1) * 2 * kTileBytes, lds + ((j + 1) & 1) * 2 * kTileBytes);
   }
   if (l >= rows) return;
   store_columns<T, DP>(static_cast<T*>(a.dq) + ((q_base + l) * a.H + head) * a.D, dq, a.scale, a.D, h);
 }
 
 // The keys' launch: a wave owns 32 keys and their sums over every query head of
-// the group and every query that sees them.  Queries and dO go through LDS in
-// tiles of 64 with their lse and delta; scores come out with a key per lane.
-template <typename T, typename I, int DP, int NW>
-__global__ void __launch_bounds__(NW * 64, 1) bwd_kv_kernel(const BwdArgs a, int64_t slots) {
+// the group and every query that sees them (half of them with NQ = 2: two
+// groups of waves take alternate 64-query blocks and join their sums through
+// LDS at the end).  Queries and dO go through LDS with their lse and delta;
+// scores come out with a key per lane.  D = 128 takes 192 registers for K, V,
+// dK and dV: scores are used up before dP is computed, which leaves two waves
+// per SIMD.
+template <typename T, typename I, int DP, int NK, int NQ>
+__global__ void __launch_bounds__(NK * NQ * 64, 2) bwd_kv_kernel(const BwdArgs a) {
   using E = Elem<T>;
   using X8 = typename E::x8;
   using Ti = Tile<DP>;
-  constexpr int KS = DP / 16, DB = DP / 32, BM = NW * 32, BQ = 64;
+  constexpr int KS = DP / 16, DB = DP / 32, BM = NK * 32, BQ = 64 * NQ, THREADS = NK * NQ * 64;
   constexpr int kTileBytes = BQ * DP * 2;
   constexpr int kStat = BQ * 4;
   constexpr int kBuf = 2 * kTileBytes + 2 * kStat;  // Q, dO, lse2, delta
   __shared__ __attribute__((aligned(1024))) char lds[2 * kBuf];
+  static_assert(NQ == 1 || 2 * kBuf >= BM * DP * 4, "the join's room");
 
   int kvh;
-  int64_t slot, tile;
-  head_and_slot(blockIdx.x, a.Hkv, slots, &kvh, &slot);
+  int64_t turn;
+  int tile;
+  head_and_turn(blockIdx.x, a.Hkv, &kvh, &turn);
   const I* qo = static_cast<const I*>(a.q_offsets);
   const I* ko = static_cast<const I*>(a.k_offsets);
-  constexpr int kShift = NW == 1 ? 5 : NW == 2 ? 6 : NW == 4 ? 7 : 8;
-  const int64_t list = find_list(ko, a.B, a.Nk, kShift, slots - 1 - slot, &tile);
+  constexpr int kShift = NK == 1 ? 5 : NK == 2 ? 6 : 7;
+  int64_t list;
+  if (a.ranked) {
+    if (!find_ranked<false>(ko, qo, a.B, a.Nk, a.Nq, kShift, turn, &list, &tile)) return;
+  } else {
+    list = find_list(ko, a.B, a.Nk, kShift, turn, &tile);
+  }
   const Span sk = list_span(ko, a.B, a.Nk, list);
   if (tile * BM >= sk.len) return;
   Span sq{0, 0};
@@ -418,120 +428,158 @@ __global__ void __launch_bounds__(NW * 64, 1) bwd_kv_kernel(const BwdArgs a, int
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int part = wave / NK;  // which 64 of a tile's queries
   const int lane = tid & 63, l = lane & 31, h = lane >> 5;
-  const int64_t key0 = uniform64(tile * BM + wave * 32);
-  const int64_t k_base = uniform64(sk.start + key0);
-  const int keys = static_cast<int>(sk.len - key0 < 32 ? (sk.len > key0 ? sk.len - key0 : 0) : 32);
-  const int64_t Lq = uniform64(sq.len);
-  const int64_t shift = uniform64(sk.len - sq.len);
-  // First query that sees a key of the block, to a whole tile.
-  int64_t first = 0;
-  if (a.causal) first = tile * BM - shift > 0 ? tile * BM - shift : 0;
-  const int64_t t0 = first / BQ;
-  const int64_t t1 = (Lq + BQ - 1) / BQ;
-  const int per = t1 > t0 ? static_cast<int>(t1 - t0) : 0;
-  const int steps = per * a.G;
+  const int key0 = tile * BM + wave % NK * 32;
+  const int64_t k_base = sk.start + key0;
+  const int keys = rows_left(sk.len, key0, 32);
+  const int Lq = sq.len;
+  const int shift = sk.len - Lq;
+  // From the first query that sees a key of the block, to a whole 64.
+  const int first = a.causal && tile * BM > shift ? (tile * BM - shift) / 64 * 64 : 0;
+  const int per = Lq > first ? (Lq - first + BQ - 1) / BQ : 0;
+  const int64_t steps = static_cast<int64_t>(per) * a.G;
 
   X8 kf[KS], vf[KS];
   load_rows<X8, KS>(kf, a.k + k_base * a.k_row + kvh * a.k_head, keys, a.k_row, a.D, l, h);
   load_rows<X8, KS>(vf, a.v + k_base * a.v_row + kvh * a.v_head, keys, a.v_row, a.D, l, h);
 
-  typename Ti::template Loader<BQ, NW * 64> lq, lg;
+  typename Ti::template Loader<BQ, THREADS> lq, lg;
   lq.init(tid, static_cast<uint32_t>(a.q_row), a.D / 8);
   lg.init(tid, static_cast<uint32_t>(a.g_row), a.D / 8);
-  const int64_t qs = uniform64(sq.start);
+  const int64_t qs = sq.start;
 
   f32x16 dk[DB], dv[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) dk[d] = dv[d] = f32x16{};
   const float c2 = a.scale * kLog2e;
-  const int t16 = lane & 15, g16 = (lane >> 4) & 1;
-  const int trow = 4 * h + (t16 >> 2);
+  const Places<DP> at(lane, 64 * part);
 
   auto load_tile = [&](int g, int t, char* __restrict__ dst) __attribute__((always_inline)) {
     const int head = kvh * a.G + g;
-    const int64_t i0 = (t0 + t) * BQ;
-    const int n = Lq - i0 < BQ ? static_cast<int>(Lq - i0) : BQ;
+    const int i0 = first + t * BQ;
+    const int n = rows_left(Lq, i0, BQ);
     lq.load(make_rsrc(a.q + (qs + i0) * a.q_row + head * a.q_head,
                       span_bytes(n, static_cast<uint32_t>(a.q_row), a.D * 2)), dst, wave);
     lg.load(make_rsrc(a.grad + (qs + i0) * a.g_row + head * a.g_head,
                       span_bytes(n, static_cast<uint32_t>(a.g_row), a.D * 2)),
             dst + kTileBytes, wave);
-    if (wave < 2) {
-      const float* st = (wave == 0 ? a.lse2 : a.delta) + head * a.Nq + qs + i0;
-      load4_to_lds(make_rsrc(st, n * 4), dst + 2 * kTileBytes + wave * kStat, lane * 4);
+    const int64_t s0 = head * a.Nq + qs + i0;
+    for (int u = wave; u < 2 * NQ; u += NK * NQ) {  // 64 values each
+      const float* from = (u < NQ ? a.lse2 : a.delta) + s0;
+      load4_to_lds(make_rsrc(from, n * 4), dst + 2 * kTileBytes + u * 256,
+                   (u % NQ * 64 + lane_again()) * 4);
     }
   };
-  auto work = [&](int t, const char* __restrict__ qt, char* __restrict__ next, int gn, int tn,
-                  bool more) __attribute__((always_inline)) {
+  auto work = [&](int t, const char* __restrict__ cur, uint32_t buf, char* __restrict__ next, int gn,
+                  int tn, bool more) __attribute__((always_inline)) {
     if (more) load_tile(gn, tn, next);
-    const char* gt = qt + kTileBytes;
-    const char* st = qt + 2 * kTileBytes;
-#pragma unroll
+#pragma unroll 1
     for (int b = 0; b < 2; ++b) {
-      const int64_t i0 = (t0 + t) * BQ + 32 * b;
+      const int i0 = first + t * BQ + 64 * part + 32 * b;
       if (keys == 0 || i0 >= Lq) return;
       if (a.causal && key0 > i0 + 31 + shift) continue;
+      const uint32_t from32 = buf + 32 * b * Ti::kRow;
+      const uint32_t ra = opaque(at.row + from32), t0 = opaque(at.tr + from32), t1 = Ti::next8(t0);
+      const char* gt = cur + kTileBytes;
+      const char* st = cur + buf + 2 * kTileBytes + (64 * part + 32 * b + 4 * h) * 4;
       f32x16 s{}, dp{};
 #pragma unroll
-      for (int x = 0; x < KS; ++x) {
-        s = E::mfma32(lds_read16<X8>(qt + Ti::at(32 * b + l, 2 * x + h)), kf[x], s);
-        dp = E::mfma32(lds_read16<X8>(gt + Ti::at(32 * b + l, 2 * x + h)), vf[x], dp);
-      }
+      for (int x = 0; x < KS; ++x) s = E::mfma32(lds_read16<X8>(cur + Ti::step2(ra, x)), kf[x], s);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const f32x4 ls = *reinterpret_cast<const f32x4*>(st + (32 * b + 8 * u + 4 * h) * 4);
-        const f32x4 de = *reinterpret_cast<const f32x4*>(st + kStat + (32 * b + 8 * u + 4 * h) * 4);
+        const f32x4 ls = *reinterpret_cast<const f32x4*>(st + 32 * u);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 4; ++e)
           s[4 * u + e] = exp2_hw(__builtin_fmaf(s[4 * u + e], c2, -ls[e]));
-          dp[4 * u + e] -= de[e];
-        }
       }
-      if (a.causal && key0 + 31 > i0 + shift) {
-        // Query i0 + r sees key0 + l if r >= key0 + l - shift - i0.
-        const int64_t lim = key0 + l - shift - i0;
-        const int from = lim > 0 ? (lim < 32 ? static_cast<int>(lim) : 32) : 0;
+      // Query i0 + r sees key0 + l if r >= key0 + l - shift - i0.
+      const bool masked = a.causal && key0 + 31 > i0 + shift;
+      const int from = key0 + l - shift - i0 - 4 * h;
+      if (masked) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const bool hidden = 8 * (i / 4) + 4 * h + i % 4 < from;
-          s[i] = hidden ? 0.0f : s[i];
-          dp[i] = hidden ? 0.0f : dp[i];
-        }
+        for (int i = 0; i < 16; ++i)
+          if (8 * (i / 4) + i % 4 < from) s[i] = 0.0f;
       }
-      X8 p[2], ds[2];
+      X8 p[2];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        p[i / 8][i % 8] = static_cast<T>(s[i]);
-        ds[i / 8][i % 8] = static_cast<T>(s[i] * dp[i]);
-      }
+      for (int i = 0; i < 16; ++i) p[i / 8][i % 8] = static_cast<T>(s[i]);
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
-          const int chunk = 4 * d + 2 * g16 + ((t16 & 3) >> 1);
-          const int o0 = Ti::at(32 * b + 16 * x + trow, chunk) + (t16 & 1) * 8;
-          const int o1 = Ti::at(32 * b + 16 * x + 8 + trow, chunk) + (t16 & 1) * 8;
-          dv[d] = E::mfma32(join<X8>(lds_read_tr(gt + o0), lds_read_tr(gt + o1)), p[x], dv[d]);
-          dk[d] = E::mfma32(join<X8>(lds_read_tr(qt + o0), lds_read_tr(qt + o1)), ds[x], dk[d]);
+          const char* f = gt + 16 * x * Ti::kRow;
+          dv[d] = E::mfma32(join<X8>(lds_read_tr(f + Ti::step4(t0, d)), lds_read_tr(f + Ti::step4(t1, d))),
+                            p[x], dv[d]);
+        }
+      __builtin_amdgcn_sched_barrier(0);
+      const uint32_t rb = opaque(at.row + from32);
+#pragma unroll
+      for (int x = 0; x < KS; ++x) dp = E::mfma32(lds_read16<X8>(gt + Ti::step2(rb, x)), vf[x], dp);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const f32x4 de = *reinterpret_cast<const f32x4*>(st + kStat + 32 * u);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dp[4 * u + e] = s[4 * u + e] * (dp[4 * u + e] - de[e]);
+      }
+      if (masked) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (8 * (i / 4) + i % 4 < from) dp[i] = 0.0f;
+      }
+      X8 ds[2];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) ds[i / 8][i % 8] = static_cast<T>(dp[i]);
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          const char* f = cur + 16 * x * Ti::kRow;
+          dk[d] = E::mfma32(join<X8>(lds_read_tr(f + Ti::step4(t0, d)), lds_read_tr(f + Ti::step4(t1, d))),
+                            ds[x], dk[d]);
         }
     }
   };
 
   if (steps > 0) load_tile(0, 0, lds);
   int g = 0, t = 0;
-  for (int i = 0; i < steps; ++i) {
+  for (int64_t i = 0; i < steps; ++i) {
     const int tn = t + 1 < per ? t + 1 : 0, gn = t + 1 < per ? g : g + 1;
     wait_lds_loads();
     __syncthreads();
-    work(t, lds + (i & 1) * kBuf, lds + ((i + 1) & 1) * kBuf, gn, tn, i + 1 < steps);
+    work(t, lds, static_cast<uint32_t>(i & 1) * kBuf, lds + ((i + 1) & 1) * kBuf, gn, tn, i + 1 < steps);
     t = tn;
     g = gn;
   }
+
+  if constexpr (NQ == 2) {
+    // One lane's values of a block of columns: 16 x 64 floats per step.
+    float* room = reinterpret_cast<float*>(lds) + wave % NK * 32 * DP + lane;
+#pragma unroll
+    for (int pass = 0; pass < 2; ++pass) {
+      f32x16* x = pass == 0 ? dk : dv;
+      __syncthreads();
+      if (part == 1) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) room[(d * 16 + i) * 64] = x[d][i];
+      }
+      __syncthreads();
+      if (part == 0) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[d][i] += room[(d * 16 + i) * 64];
+      }
+    }
+    if (part == 1) return;
+  }
   if (l >= keys) return;
-  const int64_t at = ((k_base + l) * a.Hkv + kvh) * a.D;
-  store_columns<T, DP>(static_cast<T*>(a.dk) + at, dk, a.scale, a.D, h);
-  store_columns<T, DP>(static_cast<T*>(a.dv) + at, dv, 1.0f, a.D, h);
+  const int64_t to = ((k_base + l) * a.Hkv + kvh) * a.D;
+  store_columns<T, DP>(static_cast<T*>(a.dk) + to, dk, a.scale, a.D, h);
+  store_columns<T, DP>(static_cast<T*>(a.dv) + to, dv, 1.0f, a.D, h);
 }
 
 // ---------------------------------------------------------------------------
@@ -557,7 +605,7 @@ int launch_bwd(const BwdArgs& a, hipStream_t stream) {
   if (a.Nq > 0)
     bwd_q_kernel<T, I, DP, NW><<<dim3(static_cast<unsigned>(qslots * a.H)), NW * 64, 0, stream>>>(a, qslots);
   if (a.Nk > 0 && a.dk != nullptr)
-    bwd_kv_kernel<T, I, DP, NW><<<dim3(static_cast<unsigned>(kslots * a.Hkv)), NW * 64, 0, stream>>>(a, kslots);
+    bwd_kv_kernel<T, I, DP, NW, 2><<<dim3(static_cast<unsigned>(kslots * a.Hkv)), NW * 128, 0, stream>>>(a);
   MX_LAUNCH_CHECK();
   return MX_OK;
 }
@@ -594,6 +642,8 @@ int check_problem(const mx_attention_problem* p) {
   MX_REQUIRE(p->dtype == MX_DTYPE_F16 || p->dtype == MX_DTYPE_BF16, "dtype %d is not fp16 or bf16", p->dtype);
   MX_REQUIRE(p->index_bytes == 4 || p->index_bytes == 8, "index_bytes %d", p->index_bytes);
   MX_REQUIRE(p->B >= 0 && p->Nq >= 0 && p->Nk >= 0, "negative size");
+  MX_REQUIRE(p->Nq <= MX_ATTENTION_MAX_ROWS && p->Nk <= MX_ATTENTION_MAX_ROWS, "more than %d rows",
+             MX_ATTENTION_MAX_ROWS);
   MX_REQUIRE(p->H > 0 && p->Hkv > 0 && p->H % p->Hkv == 0,
              "%d query heads are no multiple of %d key-value heads", p->H, p->Hkv);
   MX_REQUIRE(p->D > 0 && p->D <= MX_ATTENTION_MAX_D && p->D % 8 == 0,
@@ -601,6 +651,12 @@ int check_problem(const mx_attention_problem* p) {
   MX_REQUIRE(std::isfinite(p->scale) && p->scale > 0.0f, "scale must be positive and finite");
   MX_REQUIRE(p->B == 0 || (p->q_offsets != nullptr && p->k_offsets != nullptr), "offsets are null");
   return MX_OK;
+}
+
+// Tiles by rank: lists long enough that a tile's length tells in the launch's,
+// and few enough for a lane each.
+int32_t ranked_tiles(const mx_attention_problem* p) {
+  return p->causal != 0 && p->B > 0 && p->B + 2 <= 64 && (p->Nq + p->Nk) / p->B >= 1024;
 }
 
 }  // namespace
@@ -629,6 +685,7 @@ extern "C" int mx_jagged_attention_forward(const mx_attention_problem* p, const 
   a.B = p->B, a.Nq = p->Nq, a.Nk = p->Nk;
   a.H = p->H, a.G = p->H / p->Hkv, a.D = p->D;
   a.causal = p->causal, a.scale = p->scale;
+  a.ranked = ranked_tiles(p);
   a.out = out, a.lse = lse;
   const hipStream_t s = mx::as_stream(stream);
   return p->dtype == MX_DTYPE_BF16 ? MX_ATTN_DISPATCH(launch_fwd, __bf16, a, p->index_bytes, s)
@@ -675,6 +732,7 @@ extern "C" int mx_jagged_attention_backward(const mx_attention_problem* p, const
   a.B = p->B, a.Nq = p->Nq, a.Nk = p->Nk;
   a.H = p->H, a.Hkv = p->Hkv, a.G = p->H / p->Hkv, a.D = p->D;
   a.causal = p->causal, a.scale = p->scale;
+  a.ranked = ranked_tiles(p);
   a.lse = lse;
   a.lse2 = static_cast<float*>(workspace);
   a.delta = a.lse2 + p->Nq * p->H;
