@@ -24,6 +24,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -75,7 +76,13 @@ __device__ __forceinline__ int rows_left(int len, int from, int most) {
 // A buffer descriptor of `bytes` bytes from a wave-uniform base: loads past
 // them return zeros.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* base, uint32_t bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00020000);
+  // In scalar registers whatever the compiler knows of the values: it would
+  // loop over the lanes' descriptors otherwise.
+  const uint64_t u = reinterpret_cast<uint64_t>(base);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(u));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(u >> 32));
+  void* p = reinterpret_cast<void*>((static_cast<uint64_t>(hi) << 32) | lo);
+  return __builtin_amdgcn_make_buffer_rsrc(p, 0, __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
 }
 
 __device__ __forceinline__ i32x4 load16(__amdgpu_buffer_rsrc_t r, uint32_t off) {
@@ -212,8 +219,16 @@ __device__ __forceinline__ X8 join(s16x4 a, s16x4 b) {
   return __builtin_bit_cast(X8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-// All LDS-direct loads of the wave have landed.
-__device__ __forceinline__ void wait_lds_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+// A barrier before which all but the wave's last N loads have landed and its LDS
+// reads are done (a block barrier of the language would wait for every load).
+template <int N>
+__device__ __forceinline__ void wait_and_barrier() {
+  static_assert(N < 64, "what the counter holds");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | ((N >> 4) << 14));
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
 // ---------------------------------------------------------------------------
 // Packed lists
@@ -221,15 +236,18 @@ __device__ __forceinline__ void wait_lds_loads() { __builtin_amdgcn_s_waitcnt(0x
 // Rows 0..N-1 are cut by B + 1 offsets.  Two more lists without partners hold
 // the rows before the first and after the last offset (if there are any), so
 // that every row belongs to one list: list 0 those before, lists 1..B the
-// caller's, list B + 1 those after.  A launch needs the tiles of every list
-// without a host copy of the offsets: list i owns the tile slots
-// start(i) / BM + i up to start(i + 1) / BM + i + 1, which is at least
-// ceil(length / BM) of them and N / BM + B + 2 in all, and a block finds its
-// list by a search over those keys, 64 lists per step.
+// caller's, list B + 1 those after.  A launch needs the tiles of BM rows of every
+// list without a host copy of the offsets.  With s / BM = a, s % BM = r for a
+// list's start and a', r' for its end, it has a' - a tiles and one more if
+// r' > r.  So turns 0 .. N / BM - 1 are tiles that exist, turn t in the list
+// with a <= t < a' (found by a search), and N / BM + i is list i's one more,
+// or nothing.  Blocks without work come last: among the others they would idle
+// the dispatcher, which hands the shader engines blocks in turn (256 lists of
+// 128 rows with every other block empty: 90 us instead of 60).
 
 struct Span {
-  int64_t start;
-  int32_t len;  // >= 0 (rows are below 2^31)
+  int32_t start;
+  int32_t len;  // >= 0
 };
 
 __device__ __forceinline__ int64_t uniform64(int64_t v) {
@@ -239,97 +257,130 @@ __device__ __forceinline__ int64_t uniform64(int64_t v) {
 }
 
 template <typename I>
-__device__ __forceinline__ int64_t list_start(const I* offsets, int64_t B, int64_t N, int64_t i) {
+__device__ __forceinline__ int32_t list_start(const I* offsets, int32_t B, int32_t N, int32_t i) {
   if (i <= 0) return 0;
   if (i > B + 1) return N;
-  const int64_t o = static_cast<int64_t>(offsets[i - 1]);
-  return o < 0 ? 0 : (o > N ? N : o);  // malformed offsets stay in bounds
+  const I o = offsets[i - 1];
+  return o < 0 ? 0 : (o > N ? N : static_cast<int32_t>(o));  // malformed offsets stay in bounds
 }
 
-template <typename I>
-__device__ __forceinline__ Span list_span(const I* offsets, int64_t B, int64_t N, int64_t i) {
-  const int64_t s = list_start(offsets, B, N, i), e = list_start(offsets, B, N, i + 1);
-  return {uniform64(s), __builtin_amdgcn_readfirstlane(static_cast<int32_t>(e > s ? e - s : 0))};
+// A block's tile: its list's rows and their partners' (queries' keys or keys'
+// queries), and its number in the list.
+struct Found {
+  Span own, other;
+  int32_t tile;
+};
+
+// Turns rotated within groups of 8, each group by one more than the last: lists
+// of a power of two of tiles would give one XCD, or one shader engine, the same
+// tile of every list, the longest or the shortest, as blocks go to both in turn.
+__device__ __forceinline__ int32_t rotated(int32_t turn, int32_t n) {
+  return turn < (n & ~7) ? (turn & ~7) | ((turn + (turn >> 3)) & 7) : turn;
 }
 
-// The list (0..B+1) that owns tile slot `slot`, and the tile's number in it.
-template <typename I>
-__device__ __forceinline__ int64_t find_list(const I* offsets, int64_t B, int64_t N, int bm_shift,
-                                             int64_t slot, int32_t* tile) {
-  int64_t lo = 0, n = B + 2;
-  int64_t key = 0;
-  while (n > 1) {
-    const int64_t step = (n + 63) >> 6;
-    const int64_t i = lo + lane_id() * step;
-    const bool in = i < lo + n && (list_start(offsets, B, N, i) >> bm_shift) + i <= slot;
-    const int c = __popcll(__ballot(in));  // the first lane's is always at most `slot`
-    const int64_t at = (c > 0 ? c - 1 : 0) * step;
-    lo += at;
-    n = n - at < step ? n - at : step;
-  }
-  key = (list_start(offsets, B, N, lo) >> bm_shift) + lo;
-  *tile = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(slot - key));
-  return uniform64(lo);
-}
-
-// The same for a causal call of up to 62 lists, by rank: tiles with more work
-// come first, across all lists (a block's time is its tile's length: the longest
-// must not start last).  Lane i holds list i with n tiles; tile t of them has
-// work t + 1 + c (QUERIES, c the keys before its queries in tiles) or n - t + c
-// (keys: the queries from its first one on).  There are F(w) tiles of work w or
-// more, so rank r has the largest w with F(w) > r and is the (r - F(w + 1))-th
-// list that has a tile of work w.  False if there are no more tiles.
-template <bool QUERIES, typename I>
-__device__ __forceinline__ bool find_ranked(const I* own, const I* other, int64_t B, int64_t N,
-                                            int64_t Nother, int bm_shift, int64_t rank, int64_t* list,
-                                            int32_t* tile) {
-  const int i = lane_id();
-  int n = 0, c = 0;
-  if (i < B + 2) {
-    const int64_t s = list_start(own, B, N, i), e = list_start(own, B, N, i + 1);
-    const int len = static_cast<int>(e > s ? e - s : 0);
-    n = (len + (1 << bm_shift) - 1) >> bm_shift;
-    if (QUERIES && i > 0 && i <= B) {
-      const int64_t os = list_start(other, B, Nother, i), oe = list_start(other, B, Nother, i + 1);
-      const int more = static_cast<int>(oe > os ? oe - os : 0) - len;
-      c = more > 0 ? more >> bm_shift : 0;
+// The tile of turn `turn`; false if there is none.  The one more tile is the
+// list's first (FIRST: queries, whose first tiles see the fewest keys) or last
+// (keys, whose last tiles meet the fewest queries).  Steps of 64 probes narrow the lists down to 63,
+// whose bounds on both sides one more load per lane brings (up to 61 lists cost
+// one trip to memory, up to 4,030 two: every block waits for them).
+template <bool FIRST, typename I>
+__device__ __forceinline__ bool find_list(const I* own, const I* other, int32_t B, int32_t N,
+                                          int32_t Nother, int bm_shift, int32_t turn, Found* f) {
+  const int whole = N >> bm_shift;
+  int lo = rotated(turn - whole, B + 2), n = 2;  // one more: the list is known
+  if (turn < whole) {
+    // Backwards where first tiles are short (the causal mask): long ones first.
+    turn = rotated(turn, whole);
+    if (FIRST) turn = whole - 1 - turn;
+    lo = 0, n = B + 2;
+    while (n > 63) {
+      const int step = (n + 63) >> 6;
+      const int i = lo + lane_id() * step;
+      const bool in = i < lo + n && (list_start(own, B, N, i) >> bm_shift) <= turn;
+      const int c = __popcll(__ballot(in));  // the first lane's is always at most `turn`
+      const int at = (c > 0 ? c - 1 : 0) * step;
+      lo += at;
+      n = n - at < step ? n - at : step;
     }
   }
-  auto lane_count = [&](int w) {  // tiles of this list with work w or more
-    const int k = n + c - (w - 1);
+  const int i = lo + lane_id();
+  const int s = list_start(own, B, N, i), o = list_start(other, B, Nother, i);
+  // The last list that starts at or before the turn (those before it with the
+  // same start have no whole tile).
+  const int c = turn < whole ? __popcll(__ballot(lane_id() < n && (s >> bm_shift) <= turn)) : 1;
+  const int at = c > 0 ? c - 1 : 0;  // at most 62
+  const int s0 = readlane_i32(s, at), s1 = readlane_i32(s, at + 1);
+  const int o0 = readlane_i32(o, at), o1 = readlane_i32(o, at + 1);
+  const int list = lo + at, mask = (1 << bm_shift) - 1;
+  const bool more = s1 > s0 && (s1 & mask) > (s0 & mask);
+  if (turn >= whole && !more) return false;
+  f->own = {s0, s1 > s0 ? s1 - s0 : 0};
+  f->other = {o0, list > 0 && list <= B && o1 > o0 ? o1 - o0 : 0};
+  if (turn >= whole) f->tile = FIRST ? 0 : (s1 >> bm_shift) - (s0 >> bm_shift);
+  else f->tile = turn - (s0 >> bm_shift) + (FIRST && more ? 1 : 0);
+  return true;
+}
+
+// Sum over the lanes up to and including this one.
+__device__ __forceinline__ int wave_prefix(int v) {
+  // row_shr 1, 2, 4, 8 within 16 lanes, then each row's last to the next rows.
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+
+// The same by rank, for up to 62 lists: tiles with more work come first, across
+// all lists (a block's time is its tile's length: the longest must not start
+// last).  A lane holds a list; under the causal mask tile t of n has work
+// t + 1 + c (QUERIES, c the keys before its queries in tiles) or n - t (keys:
+// the queries from its first one on), else every tile of a list has its
+// partners' number.  With F(w) the tiles of work w or more, rank r has the
+// largest w with F(w) > r and is number r - F(w + 1) of that work in the order
+// of the lists.  False if there are no more tiles.
+template <bool QUERIES, typename I>
+__device__ __forceinline__ bool find_ranked(const I* own, const I* other, int32_t B, int32_t N,
+                                            int32_t Nother, int bm_shift, bool causal, int32_t rank,
+                                            Found* f) {
+  const int i = lane_id();
+  const int s = list_start(own, B, N, i), os = list_start(other, B, Nother, i);
+  const int e = list_start(own, B, N, i + 1), oe = list_start(other, B, Nother, i + 1);
+  const int len = e > s ? e - s : 0;  // past the last list: N to N
+  const int olen = i > 0 && i <= B && oe > os ? oe - os : 0;
+  const int n = (len + (1 << bm_shift) - 1) >> bm_shift;
+  const int top = !causal ? 1 + (olen >> bm_shift)  // the most work of a tile of the list
+                  : n + (QUERIES && olen > len ? (olen - len) >> bm_shift : 0);
+  auto count = [&](int w) {  // tiles of this list with work w or more
+    if (!causal) return top >= w ? n : 0;
+    const int k = top - w + 1;
     return k < 0 ? 0 : (k < n ? k : n);
   };
-  auto total = [&](int w) {
-    int v = lane_count(w);
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
-    return __builtin_amdgcn_readfirstlane(v);
-  };
-  int lo = 0, hi = n + c + 1;  // F(lo) > rank >= F(hi)
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) {
-    const int v = __shfl_xor(hi, m, 64);
-    hi = v > hi ? v : hi;
+  auto total = [&](int w) { return readlane_i32(wave_prefix(count(w)), 63); };
+  if (rank >= total(0)) return false;
+  int lo = 0, hi = 1;  // F(lo) > rank >= F(hi)
+  while (total(hi) > rank) {
+    lo = hi;
+    hi *= 2;
   }
-  hi = __builtin_amdgcn_readfirstlane(hi);
-  if (rank >= total(1)) return false;
-  lo = 1;
   while (hi - lo > 1) {
     const int mid = lo + (hi - lo) / 2;
     if (total(mid) > rank) lo = mid;
     else hi = mid;
   }
-  const int k = static_cast<int>(rank) - total(lo + 1);
-  const bool has = lane_count(lo) > lane_count(lo + 1);
-  const uint64_t set = __ballot(has);
-  const bool me = has && __popcll(set & ((1ull << i) - 1)) == static_cast<unsigned>(k);
-  const int at = __builtin_ctzll(__ballot(me));
-  *list = at;
-  *tile = __builtin_amdgcn_readfirstlane(__shfl(QUERIES ? lo - 1 - c : n + c - lo, at, 64));
+  // Of work lo: this list's tiles, and those of the lists before it.
+  const int here = count(lo) - count(lo + 1);
+  const int k = rank - total(lo + 1) - (wave_prefix(here) - here);
+  const int at = __builtin_ctzll(__ballot(k >= 0 && k < here) | (1ull << 63));
+  f->own = {readlane_i32(s, at), readlane_i32(len, at)};
+  f->other = {readlane_i32(os, at), readlane_i32(olen, at)};
+  f->tile = readlane_i32(!causal ? k : QUERIES ? lo - 1 - (top - n) : n - lo, at);
   return true;
 }
 
-inline int64_t tile_slots(int64_t N, int64_t B, int bm) { return N / bm + B + 2; }
+inline int64_t tile_turns(int64_t N, int64_t B, int bm) { return N / bm + B + 2; }
 
 }  // namespace attn
 }  // namespace mx

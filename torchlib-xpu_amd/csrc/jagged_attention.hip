@@ -17,7 +17,7 @@ struct FwdArgs {
   int64_t q_row, q_head;           // strides in bytes
   int64_t k_row, k_head, v_row, v_head;
   const void *q_offsets, *k_offsets;
-  int64_t B, Nq, Nk;
+  int32_t B, Nq, Nk;
   int32_t H, G, D;                 // G query heads per key-value head
   int32_t causal;
   int32_t ranked;                  // find_ranked finds the tiles
@@ -30,32 +30,35 @@ struct FwdArgs {
 // go to the 8 XCDs in turn: with a multiple of 8 heads each XCD keeps H / 8
 // neighbouring heads (which share keys) and takes all their tiles, so its L2
 // holds few keys and the causal tiles, unequal in length, spread evenly.
-__device__ __forceinline__ void head_and_turn(int64_t bid, int H, int* head, int64_t* turn) {
+__device__ __forceinline__ void head_and_turn(uint32_t bid, uint32_t H, int* head, int* turn) {
   if (H % 8 == 0) {
-    const int per = H / 8;
-    const int64_t x = bid % 8, y = bid / 8;
-    *head = static_cast<int>(x * per + y % per);
+    const uint32_t per = H / 8, x = bid % 8, y = bid / 8;
+    *head = x * per + y % per;
     *turn = y / per;
   } else {
-    *head = static_cast<int>(bid % H);
+    *head = bid % H;
     *turn = bid / H;
   }
 }
 
-// Writes one lane's row of a transposed result: column l of acc is a row of
-// `out`, its values scaled and rounded to the output's type.
+// Writes a transposed result: column l of acc, scaled and rounded to the
+// output's type, is row l (of `rows`) at `base` of a contiguous [.., heads, D].
 template <typename T, int DP>
-__device__ __forceinline__ void store_columns(T* out, const f32x16* acc, float scale, int D, int h) {
+__device__ __forceinline__ void store_rows(void* base, const f32x16* acc, float scale, int rows,
+                                           int heads, int D, int l, int h) {
   typedef T x4 __attribute__((ext_vector_type(4)));
+  const uint32_t stride = static_cast<uint32_t>(heads) * D * 2;
+  const __amdgpu_buffer_rsrc_t r = make_rsrc(base, span_bytes(rows, stride, D * 2));
+  const uint32_t row = l < rows ? l * stride + h * 8 : kOutside;
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
     for (int i = 0; i < 16; i += 4) {
-      const int col = 32 * d + 8 * (i / 4) + 4 * h;
+      const int col = 32 * d + 8 * (i / 4);  // and 4 more from the other half-wave: D is a multiple of 8
       x4 w;
 #pragma unroll
       for (int e = 0; e < 4; ++e) w[e] = static_cast<T>(acc[d][i + e] * scale);
-      if (col < D) *reinterpret_cast<x4*>(out + col) = w;
+      __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, w), r, col < D ? row + col * 2 : kOutside, 0, 0);
     }
 }
 
@@ -72,7 +75,10 @@ __device__ __forceinline__ void load_rows(X8* f, const char* base, int rows, int
   }
 }
 
-constexpr int kBN = 64;  // keys per tile
+
+constexpr int kBN = 64;        // keys per tile
+constexpr int kRowWaves = 4;   // waves of 32 queries: tiles of 128
+constexpr int kRowShift = 7;
 
 // One block: NW waves, 32 queries each, of one list and head.  Tiles of 64 keys
 // and values go to LDS, the next one while this one is worked on.  Per tile a
@@ -80,37 +86,35 @@ constexpr int kBN = 64;  // keys per tile
 // queries in registers, and adds V^T P^T to its outputs, which are rescaled
 // only when a maximum has grown by more than 2^8.  Probabilities are rounded to
 // the input type for the second product; sums, maxima and outputs are fp32.
-template <typename T, typename I, int DP, int NW>
-__global__ void __launch_bounds__(NW * 64, 2) fwd_kernel(const FwdArgs a, int64_t slots) {
+template <typename T, typename I, int DP, int NS>
+__global__ void __launch_bounds__(kRowWaves * NS * 64, 2) fwd_kernel(const FwdArgs a) {
   using E = Elem<T>;
   using X8 = typename E::x8;
   using Ti = Tile<DP>;
-  constexpr int KS = DP / 16, DB = DP / 32, BM = NW * 32;
+  constexpr int KS = DP / 16, DB = DP / 32, BM = kRowWaves * 32;
   constexpr int kTileBytes = kBN * DP * 2;
-  __shared__ __attribute__((aligned(1024))) char lds[4 * kTileBytes];  // K0 V0 K1 V1
+  __shared__ __attribute__((aligned(1024))) char lds[NS * 4 * kTileBytes];  // K0 V0 K1 V1 per group
 
   int head;
-  int64_t turn;
-  int tile;
+  int turn;
   head_and_turn(blockIdx.x, a.H, &head, &turn);
   const I* qo = static_cast<const I*>(a.q_offsets);
   const I* ko = static_cast<const I*>(a.k_offsets);
-  constexpr int kShift = NW == 1 ? 5 : NW == 2 ? 6 : 7;
-  int64_t list;
+  Found f;
   if (a.ranked) {
-    if (!find_ranked<true>(qo, ko, a.B, a.Nq, a.Nk, kShift, turn, &list, &tile)) return;
-  } else {  // a list's last tiles first: the causal mask makes them its longest
-    list = find_list(qo, a.B, a.Nq, kShift, slots - 1 - turn, &tile);
+    if (!find_ranked<true>(qo, ko, a.B, a.Nq, a.Nk, kRowShift, a.causal != 0, turn, &f)) return;
+  } else {
+    if (!find_list<true>(qo, ko, a.B, a.Nq, a.Nk, kRowShift, turn, &f)) return;
   }
-  const Span sq = list_span(qo, a.B, a.Nq, list);
+  const Span sq = f.own, sk = f.other;
+  const int tile = f.tile;
   if (tile * BM >= sq.len) return;
-  Span sk{0, 0};
-  if (list > 0 && list <= a.B) sk = list_span(ko, a.B, a.Nk, list);
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, l = lane & 31, h = lane >> 5;
-  const int row0 = tile * BM + wave * 32;  // the wave's first query in the list
+  const int group = wave / kRowWaves;                   // of the key tiles j with j % NS == group
+  const int row0 = tile * BM + wave % kRowWaves * 32;  // the wave's first query in the list
   const int64_t q_base = sq.start + row0;
   const int rows = rows_left(sq.len, row0, 32);
   const int Lk = sk.len;
@@ -126,12 +130,13 @@ __global__ void __launch_bounds__(NW * 64, 2) fwd_kernel(const FwdArgs a, int64_
   // Queries: the B operand of K Q^T.
   X8 qf[KS];
   load_rows<X8, KS>(qf, a.q + q_base * a.q_row + head * a.q_head, rows, a.q_row, a.D, l, h);
+  __builtin_amdgcn_sched_barrier(0);
 
-  typename Ti::template Loader<kBN, NW * 64> lk, lv;
-  lk.init(tid, static_cast<uint32_t>(a.k_row), a.D / 8);
-  lv.init(tid, static_cast<uint32_t>(a.v_row), a.D / 8);
-  const char* kp = a.k + sk.start * a.k_row + (head / a.G) * a.k_head;
-  const char* vp = a.v + sk.start * a.v_row + (head / a.G) * a.v_head;
+  typename Ti::template Loader<kBN, kRowWaves * 64> lk, lv;
+  lk.init(tid % (kRowWaves * 64), static_cast<uint32_t>(a.k_row), a.D / 8);
+  lv.init(tid % (kRowWaves * 64), static_cast<uint32_t>(a.v_row), a.D / 8);
+  const char* kp = a.k + int64_t{sk.start} * a.k_row + (head / a.G) * a.k_head;
+  const char* vp = a.v + int64_t{sk.start} * a.v_row + (head / a.G) * a.v_head;
   f32x16 o[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) o[d] = f32x16{};
@@ -145,21 +150,21 @@ __global__ void __launch_bounds__(NW * 64, 2) fwd_kernel(const FwdArgs a, int64_
   auto load_tile = [&](int j, char* __restrict__ dst) __attribute__((always_inline)) {
     const int n = rows_left(Lk, j * kBN, kBN);
     lk.load(make_rsrc(kp + static_cast<int64_t>(j) * kBN * a.k_row,
-                      span_bytes(n, static_cast<uint32_t>(a.k_row), a.D * 2)), dst, wave);
+                      span_bytes(n, static_cast<uint32_t>(a.k_row), a.D * 2)), dst, wave % kRowWaves);
     lv.load(make_rsrc(vp + static_cast<int64_t>(j) * kBN * a.v_row,
                       span_bytes(n, static_cast<uint32_t>(a.v_row), a.D * 2)),
-            dst + kTileBytes, wave);
+            dst + kTileBytes, wave % kRowWaves);
   };
   auto work = [&](int j, const char* __restrict__ cur, uint32_t buf,
                   char* __restrict__ next) __attribute__((always_inline)) {
-    if (j + 1 < tiles) load_tile(j + 1, next);
+    if (j + NS < tiles) load_tile(j + NS, next);
     const int k0 = j * kBN;
     if (k0 >= wave_end) return;
     const uint32_t ra = opaque(at.row + buf);
 
-    f32x16 s[2];
+    f32x16 s[kBN / 32];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < kBN / 32; ++b) {
       s[b] = f32x16{};
 #pragma unroll
       for (int x = 0; x < KS; ++x)
@@ -169,7 +174,7 @@ __global__ void __launch_bounds__(NW * 64, 2) fwd_kernel(const FwdArgs a, int64_
     if (k0 + kBN > all_end) {  // the tile reaches past a query's last key
       const int last = mine - k0 - 4 * h;
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+      for (int b = 0; b < kBN / 32; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (32 * b + 8 * (i / 4) + i % 4 >= last) s[b][i] = -INFINITY;
@@ -177,7 +182,7 @@ __global__ void __launch_bounds__(NW * 64, 2) fwd_kernel(const FwdArgs a, int64_
 
     float top = s[0][0];
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < kBN / 32; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
     top = fmaxf(top, other_half(top));
@@ -191,9 +196,9 @@ __global__ void __launch_bounds__(NW * 64, 2) fwd_kernel(const FwdArgs a, int64_
     }
     const float mc = m == -INFINITY ? 0.0f : m * c2;
 
-    X8 p[4];
+    X8 p[kBN / 16];
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < kBN / 32; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float e = exp2_hw(__builtin_fmaf(s[b][i], c2, -mc));
@@ -203,7 +208,7 @@ __global__ void __launch_bounds__(NW * 64, 2) fwd_kernel(const FwdArgs a, int64_
 
     const uint32_t t0 = opaque(at.tr + buf), t1 = Ti::next8(t0);
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
+    for (int x = 0; x < kBN / 16; ++x)
 #pragma unroll
       for (int d = 0; d < DB; ++d) {
         const char* f = cur + kTileBytes + 16 * x * Ti::kRow;
@@ -212,19 +217,43 @@ __global__ void __launch_bounds__(NW * 64, 2) fwd_kernel(const FwdArgs a, int64_
       }
   };
 
-  if (tiles > 0) load_tile(0, lds);
-  for (int j = 0; j < tiles; ++j) {
-    wait_lds_loads();
-    __syncthreads();
-    work(j, lds, (j & 1) * 2 * kTileBytes, lds + ((j + 1) & 1) * 2 * kTileBytes);
+  char* const mine_lds = lds + group * 4 * kTileBytes;
+  if (group < tiles) load_tile(group, mine_lds);
+  for (int j = group, t = 0; t < (tiles + NS - 1) / NS; j += NS, ++t) {
+    wait_and_barrier<0>();
+    work(j, mine_lds, (t & 1) * 2 * kTileBytes, mine_lds + ((t + 1) & 1) * 2 * kTileBytes);
   }
 
   sum += other_half(sum);
+  if constexpr (NS == 2) {
+    // The second group's maxima, sums and outputs: 16 DB + 2 floats a lane.
+    static_assert(sizeof(lds) >= kRowWaves * 64 * (16 * DB + 2) * 4, "the join's room");
+    float* room = reinterpret_cast<float*>(lds) + wave % kRowWaves * 64 * (16 * DB + 2) + lane;
+    wait_and_barrier<0>();
+    if (group == 1) {
+      room[0] = m;
+      room[64] = sum;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) room[(2 + 16 * d + i) * 64] = o[d][i];
+    }
+    wait_and_barrier<0>();
+    if (group == 1) return;
+    const float mb = room[0], top = fmaxf(m, mb);
+    const float fa = top == -INFINITY ? 0.0f : exp2_hw((m - top) * c2);
+    const float fb = top == -INFINITY ? 0.0f : exp2_hw((mb - top) * c2);
+    sum = sum * fa + room[64] * fb;
+    m = top;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[d][i] = o[d][i] * fa + room[(2 + 16 * d + i) * 64] * fb;
+  }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  if (l >= rows) return;
-  store_columns<T, DP>(static_cast<T*>(a.out) + ((q_base + l) * a.H + head) * a.D, o, inv, a.D, h);
-  if (a.lse != nullptr && h == 0)
-    a.lse[head * a.Nq + q_base + l] = sum == 0.0f ? -INFINITY : m * a.scale + __logf(sum);
+  store_rows<T, DP>(static_cast<T*>(a.out) + (q_base * a.H + head) * a.D, o, inv, rows, a.H, a.D, l, h);
+  if (a.lse != nullptr && h == 0 && l < rows)
+    a.lse[int64_t{head} * a.Nq + q_base + l] = sum == 0.0f ? -INFINITY : m * a.scale + __logf(sum);
 }
 
 // ---------------------------------------------------------------------------
@@ -244,7 +273,7 @@ struct BwdArgs {
   const char *q, *k, *v, *out, *grad;  // bytes; out and grad with q's shape
   int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, g_row, g_head;
   const void *q_offsets, *k_offsets;
-  int64_t B, Nq, Nk;
+  int32_t B, Nq, Nk;
   int32_t H, Hkv, G, D;
   int32_t causal;
   int32_t ranked;                  // find_ranked finds the tiles
@@ -254,37 +283,35 @@ struct BwdArgs {
   void *dq, *dk, *dv;                  // contiguous
 };
 
-template <typename T, typename I, int DP, int NW>
-__global__ void __launch_bounds__(NW * 64, 2) bwd_q_kernel(const BwdArgs a, int64_t slots) {
+template <typename T, typename I, int DP, int NS>
+__global__ void __launch_bounds__(kRowWaves * NS * 64, 2) bwd_q_kernel(const BwdArgs a) {
   using E = Elem<T>;
   using X8 = typename E::x8;
   using Ti = Tile<DP>;
-  constexpr int KS = DP / 16, DB = DP / 32, BM = NW * 32;
+  constexpr int KS = DP / 16, DB = DP / 32, BM = kRowWaves * 32;
   constexpr int kTileBytes = kBN * DP * 2;
-  __shared__ __attribute__((aligned(1024))) char lds[4 * kTileBytes];
+  __shared__ __attribute__((aligned(1024))) char lds[NS * 4 * kTileBytes];
 
   int head;
-  int64_t turn;
-  int tile;
+  int turn;
   head_and_turn(blockIdx.x, a.H, &head, &turn);
   const I* qo = static_cast<const I*>(a.q_offsets);
   const I* ko = static_cast<const I*>(a.k_offsets);
-  constexpr int kShift = NW == 1 ? 5 : NW == 2 ? 6 : 7;
-  int64_t list;
+  Found f;
   if (a.ranked) {
-    if (!find_ranked<true>(qo, ko, a.B, a.Nq, a.Nk, kShift, turn, &list, &tile)) return;
-  } else {  // a list's last tiles first: the causal mask makes them its longest
-    list = find_list(qo, a.B, a.Nq, kShift, slots - 1 - turn, &tile);
+    if (!find_ranked<true>(qo, ko, a.B, a.Nq, a.Nk, kRowShift, a.causal != 0, turn, &f)) return;
+  } else {
+    if (!find_list<true>(qo, ko, a.B, a.Nq, a.Nk, kRowShift, turn, &f)) return;
   }
-  const Span sq = list_span(qo, a.B, a.Nq, list);
+  const Span sq = f.own, sk = f.other;
+  const int tile = f.tile;
   if (tile * BM >= sq.len) return;
-  Span sk{0, 0};
-  if (list > 0 && list <= a.B) sk = list_span(ko, a.B, a.Nk, list);
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, l = lane & 31, h = lane >> 5;
-  const int row0 = tile * BM + wave * 32;  // the wave's first query in the list
+  const int group = wave / kRowWaves;                   // of the key tiles j with j % NS == group
+  const int row0 = tile * BM + wave % kRowWaves * 32;  // the wave's first query in the list
   const int64_t q_base = sq.start + row0;
   const int rows = rows_left(sq.len, row0, 32);
   const int Lk = sk.len;
@@ -311,20 +338,20 @@ __global__ void __launch_bounds__(NW * 64, 2) bwd_q_kernel(const BwdArgs a, int6
         delta = __builtin_fmaf(static_cast<float>(of[s][e]), static_cast<float>(gf[s][e]), delta);
     delta += other_half(delta);
     if (l < rows) {
-      const int64_t at = head * a.Nq + q_base + l;
+      const int64_t at = int64_t{head} * a.Nq + q_base + l;
       lse2 = a.lse[at] * kLog2e;
-      if (h == 0) {
+      if (h == 0 && group == 0) {
         a.lse2[at] = lse2;
         a.delta[at] = delta;
       }
     }
   }
 
-  typename Ti::template Loader<kBN, NW * 64> lk, lv;
-  lk.init(tid, static_cast<uint32_t>(a.k_row), a.D / 8);
-  lv.init(tid, static_cast<uint32_t>(a.v_row), a.D / 8);
-  const char* kp = a.k + sk.start * a.k_row + (head / a.G) * a.k_head;
-  const char* vp = a.v + sk.start * a.v_row + (head / a.G) * a.v_head;
+  typename Ti::template Loader<kBN, kRowWaves * 64> lk, lv;
+  lk.init(tid % (kRowWaves * 64), static_cast<uint32_t>(a.k_row), a.D / 8);
+  lv.init(tid % (kRowWaves * 64), static_cast<uint32_t>(a.v_row), a.D / 8);
+  const char* kp = a.k + int64_t{sk.start} * a.k_row + (head / a.G) * a.k_head;
+  const char* vp = a.v + int64_t{sk.start} * a.v_row + (head / a.G) * a.v_head;
 
   f32x16 dq[DB];
 #pragma unroll
@@ -335,16 +362,16 @@ __global__ void __launch_bounds__(NW * 64, 2) bwd_q_kernel(const BwdArgs a, int6
   auto load_tile = [&](int j, char* __restrict__ dst) __attribute__((always_inline)) {
     const int n = rows_left(Lk, j * kBN, kBN);
     lk.load(make_rsrc(kp + static_cast<int64_t>(j) * kBN * a.k_row,
-                      span_bytes(n, static_cast<uint32_t>(a.k_row), a.D * 2)), dst, wave);
+                      span_bytes(n, static_cast<uint32_t>(a.k_row), a.D * 2)), dst, wave % kRowWaves);
     lv.load(make_rsrc(vp + static_cast<int64_t>(j) * kBN * a.v_row,
                       span_bytes(n, static_cast<uint32_t>(a.v_row), a.D * 2)),
-            dst + kTileBytes, wave);
+            dst + kTileBytes, wave % kRowWaves);
   };
   auto work = [&](int j, const char* __restrict__ cur, uint32_t buf,
                   char* __restrict__ next) __attribute__((always_inline)) {
-    if (j + 1 < tiles) load_tile(j + 1, next);
+    if (j + NS < tiles) load_tile(j + NS, next);
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < kBN / 32; ++b) {
       const int k0 = j * kBN + 32 * b;
       if (k0 >= wave_end) return;
       const uint32_t ra = opaque(at.row + buf), t0 = opaque(at.tr + buf), t1 = Ti::next8(t0);
@@ -379,14 +406,31 @@ __global__ void __launch_bounds__(NW * 64, 2) bwd_q_kernel(const BwdArgs a, int6
     }
   };
 
-  if (tiles > 0) load_tile(0, lds);
-  for (int j = 0; j < tiles; ++j) {
-    wait_lds_loads();
-    __syncthreads();
-    work(j, lds, (j & 1) * 2 * kTileBytes, lds + ((j + 1) & 1) * 2 * kTileBytes);
+  char* const mine_lds = lds + group * 4 * kTileBytes;
+  if (group < tiles) load_tile(group, mine_lds);
+  for (int j = group, t = 0; t < (tiles + NS - 1) / NS; j += NS, ++t) {
+    wait_and_barrier<0>();
+    work(j, mine_lds, (t & 1) * 2 * kTileBytes, mine_lds + ((t + 1) & 1) * 2 * kTileBytes);
   }
-  if (l >= rows) return;
-  store_columns<T, DP>(static_cast<T*>(a.dq) + ((q_base + l) * a.H + head) * a.D, dq, a.scale, a.D, h);
+
+  if constexpr (NS == 2) {
+    static_assert(sizeof(lds) >= kRowWaves * 64 * 16 * DB * 4, "the join's room");
+    float* room = reinterpret_cast<float*>(lds) + wave % kRowWaves * 64 * 16 * DB + lane;
+    wait_and_barrier<0>();
+    if (group == 1) {
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) room[(16 * d + i) * 64] = dq[d][i];
+    }
+    wait_and_barrier<0>();
+    if (group == 1) return;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dq[d][i] += room[(16 * d + i) * 64];
+  }
+  store_rows<T, DP>(static_cast<T*>(a.dq) + (q_base * a.H + head) * a.D, dq, a.scale, rows, a.H, a.D, l, h);
 }
 
 // The keys' launch: a wave owns 32 keys and their sums over every query head of
@@ -396,12 +440,12 @@ __global__ void __launch_bounds__(NW * 64, 2) bwd_q_kernel(const BwdArgs a, int6
 // scores come out with a key per lane.  D = 128 takes 192 registers for K, V,
 // dK and dV: scores are used up before dP is computed, which leaves two waves
 // per SIMD.
-template <typename T, typename I, int DP, int NK, int NQ>
-__global__ void __launch_bounds__(NK * NQ * 64, 2) bwd_kv_kernel(const BwdArgs a) {
+template <typename T, typename I, int DP, int NQ>
+__global__ void __launch_bounds__(kRowWaves * NQ * 64, 2) bwd_kv_kernel(const BwdArgs a) {
   using E = Elem<T>;
   using X8 = typename E::x8;
   using Ti = Tile<DP>;
-  constexpr int KS = DP / 16, DB = DP / 32, BM = NK * 32, BQ = 64 * NQ, THREADS = NK * NQ * 64;
+  constexpr int KS = DP / 16, DB = DP / 32, BM = kRowWaves * 32, BQ = 64 * NQ, THREADS = kRowWaves * NQ * 64;
   constexpr int kTileBytes = BQ * DP * 2;
   constexpr int kStat = BQ * 4;
   constexpr int kBuf = 2 * kTileBytes + 2 * kStat;  // Q, dO, lse2, delta
@@ -409,28 +453,25 @@ __global__ void __launch_bounds__(NK * NQ * 64, 2) bwd_kv_kernel(const BwdArgs a
   static_assert(NQ == 1 || 2 * kBuf >= BM * DP * 4, "the join's room");
 
   int kvh;
-  int64_t turn;
-  int tile;
+  int turn;
   head_and_turn(blockIdx.x, a.Hkv, &kvh, &turn);
   const I* qo = static_cast<const I*>(a.q_offsets);
   const I* ko = static_cast<const I*>(a.k_offsets);
-  constexpr int kShift = NK == 1 ? 5 : NK == 2 ? 6 : 7;
-  int64_t list;
+  Found f;
   if (a.ranked) {
-    if (!find_ranked<false>(ko, qo, a.B, a.Nk, a.Nq, kShift, turn, &list, &tile)) return;
+    if (!find_ranked<false>(ko, qo, a.B, a.Nk, a.Nq, kRowShift, a.causal != 0, turn, &f)) return;
   } else {
-    list = find_list(ko, a.B, a.Nk, kShift, turn, &tile);
+    if (!find_list<false>(ko, qo, a.B, a.Nk, a.Nq, kRowShift, turn, &f)) return;
   }
-  const Span sk = list_span(ko, a.B, a.Nk, list);
+  const Span sk = f.own, sq = f.other;
+  const int tile = f.tile;
   if (tile * BM >= sk.len) return;
-  Span sq{0, 0};
-  if (list > 0 && list <= a.B) sq = list_span(qo, a.B, a.Nq, list);
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int part = wave / NK;  // which 64 of a tile's queries
+  const int part = wave / kRowWaves;  // which 64 of a tile's queries
   const int lane = tid & 63, l = lane & 31, h = lane >> 5;
-  const int key0 = tile * BM + wave % NK * 32;
+  const int key0 = tile * BM + wave % kRowWaves * 32;
   const int64_t k_base = sk.start + key0;
   const int keys = rows_left(sk.len, key0, 32);
   const int Lq = sq.len;
@@ -464,11 +505,11 @@ __global__ void __launch_bounds__(NK * NQ * 64, 2) bwd_kv_kernel(const BwdArgs a
     lg.load(make_rsrc(a.grad + (qs + i0) * a.g_row + head * a.g_head,
                       span_bytes(n, static_cast<uint32_t>(a.g_row), a.D * 2)),
             dst + kTileBytes, wave);
-    const int64_t s0 = head * a.Nq + qs + i0;
-    for (int u = wave; u < 2 * NQ; u += NK * NQ) {  // 64 values each
-      const float* from = (u < NQ ? a.lse2 : a.delta) + s0;
-      load4_to_lds(make_rsrc(from, n * 4), dst + 2 * kTileBytes + u * 256,
-                   (u % NQ * 64 + lane_again()) * 4);
+    const int64_t s0 = int64_t{head} * a.Nq + qs + i0;
+    if (wave < 2 * NQ) {  // 64 values each
+      const float* from = (wave < NQ ? a.lse2 : a.delta) + s0;
+      load4_to_lds(make_rsrc(from, n * 4), dst + 2 * kTileBytes + wave * 256,
+                   (wave % NQ * 64 + lane_again()) * 4);
     }
   };
   auto work = [&](int t, const char* __restrict__ cur, uint32_t buf, char* __restrict__ next, int gn,
@@ -546,8 +587,7 @@ __global__ void __launch_bounds__(NK * NQ * 64, 2) bwd_kv_kernel(const BwdArgs a
   int g = 0, t = 0;
   for (int64_t i = 0; i < steps; ++i) {
     const int tn = t + 1 < per ? t + 1 : 0, gn = t + 1 < per ? g : g + 1;
-    wait_lds_loads();
-    __syncthreads();
+    wait_and_barrier<0>();
     work(t, lds, static_cast<uint32_t>(i & 1) * kBuf, lds + ((i + 1) & 1) * kBuf, gn, tn, i + 1 < steps);
     t = tn;
     g = gn;
@@ -555,7 +595,7 @@ __global__ void __launch_bounds__(NK * NQ * 64, 2) bwd_kv_kernel(const BwdArgs a
 
   if constexpr (NQ == 2) {
     // One lane's values of a block of columns: 16 x 64 floats per step.
-    float* room = reinterpret_cast<float*>(lds) + wave % NK * 32 * DP + lane;
+    float* room = reinterpret_cast<float*>(lds) + wave % kRowWaves * 32 * DP + lane;
 #pragma unroll
     for (int pass = 0; pass < 2; ++pass) {
       f32x16* x = pass == 0 ? dk : dv;
@@ -576,36 +616,66 @@ __global__ void __launch_bounds__(NK * NQ * 64, 2) bwd_kv_kernel(const BwdArgs a
     }
     if (part == 1) return;
   }
-  if (l >= keys) return;
-  const int64_t to = ((k_base + l) * a.Hkv + kvh) * a.D;
-  store_columns<T, DP>(static_cast<T*>(a.dk) + to, dk, a.scale, a.D, h);
-  store_columns<T, DP>(static_cast<T*>(a.dv) + to, dv, 1.0f, a.D, h);
+  const int64_t to = (k_base * a.Hkv + kvh) * a.D;
+  store_rows<T, DP>(static_cast<T*>(a.dk) + to, dk, a.scale, keys, a.Hkv, a.D, l, h);
+  store_rows<T, DP>(static_cast<T*>(a.dv) + to, dv, 1.0f, keys, a.Hkv, a.D, l, h);
 }
 
 // ---------------------------------------------------------------------------
 // Launches
 // ---------------------------------------------------------------------------
 
+
+// Waves beyond a block's four where the launch's tiles of 128 rows do not fill
+// the chip, on lists long enough to share out.  Times in us, 8 heads of 128:
+//   forward, key tiles over two groups: 1 list of 4096 94 -> 78, 16 lists of 128
+//   queries and 1128 keys 34.4 -> 32.5; 4 lists of 2048 (512 tiles) 58 -> 60;
+//   backward's keys, queries over two groups (whole backward): 1 x 4096
+//   310 -> 258, 4 x 2048 (512 tiles) 184 -> 173, 6 x 2048 211 -> 233, 16 x 512
+//   (512 tiles) 71 -> 81, the same with 2 key-value heads 127 -> 101.
+bool split_keys(int64_t Nq, int64_t Nk, int64_t B, int64_t H) {
+  return B > 0 && ceil_div(Nq, 128) * H <= num_cus() && Nk / B >= 512;
+}
+bool split_queries(int64_t Nq, int64_t Nk, int64_t B, int64_t Hkv, int64_t G) {
+  return B > 0 && ceil_div(Nk, 128) * Hkv <= 2 * num_cus() && Nq / B * G >= 1024;
+}
+
+int blocks_of(int64_t rows, int64_t B, int64_t heads, unsigned* blocks) {
+  const int64_t n = tile_turns(rows, B, 128) * heads;
+  MX_REQUIRE(n < (1ll << 31), "too many tiles: %lld", (long long)n);
+  *blocks = static_cast<unsigned>(n);
+  return MX_OK;
+}
+
 template <typename T, typename I, int DP>
 int launch_fwd(const FwdArgs& a, hipStream_t stream) {
-  constexpr int NW = 4;
-  const int64_t slots = tile_slots(a.Nq, a.B, NW * 32);
-  MX_REQUIRE(slots * a.H < (1ll << 31), "too many query tiles: %lld", (long long)(slots * a.H));
-  fwd_kernel<T, I, DP, NW><<<dim3(static_cast<unsigned>(slots * a.H)), NW * 64, 0, stream>>>(a, slots);
+  unsigned blocks;
+  if (int rc = blocks_of(a.Nq, a.B, a.H, &blocks)) return rc;
+  if (split_keys(a.Nq, a.Nk, a.B, a.H))
+    fwd_kernel<T, I, DP, 2><<<dim3(blocks), 512, 0, stream>>>(a);
+  else
+    fwd_kernel<T, I, DP, 1><<<dim3(blocks), 256, 0, stream>>>(a);
   MX_LAUNCH_CHECK();
   return MX_OK;
 }
 
 template <typename T, typename I, int DP>
 int launch_bwd(const BwdArgs& a, hipStream_t stream) {
-  constexpr int NW = 4;
-  const int64_t qslots = tile_slots(a.Nq, a.B, NW * 32), kslots = tile_slots(a.Nk, a.B, NW * 32);
-  MX_REQUIRE(qslots * a.H < (1ll << 31) && kslots * a.Hkv < (1ll << 31), "too many tiles: %lld",
-             (long long)(qslots * a.H));
-  if (a.Nq > 0)
-    bwd_q_kernel<T, I, DP, NW><<<dim3(static_cast<unsigned>(qslots * a.H)), NW * 64, 0, stream>>>(a, qslots);
-  if (a.Nk > 0 && a.dk != nullptr)
-    bwd_kv_kernel<T, I, DP, NW, 2><<<dim3(static_cast<unsigned>(kslots * a.Hkv)), NW * 128, 0, stream>>>(a);
+  unsigned qblocks, kblocks;
+  if (int rc = blocks_of(a.Nq, a.B, a.H, &qblocks)) return rc;
+  if (int rc = blocks_of(a.Nk, a.B, a.Hkv, &kblocks)) return rc;
+  if (a.Nq > 0) {
+    if (split_keys(a.Nq, a.Nk, a.B, a.H))
+      bwd_q_kernel<T, I, DP, 2><<<dim3(qblocks), 512, 0, stream>>>(a);
+    else
+      bwd_q_kernel<T, I, DP, 1><<<dim3(qblocks), 256, 0, stream>>>(a);
+  }
+  if (a.Nk > 0 && a.dk != nullptr) {
+    if (split_queries(a.Nq, a.Nk, a.B, a.Hkv, a.G))
+      bwd_kv_kernel<T, I, DP, 2><<<dim3(kblocks), 512, 0, stream>>>(a);
+    else
+      bwd_kv_kernel<T, I, DP, 1><<<dim3(kblocks), 256, 0, stream>>>(a);
+  }
   MX_LAUNCH_CHECK();
   return MX_OK;
 }
@@ -642,8 +712,9 @@ int check_problem(const mx_attention_problem* p) {
   MX_REQUIRE(p->dtype == MX_DTYPE_F16 || p->dtype == MX_DTYPE_BF16, "dtype %d is not fp16 or bf16", p->dtype);
   MX_REQUIRE(p->index_bytes == 4 || p->index_bytes == 8, "index_bytes %d", p->index_bytes);
   MX_REQUIRE(p->B >= 0 && p->Nq >= 0 && p->Nk >= 0, "negative size");
-  MX_REQUIRE(p->Nq <= MX_ATTENTION_MAX_ROWS && p->Nk <= MX_ATTENTION_MAX_ROWS, "more than %d rows",
-             MX_ATTENTION_MAX_ROWS);
+  MX_REQUIRE(p->Nq <= MX_ATTENTION_MAX_ROWS && p->Nk <= MX_ATTENTION_MAX_ROWS &&
+                 p->B <= MX_ATTENTION_MAX_ROWS,
+             "more than %d rows or lists", MX_ATTENTION_MAX_ROWS);
   MX_REQUIRE(p->H > 0 && p->Hkv > 0 && p->H % p->Hkv == 0,
              "%d query heads are no multiple of %d key-value heads", p->H, p->Hkv);
   MX_REQUIRE(p->D > 0 && p->D <= MX_ATTENTION_MAX_D && p->D % 8 == 0,
@@ -653,10 +724,13 @@ int check_problem(const mx_attention_problem* p) {
   return MX_OK;
 }
 
-// Tiles by rank: lists long enough that a tile's length tells in the launch's,
-// and few enough for a lane each.
+// Tiles by rank: lists few enough for a lane each, long enough that a tile's
+// length tells in the launch's, and more tiles than the chip holds at once (8
+// lists of 2048, 8 heads of 64, in us: forward 70 -> 55, backward 194 -> 158; 16
+// lists of 512: 24.9 either way, and 0.4 more where all start at once).
 int32_t ranked_tiles(const mx_attention_problem* p) {
-  return p->causal != 0 && p->B > 0 && p->B + 2 <= 64 && (p->Nq + p->Nk) / p->B >= 1024;
+  return p->B > 0 && p->B + 2 <= 64 && (p->Nq + p->Nk) / p->B >= 1024 &&
+         ceil_div(p->Nq, 128) * p->H > 2 * num_cus();
 }
 
 }  // namespace
@@ -682,7 +756,7 @@ extern "C" int mx_jagged_attention_forward(const mx_attention_problem* p, const 
   a.k_row = k->row_stride * 2, a.k_head = k->head_stride * 2;
   a.v_row = v->row_stride * 2, a.v_head = v->head_stride * 2;
   a.q_offsets = p->q_offsets, a.k_offsets = p->k_offsets;
-  a.B = p->B, a.Nq = p->Nq, a.Nk = p->Nk;
+  a.B = static_cast<int32_t>(p->B), a.Nq = static_cast<int32_t>(p->Nq), a.Nk = static_cast<int32_t>(p->Nk);
   a.H = p->H, a.G = p->H / p->Hkv, a.D = p->D;
   a.causal = p->causal, a.scale = p->scale;
   a.ranked = ranked_tiles(p);
@@ -729,7 +803,7 @@ extern "C" int mx_jagged_attention_backward(const mx_attention_problem* p, const
   a.o_row = out->row_stride * 2, a.o_head = out->head_stride * 2;
   a.g_row = grad_out->row_stride * 2, a.g_head = grad_out->head_stride * 2;
   a.q_offsets = p->q_offsets, a.k_offsets = p->k_offsets;
-  a.B = p->B, a.Nq = p->Nq, a.Nk = p->Nk;
+  a.B = static_cast<int32_t>(p->B), a.Nq = static_cast<int32_t>(p->Nq), a.Nk = static_cast<int32_t>(p->Nk);
   a.H = p->H, a.Hkv = p->Hkv, a.G = p->H / p->Hkv, a.D = p->D;
   a.causal = p->causal, a.scale = p->scale;
   a.ranked = ranked_tiles(p);
