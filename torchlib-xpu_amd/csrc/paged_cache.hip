@@ -103,13 +103,12 @@ struct StepArgs {
   int64_t q_row, q_head;   // bytes
   const void* lengths;
   int32_t lengths_bytes;
-  int32_t H, Hkv, G, D;
+  int32_t B, H, Hkv, G, D;
   int32_t head_blocks;     // of 16 query heads of a key-value head
-  int32_t splits;
-  int64_t chunk;           // keys of a split
+  int32_t workers;         // per head block: they share all tiles; 0: a block per sequence
   float scale;
   void* out;               // [B, H, D]
-  float* part;             // [B, H, splits, D + 2]: sums, then maximum and sum of weights
+  float* part;             // [workers, 2, H, D + 2]: sums, then maximum and sum of weights
 };
 
 constexpr int kStepWaves = 4;
@@ -131,14 +130,49 @@ __device__ __forceinline__ int64_t shfl64(int64_t v, int lane) {
   return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
 }
 
-// One block: a sequence, up to 16 query heads of one key-value head, one split
-// of its keys; its waves take tiles of 32 keys in turn.  Every key and value is
-// read once, straight into registers in the matrix operands' layouts (r = lane
-// % 16, g = lane / 16): K K-major (16 keys x 32 columns per 16x16x32 product,
-// a head per result column), V with 8 keys and DP / 16 columns per lane,
-// transposed in registers.
+// Tokens of sequence b that there are, and its tiles of 128 keys.
+constexpr int kTileKeys = kStepWaves * kStepKeys;
+
+__device__ __forceinline__ int32_t tokens_of(const StepArgs& a, int32_t b) {
+  const int64_t n = ld_index(a.lengths, a.lengths_bytes, b), most = a.c.width * a.c.page_size;
+  return static_cast<int32_t>(n < 0 ? 0 : (n < most ? n : most));
+}
+__device__ __forceinline__ int32_t tiles_of(int32_t tokens) { return (tokens + kTileKeys - 1) / kTileKeys; }
+
+// The sequences' tiles end to end are cut into equal shares, one for a worker
+// (and no more than tiles): share w begins at tile w total / shares.  A sequence's tiles may be cut anywhere;
+// what a share has of one that it does not have whole is joined later.  Shares
+// are equal whatever the lengths (a block per sequence waits for the longest).
+__device__ __forceinline__ int64_t share_begin(int64_t w, int64_t total, int64_t shares) {
+  return w * total / shares;
+}
+__device__ __forceinline__ int64_t share_of(int64_t tile, int64_t total, int64_t shares) {
+  return ((tile + 1) * shares - 1) / total;
+}
+
+// Tiles of all sequences, and of those before `b`.
+__device__ __forceinline__ int64_t count_tiles(const StepArgs& a, int32_t b, int64_t* before) {
+  int64_t all = 0, prior = 0;
+  for (int32_t i0 = 0; i0 < a.B; i0 += 64) {
+    const int32_t i = i0 + lane_id();
+    const int32_t n = i < a.B ? tiles_of(tokens_of(a, i)) : 0;
+    // 64 sequences of less than 2^24 tiles each.
+    all += readlane_i32(wave_prefix(n), 63);
+    if (i0 < b) prior += readlane_i32(wave_prefix(i < b ? n : 0), 63);
+  }
+  *before = prior;
+  return all;
+}
+
+// One block: up to 16 query heads of one key-value head, and a share of its
+// tiles (or one sequence); its waves take 32 of a tile's 128 keys each.  Every
+// key and value is read once, straight into registers in the matrix operands'
+// layouts (r = lane % 16, g = lane / 16): 16 keys x 32 columns of K per 16x16x32
+// product, a head per result column; 8 keys and DP / 16 columns of V per lane,
+// transposed in registers.  Probabilities are rounded to the cache's type for
+// the second product; scores, sums and the running maximum are fp32.
 template <typename T, int DP>
-__global__ void __launch_bounds__(kStepWaves * 64) step_kernel(const StepArgs a) {
+__global__ void __launch_bounds__(kStepWaves * 64, 2) step_kernel(const StepArgs a) {
   using E = Elem<T>;
   using X8 = typename E::x8;
   constexpr int KS = DP / 32;  // products along D of a score
@@ -147,191 +181,305 @@ __global__ void __launch_bounds__(kStepWaves * 64) step_kernel(const StepArgs a)
   __shared__ float sh_o[kStepWaves][16][DP + 1];
   __shared__ float sh_m[kStepWaves][16], sh_l[kStepWaves][16];
 
-  const int hb = blockIdx.x % a.head_blocks;
-  const int64_t y = blockIdx.x / a.head_blocks;
-  const int kvh = static_cast<int>(y % a.Hkv);
-  const int64_t z = y / a.Hkv;
-  const int split = static_cast<int>(z % a.splits);
-  const int64_t b = z / a.splits;
-  int64_t len = uniform64(ld_index(a.lengths, a.lengths_bytes, b));
-  const int64_t most = a.c.width * a.c.page_size;
-  len = len < most ? len : most;
-  const int64_t begin = split * a.chunk;
-  if (begin >= len && split > 0) return;
-  const int64_t end = begin + a.chunk < len ? begin + a.chunk : len;
-
+  const int heads_all = a.Hkv * a.head_blocks;
+  const int hh = blockIdx.x % heads_all, worker = blockIdx.x / heads_all;
+  const int kvh = hh / a.head_blocks, hb = hh % a.head_blocks;
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, r = lane & 15, g = lane >> 4;
   const int head0 = kvh * a.G + hb * 16;
   const int heads = a.G - hb * 16 < 16 ? a.G - hb * 16 : 16;
-
-  X8 qf[KS];
-#pragma unroll
-  for (int s = 0; s < KS; ++s) {
-    const int col = 32 * s + 8 * g;
-    i32x4 w{};
-    if (r < heads && col < a.D)
-      w = *reinterpret_cast<const i32x4*>(a.q + b * a.q_row + (head0 + r) * a.q_head + col * 2);
-    qf[s] = __builtin_bit_cast(X8, w);
-  }
-
   const float c2 = a.scale * kLog2e;
-  float m = -INFINITY, sum = 0.0f;
-  f32x4 o[EV];
-#pragma unroll
-  for (int t = 0; t < EV; ++t) o[t] = f32x4{};
-  const int32_t* row = a.c.table + b * a.c.table_row;
   const char* kb = a.c.k + kvh * a.c.k_head;
   const char* vb = a.c.v + kvh * a.c.v_head;
 
-  for (int64_t k0 = begin + wave * kStepKeys; k0 < end; k0 += kStepWaves * kStepKeys) {
-    // Lane i finds the place of key k0 + i % 32.
-    const int64_t key = k0 + (lane & 31);
-    int slot = 0;
-    int64_t page = -1;
-    if (key < end) page = row[page_of(a.c, key, &slot)];
-    const bool there = page >= 0 && page < a.c.pages;
-    const uint32_t seen = static_cast<uint32_t>(__ballot(there));
-    const int64_t koff = there ? page * a.c.k_page + slot * a.c.k_slot : 0;
-    const int64_t voff = there ? page * a.c.v_page + slot * a.c.v_slot : 0;
-
-    i32x4 kw[2][KS];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const char* p = kb + shfl64(koff, 16 * u + r);
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const int col = 32 * s + 8 * g;
-        kw[u][s] = i32x4{};
-        if (col < a.D) kw[u][s] = *reinterpret_cast<const i32x4*>(p + col * 2);
+  // The share: tiles [at, stop) counted from sequence b's first one.
+  int32_t b = worker, len;
+  int64_t at = 0, stop = 0;
+  if (a.workers == 0) {
+    len = __builtin_amdgcn_readfirstlane(tokens_of(a, b));
+    stop = len > 0 ? tiles_of(len) : 1;  // an empty sequence is written too
+  } else {
+    int64_t prior;
+    const int64_t total = count_tiles(a, 0, &prior);
+    const int64_t shares = total < a.workers ? total : a.workers;  // none is empty
+    if (worker >= shares) return;
+    at = share_begin(worker, total, shares);
+    stop = share_begin(worker + 1, total, shares);
+    len = 0;
+    for (int32_t i0 = 0; i0 < a.B; i0 += 64) {
+      const int32_t i = i0 + lane_id();
+      const int32_t tokens = i < a.B ? tokens_of(a, i) : 0;
+      const int32_t upto = wave_prefix(tiles_of(tokens));
+      const int32_t here = readlane_i32(upto, 63);
+      if (at >= here) {
+        at -= here;
+        stop -= here;
+        continue;
       }
-    }
-    VP vw[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int n = 16 * (i / 4) + 4 * g + i % 4;
-      const char* p = vb + shfl64(voff, n);
-      vw[i] = VP{};
-      if (EV * r < a.D && ((seen >> n) & 1)) vw[i] = *reinterpret_cast<const VP*>(p + EV * r * 2);
-    }
-
-    f32x4 s[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      s[u] = f32x4{};
-#pragma unroll
-      for (int x = 0; x < KS; ++x) s[u] = E::mfma16(__builtin_bit_cast(X8, kw[u][x]), qf[x], s[u]);
-    }
-    if (seen != 0xffffffffu) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (((seen >> (16 * u + 4 * g + i)) & 1) == 0) s[u][i] = -INFINITY;
-    }
-    float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                      fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-    if (__any((top - m) * c2 > 8.0f)) {
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, other_half(top));
-      const float m2 = fmaxf(m, top);
-      const float f = m2 == -INFINITY ? 1.0f : exp2_hw((m - m2) * c2);
-      sum *= f;
-#pragma unroll
-      for (int t = 0; t < EV; ++t) o[t] *= f;
-      m = m2;
-    }
-    const float mc = m == -INFINITY ? 0.0f : m * c2;
-    X8 p;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float e = exp2_hw(__builtin_fmaf(s[i / 4][i % 4], c2, -mc));
-      sum += e;
-      p[i] = static_cast<T>(e);
-    }
-    typedef T TV __attribute__((ext_vector_type(EV)));
-#pragma unroll
-    for (int t = 0; t < EV; ++t) {
-      X8 vt;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) vt[i] = __builtin_bit_cast(TV, vw[i])[t];
-      o[t] = E::mfma16(vt, p, o[t]);
+      const int l = __builtin_ctzll(__ballot(at < upto));
+      b = i0 + l;
+      len = readlane_i32(tokens, l);
+      const int32_t skip = readlane_i32(upto, l) - tiles_of(len);
+      at -= skip;
+      stop -= skip;
+      break;
     }
   }
 
-  // The waves' sums: lane (r, g) holds head r, columns EV (4 g + i) + t.
-  sum += __shfl_xor(sum, 16, 64);
-  sum += other_half(sum);
-  if (g == 0) {
-    sh_m[wave][r] = m;
-    sh_l[wave][r] = sum;
-  }
+  while (true) {
+    const int32_t n = tiles_of(len);
+    const int32_t t0 = static_cast<int32_t>(at), t1 = static_cast<int32_t>(stop < n ? stop : n);
+    const int32_t end = t1 * kTileKeys < len ? t1 * kTileKeys : len;
+
+    X8 qf[KS];
 #pragma unroll
-  for (int t = 0; t < EV; ++t)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sh_o[wave][r][EV * (4 * g + i) + t] = o[t][i];
-  __syncthreads();
-  for (int u = tid; u < heads * a.D; u += kStepWaves * 64) {
-    const int n = u / a.D, d = u - n * a.D;
-    float mm = sh_m[0][n];
-#pragma unroll
-    for (int w = 1; w < kStepWaves; ++w) mm = fmaxf(mm, sh_m[w][n]);
-    float acc = 0.0f, l = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kStepWaves; ++w) {
-      const float f = mm == -INFINITY ? 0.0f : exp2_hw((sh_m[w][n] - mm) * c2);
-      acc += f * sh_o[w][n][d];
-      l += f * sh_l[w][n];
+    for (int s = 0; s < KS; ++s) {
+      const int col = 32 * s + 8 * g;
+      i32x4 w{};
+      if (r < heads && col < a.D)
+        w = *reinterpret_cast<const i32x4*>(a.q + b * a.q_row + (head0 + r) * a.q_head + col * 2);
+      qf[s] = __builtin_bit_cast(X8, w);
     }
-    const int64_t at = b * a.H + head0 + n;
-    if (a.splits == 1) {
-      static_cast<T*>(a.out)[at * a.D + d] = static_cast<T>(l == 0.0f ? 0.0f : acc / l);
-    } else {
-      float* to = a.part + (at * a.splits + split) * (a.D + 2);
-      to[d] = acc;
-      if (d == 0) {
-        to[a.D] = mm;
-        to[a.D + 1] = l;
+    float m = -INFINITY, sum = 0.0f;
+    f32x4 o[EV];
+#pragma unroll
+    for (int t = 0; t < EV; ++t) o[t] = f32x4{};
+
+    // Lane i finds the place of key i % 32 of a tile; the table's entries of
+    // the next tile are asked for before this one's keys.
+    const int32_t* row = a.c.table + b * a.c.table_row;
+    auto entry = [&](int32_t k0, int* slot) {
+      const int32_t key = k0 + (lane & 31);
+      *slot = 0;
+      return key < end ? row[page_of(a.c, key, slot)] : -1;
+    };
+    const int32_t first = t0 * kTileKeys + wave * kStepKeys;
+    int slot_next = 0;
+    int32_t page_next = entry(first, &slot_next);
+    for (int32_t k0 = first; k0 < end; k0 += kTileKeys) {
+      const int64_t page = page_next;
+      const int slot = slot_next;
+      page_next = entry(k0 + kTileKeys, &slot_next);
+      const bool there = page >= 0 && page < a.c.pages;
+      const uint32_t seen = static_cast<uint32_t>(__ballot(there));
+      const int64_t koff = there ? page * a.c.k_page + slot * a.c.k_slot : 0;
+      const int64_t voff = there ? page * a.c.v_page + slot * a.c.v_slot : 0;
+
+      i32x4 kw[2][KS];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const char* p = kb + shfl64(koff, 16 * u + r);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const int col = 32 * s + 8 * g;
+          kw[u][s] = i32x4{};
+          if (col < a.D) kw[u][s] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(p + col * 2));
+        }
+      }
+      VP vw[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int nk = 16 * (i / 4) + 4 * g + i % 4;
+        const char* p = vb + shfl64(voff, nk);
+        vw[i] = VP{};
+        if (EV * r < a.D && ((seen >> nk) & 1)) vw[i] = __builtin_nontemporal_load(reinterpret_cast<const VP*>(p + EV * r * 2));
+      }
+
+      f32x4 s[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        s[u] = f32x4{};
+#pragma unroll
+        for (int x = 0; x < KS; ++x) s[u] = E::mfma16(__builtin_bit_cast(X8, kw[u][x]), qf[x], s[u]);
+      }
+      if (seen != 0xffffffffu) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (((seen >> (16 * u + 4 * g + i)) & 1) == 0) s[u][i] = -INFINITY;
+      }
+      float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                        fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+      if (__any((top - m) * c2 > 8.0f)) {
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, other_half(top));
+        const float m2 = fmaxf(m, top);
+        const float f = m2 == -INFINITY ? 1.0f : exp2_hw((m - m2) * c2);
+        sum *= f;
+#pragma unroll
+        for (int t = 0; t < EV; ++t) o[t] *= f;
+        m = m2;
+      }
+      const float mc = m == -INFINITY ? 0.0f : m * c2;
+      X8 p;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float e = exp2_hw(__builtin_fmaf(s[i / 4][i % 4], c2, -mc));
+        sum += e;
+        p[i] = static_cast<T>(e);
+      }
+      typedef T TV __attribute__((ext_vector_type(EV)));
+#pragma unroll
+      for (int t = 0; t < EV; ++t) {
+        X8 vt;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) vt[i] = __builtin_bit_cast(TV, vw[i])[t];
+        o[t] = E::mfma16(vt, p, o[t]);
       }
     }
+
+    // The waves' sums: lane (r, g) holds head r, columns EV (4 g + i) + t.
+    sum += __shfl_xor(sum, 16, 64);
+    sum += other_half(sum);
+    if (g == 0) {
+      sh_m[wave][r] = m;
+      sh_l[wave][r] = sum;
+    }
+#pragma unroll
+    for (int t = 0; t < EV; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sh_o[wave][r][EV * (4 * g + i) + t] = o[t][i];
+    __syncthreads();
+    const bool whole = t0 == 0 && t1 == n;
+    for (int u = tid; u < heads * a.D; u += kStepWaves * 64) {
+      const int nh = u / a.D, d = u - nh * a.D;
+      float mm = sh_m[0][nh];
+#pragma unroll
+      for (int w = 1; w < kStepWaves; ++w) mm = fmaxf(mm, sh_m[w][nh]);
+      float acc = 0.0f, l = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kStepWaves; ++w) {
+        const float f = mm == -INFINITY ? 0.0f : exp2_hw((sh_m[w][nh] - mm) * c2);
+        acc += f * sh_o[w][nh][d];
+        l += f * sh_l[w][nh];
+      }
+      if (whole) {
+        static_cast<T*>(a.out)[(static_cast<int64_t>(b) * a.H + head0 + nh) * a.D + d] =
+            static_cast<T>(l == 0.0f ? 0.0f : acc / l);
+      } else {
+        // A sequence begun by an earlier share, or one that a later share ends.
+        float* to = a.part + ((static_cast<int64_t>(worker) * 2 + (t0 > 0 ? 0 : 1)) * a.H + head0 + nh) * (a.D + 2);
+        to[d] = acc;
+        if (d == 0) {
+          to[a.D] = mm;
+          to[a.D + 1] = l;
+        }
+      }
+    }
+    if (stop <= n) return;
+    // The next sequence that has tokens.
+    stop -= n;
+    at = 0;
+    do {
+      ++b;
+      len = __builtin_amdgcn_readfirstlane(tokens_of(a, b));
+    } while (len == 0 && b + 1 < a.B);
+    if (len == 0) return;
+    __syncthreads();
   }
 }
 
-// Joins the splits of a sequence and head, in their order: one wave each.
+// Joins the shares of a sequence and head, in their order, and writes the
+// sequences without tokens; one that a share had whole is written already.  A
+// block per sequence and head: its waves take equal runs of the shares.
+constexpr int kJoinMost = 16;
+
 template <typename T>
-__global__ void __launch_bounds__(64) join_kernel(const StepArgs a) {
-  const int64_t at = blockIdx.x;
-  const int64_t b = at / a.H;
-  int64_t len = ld_index(a.lengths, a.lengths_bytes, b);
-  const int64_t most = a.c.width * a.c.page_size;
-  len = len < most ? len : most;
-  int n = len > 0 ? static_cast<int>((len + a.chunk - 1) / a.chunk) : 1;
-  n = n < a.splits ? n : a.splits;
-  const float* part = a.part + at * a.splits * (a.D + 2);
+__global__ void __launch_bounds__(kJoinMost * 64) join_kernel(const StepArgs a) {
+  __shared__ float sh_o[kJoinMost][MX_ATTENTION_MAX_D], sh_m[kJoinMost], sh_l[kJoinMost];
+  const int32_t b = blockIdx.x / a.H, head = blockIdx.x % a.H;
+  T* out = static_cast<T*>(a.out) + static_cast<int64_t>(blockIdx.x) * a.D;
+  const int32_t n = __builtin_amdgcn_readfirstlane(tiles_of(tokens_of(a, b)));
+  if (n == 0) {
+    for (int d = threadIdx.x; d < a.D; d += blockDim.x) out[d] = static_cast<T>(0.0f);
+    return;
+  }
+  int64_t before;
+  const int64_t total = count_tiles(a, b, &before);
+  const int64_t all = total < a.workers ? total : a.workers;
+  const int64_t w0 = share_of(before, total, all), w1 = share_of(before + n - 1, total, all);
+  if (w0 == w1) return;
+  const int shares = static_cast<int>(w1 - w0 + 1);
+  const int waves = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = lane_id();
+  const int from = shares * wave / waves, to = shares * (wave + 1) / waves;
   const float c2 = a.scale * kLog2e;
-  float mm = -INFINITY;
-  for (int s = 0; s < n; ++s) mm = fmaxf(mm, part[s * (a.D + 2) + a.D]);
-  for (int d = threadIdx.x; d < a.D; d += 64) {
-    float acc = 0.0f, l = 0.0f;
-    for (int s = 0; s < n; ++s) {
-      const float* p = part + s * (a.D + 2);
-      const float f = mm == -INFINITY ? 0.0f : exp2_hw((p[a.D] - mm) * c2);
-      acc += f * p[d];
-      l += f * p[a.D + 1];
+  float m = -INFINITY, l = 0.0f, x0 = 0.0f, x1 = 0.0f;
+  auto place = [&](int s) {
+    return a.part + (((w0 + s) * 2 + (s == 0 ? 1 : 0)) * a.H + head) * (a.D + 2);
+  };
+  for (int s0 = from; s0 < to; s0 += 64) {
+    const int k = to - s0 < 64 ? to - s0 : 64;
+    float ms = -INFINITY, ls = 0.0f;
+    if (lane < k) {
+      const float* p = place(s0 + lane);
+      ms = p[a.D];
+      ls = p[a.D + 1];
     }
-    static_cast<T*>(a.out)[at * a.D + d] = static_cast<T>(l == 0.0f ? 0.0f : acc / l);
+    float top = ms;
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+    const float m2 = fmaxf(m, top);
+    const float base = m2 == -INFINITY ? 0.0f : m2;
+    const float old = exp2_hw((m - base) * c2);
+    const float f = exp2_hw((ms - base) * c2);
+    l = l * old + wave_sum(f * ls);
+    x0 *= old;
+    x1 *= old;
+    m = m2;
+    for (int s = 0; s < k; s += 8) {  // 8 shares' sums asked for at once
+      float v0[8], v1[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        v0[u] = v1[u] = 0.0f;
+        if (s + u < k) {
+          const float* p = place(s0 + s + u);
+          if (lane < a.D) v0[u] = p[lane];
+          if (lane + 64 < a.D) v1[u] = p[lane + 64];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float fs = __uint_as_float(readlane_i32(__float_as_uint(f), s + u));
+        x0 += fs * v0[u];
+        x1 += fs * v1[u];
+      }
+    }
+  }
+  sh_o[wave][lane] = x0;
+  sh_o[wave][lane + 64] = x1;
+  if (lane == 0) {
+    sh_m[wave] = m;
+    sh_l[wave] = l;
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < a.D; d += blockDim.x) {
+    float mm = sh_m[0];
+    for (int w = 1; w < waves; ++w) mm = fmaxf(mm, sh_m[w]);
+    const float base = mm == -INFINITY ? 0.0f : mm;
+    float acc = 0.0f, sum = 0.0f;
+    for (int w = 0; w < waves; ++w) {
+      const float f = exp2_hw((sh_m[w] - base) * c2);
+      acc += f * sh_o[w][d];
+      sum += f * sh_l[w];
+    }
+    out[d] = static_cast<T>(sum == 0.0f ? 0.0f : acc / sum);
   }
 }
 
-// Splits of the keys: enough blocks to fill the chip, of at least 256 keys.
-void plan_splits(int64_t B, int32_t Hkv, int32_t head_blocks, int64_t most, int32_t* splits, int64_t* chunk) {
-  const int64_t blocks = B * Hkv * head_blocks;
-  const int64_t want = blocks > 0 ? ceil_div(static_cast<int64_t>(num_cus()) * 4, blocks) : 1;
-  int64_t c = ceil_div(ceil_div(most, want > 0 ? want : 1), 128) * 128;
-  if (c < 256) c = 256;
-  *chunk = c;
-  *splits = static_cast<int32_t>(most > 0 ? ceil_div(most, c) : 1);
+// Workers of a call: two blocks for every CU (64 ragged sequences of up to 4096
+// tokens, 8 x 128: a block per sequence in halves 147 us, shares with one, two
+// and three blocks a CU 119, 106 and 122), or 0, a block per sequence and head,
+// where these are enough to even out by themselves (1024 of up to 200 tokens, 8
+// x 64: 71 us, in shares 108; 256 of up to 2000, 8 x 128: 219, in shares 205)
+// or no sequence has two tiles.
+int32_t plan_workers(int64_t B, int32_t heads, int64_t most) {
+  const int64_t tiles = ceil_div(most, kTileKeys);
+  if (tiles <= 1 || B * heads >= 8 * static_cast<int64_t>(num_cus())) return 0;
+  const int64_t w = ceil_div(static_cast<int64_t>(num_cus()) * 2, heads);
+  return static_cast<int32_t>(w < B * tiles ? w : B * tiles);
 }
 
 int32_t head_blocks_of(int32_t H, int32_t Hkv) { return static_cast<int32_t>(ceil_div(H / Hkv, 16)); }
@@ -368,20 +516,24 @@ Cache cache_of(const mx_paged_cache* c) {
 }
 
 template <typename T, int DP>
-int launch_step(const StepArgs& a, int64_t B, hipStream_t s) {
-  const int64_t blocks = B * a.splits * a.Hkv * a.head_blocks;
-  MX_REQUIRE(blocks < (1ll << 31) && B * a.H < (1ll << 31), "too many sequences: %lld", (long long)B);
+int launch_step(const StepArgs& a, hipStream_t s) {
+  const int64_t blocks = static_cast<int64_t>(a.workers > 0 ? a.workers : a.B) * a.Hkv * a.head_blocks;
+  const int64_t joins = static_cast<int64_t>(a.B) * a.H;
+  MX_REQUIRE(blocks < (1ll << 31) && joins < (1ll << 31), "too many sequences: %d", a.B);
   step_kernel<T, DP><<<dim3(static_cast<unsigned>(blocks)), kStepWaves * 64, 0, s>>>(a);
-  if (a.splits > 1) join_kernel<T><<<dim3(static_cast<unsigned>(B * a.H)), 64, 0, s>>>(a);
+  if (a.workers > 0) {
+    const int waves = a.workers / a.B < 8 ? 1 : a.workers / a.B < 32 ? 4 : kJoinMost;
+    join_kernel<T><<<dim3(static_cast<unsigned>(joins)), waves * 64, 0, s>>>(a);
+  }
   MX_LAUNCH_CHECK();
   return MX_OK;
 }
 
 template <typename T>
-int step_by_width(const StepArgs& a, int64_t B, hipStream_t s) {
-  if (a.D <= 32) return launch_step<T, 32>(a, B, s);
-  if (a.D <= 64) return launch_step<T, 64>(a, B, s);
-  return launch_step<T, 128>(a, B, s);
+int step_by_width(const StepArgs& a, hipStream_t s) {
+  if (a.D <= 32) return launch_step<T, 32>(a, s);
+  if (a.D <= 64) return launch_step<T, 64>(a, s);
+  return launch_step<T, 128>(a, s);
 }
 
 }  // namespace
@@ -428,10 +580,8 @@ extern "C" size_t mx_paged_cache_attention_workspace_bytes(const mx_paged_cache*
                                                            int32_t H, int32_t Hkv, int32_t D) {
   using namespace mx::attn;
   if (cache == nullptr || B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || D <= 0) return 0;
-  int32_t splits = 1;
-  int64_t chunk = 0;
-  plan_splits(B, Hkv, head_blocks_of(H, Hkv), cache->table_width * cache->page_size, &splits, &chunk);
-  return splits == 1 ? 0 : static_cast<size_t>(B) * H * splits * (D + 2) * sizeof(float);
+  const int64_t workers = plan_workers(B, Hkv * head_blocks_of(H, Hkv), cache->table_width * cache->page_size);
+  return static_cast<size_t>(workers) * 2 * H * (D + 2) * sizeof(float);
 }
 
 extern "C" int mx_paged_cache_attention(const mx_paged_cache* cache, int32_t dtype,
@@ -442,7 +592,8 @@ extern "C" int mx_paged_cache_attention(const mx_paged_cache* cache, int32_t dty
   using namespace mx::attn;
   mx::clear_error();
   if (int rc = check_cache(cache, dtype, Hkv, D)) return rc;
-  MX_REQUIRE(B >= 0, "negative size");
+  MX_REQUIRE(B >= 0 && B < (1ll << 31), "%lld sequences", (long long)B);
+  MX_REQUIRE(cache->table_width * cache->page_size < (1ll << 31), "more than 2^31 tokens in a row of the table");
   MX_REQUIRE(H > 0 && H % Hkv == 0, "%d query heads are no multiple of %d key-value heads", H, Hkv);
   MX_REQUIRE(std::isfinite(scale) && scale > 0.0f, "scale must be positive and finite");
   MX_REQUIRE(lengths_bytes == 4 || lengths_bytes == 8, "lengths_bytes %d", lengths_bytes);
@@ -458,15 +609,15 @@ extern "C" int mx_paged_cache_attention(const mx_paged_cache* cache, int32_t dty
   a.q = static_cast<const char*>(q->data);
   a.q_row = q->row_stride * 2, a.q_head = q->head_stride * 2;
   a.lengths = lengths, a.lengths_bytes = lengths_bytes;
-  a.H = H, a.Hkv = Hkv, a.G = H / Hkv, a.D = D;
+  a.B = static_cast<int32_t>(B), a.H = H, a.Hkv = Hkv, a.G = H / Hkv, a.D = D;
   a.head_blocks = head_blocks_of(H, Hkv);
   a.scale = scale;
   a.out = out;
-  plan_splits(B, Hkv, a.head_blocks, cache->table_width * cache->page_size, &a.splits, &a.chunk);
+  a.workers = plan_workers(B, Hkv * a.head_blocks, cache->table_width * cache->page_size);
   const size_t need = mx_paged_cache_attention_workspace_bytes(cache, B, H, Hkv, D);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return mx::set_error(MX_EWORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
   a.part = static_cast<float*>(workspace);
   const hipStream_t s = mx::as_stream(stream);
-  return dtype == MX_DTYPE_BF16 ? step_by_width<__bf16>(a, B, s) : step_by_width<_Float16>(a, B, s);
+  return dtype == MX_DTYPE_BF16 ? step_by_width<__bf16>(a, s) : step_by_width<_Float16>(a, s);
 }
