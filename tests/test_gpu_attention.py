@@ -284,3 +284,82 @@ def test_refusals(dev):
     q = x.detach().requires_grad_()
     with pytest.raises(RuntimeError, match="second derivative"):
         torch.autograd.grad(op(q, x, x, o).sum(), q, create_graph=True)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("H,D,n", [(1, 64, 200), (4, 128, 1100)])
+def test_masked_keys_and_values_do_not_show(dev, bad, H, D, n):
+    """Under the causal mask what later events hold reaches no earlier one, and
+    what a query sees of it reaches the query."""
+    o = torch.tensor([0, n], device=dev)
+    q, k, v = (make(n, H, D, "bfloat16", i).to(dev) for i in range(3))
+    want = torch.ops.mx_fbgemm.jagged_attention(q, k, v, o)
+    for at in (1, 70, n - 1):
+        for which in (k, v):
+            keep = which[at].clone()
+            which[at] = bad
+            got = torch.ops.mx_fbgemm.jagged_attention(q, k, v, o)
+            which[at] = keep
+            # Rows that share a wave with a bad one are worked out another way:
+            # equal to the two ways' roundings.
+            g, w = got[:at].double(), want[:at].double()
+            assert torch.isfinite(g).all()
+            assert ((g - w).norm() <= 2 * 2.0 ** -8 * w.norm())
+            assert torch.equal(got[: at // 128 * 128], want[: at // 128 * 128])
+            if which is v:
+                assert not torch.isfinite(got[at:]).any()
+            else:
+                assert not torch.isfinite(got[at:]).all()
+
+
+@pytest.mark.parametrize("low", [-60000.0, -3.0e38])
+def test_scores_of_the_types_lowest_values(dev, low):
+    """Keys that give scores near the lowest numbers: weights of zero, no NaN."""
+    dtype = "float16" if low > -65505 else "bfloat16"
+    n = 130
+    q, k, v = (make(n, 1, 32, dtype, i) for i in range(3))
+    q = q.abs()
+    k[10:20] = low
+    o = offsets_of([n])
+    to = torch.from_numpy(o).to(dev)
+    out = torch.ops.mx_fbgemm.jagged_attention(q.to(dev), k.to(dev), v.to(dev), to, to, True)
+    assert torch.isfinite(out).all()
+    keep = [i for i in range(n) if not 10 <= i < 20]
+    some = torch.ops.mx_fbgemm.jagged_attention(
+        q[keep].to(dev), k[keep].to(dev), v[keep].to(dev), torch.tensor([0, 120], device=dev),
+        torch.tensor([0, 120], device=dev), True)
+    g, w = out[keep].double(), some.double()
+    assert ((g - w).norm() <= 2 * 2.0 ** -8 * w.norm())
+
+
+@pytest.mark.parametrize("H,Hkv,D,n", [(1, 1, 64, 200), (4, 2, 128, 1100)])
+def test_masked_pairs_do_not_show_in_gradients(dev, H, Hkv, D, n):
+    """What a row holds reaches only gradients of pairs that the mask lets through:
+    a bad key or value not the earlier queries', a bad query or incoming gradient
+    not the later keys'."""
+    o = torch.tensor([0, n], device=dev)
+    q, g = (make(n, H, D, "bfloat16", i) for i in (0, 1))
+    k, v = (make(n, Hkv, D, "bfloat16", i) for i in (2, 3))
+    r = attention(*(x.double().numpy() for x in (q, k, v)), [0, n], [0, n], True, D ** -0.5, "bfloat16",
+                  g.double().numpy())
+    q, k, v, g = (x.to(dev) for x in (q, k, v, g))
+
+    def near(got, want, tol, s, what):
+        check(got[s].double().cpu().numpy(), want[s], tol[s], what)
+
+    for at in (1, 70, n - 2):
+        for name, x in (("q", q), ("k", k), ("v", v), ("g", g)):
+            keep = x[at].clone()
+            x[at] = float("nan")
+            leaves = [t.detach().clone().requires_grad_() for t in (q, k, v)]
+            out = torch.ops.mx_fbgemm.jagged_attention(*leaves, o)
+            dq, dk, dv = torch.autograd.grad(out, leaves, g)
+            x[at] = keep
+            if name in "kv":
+                near(dq, r.dq, r.dq_tol, slice(0, at), f"dq before a bad {name}")
+                assert torch.isnan(dq[at:]).all()
+            else:
+                near(dk, r.dk, r.dk_tol, slice(at + 1, n), f"dk after a bad {name}")
+                near(dv, r.dv, r.dv_tol, slice(at + 1, n), f"dv after a bad {name}")
+                near(dq, r.dq, r.dq_tol, slice(at + 1, n), f"dq after a bad {name}")
+                assert torch.isnan(dk[: at + 1]).all()

@@ -80,8 +80,80 @@ constexpr int kBN = 64;        // keys per tile
 constexpr int kRowWaves = 4;   // waves of 32 queries: tiles of 128
 constexpr int kRowShift = 7;
 
-// One block: NW waves, 32 queries each, of one list and head.  Tiles of 64 keys
-// and values go to LDS, the next one while this one is worked on.  Per tile a
+// This lane's row f (its half of the columns) times the row at p, summed over
+// both half-waves.
+template <int DP, typename X8>
+__device__ __forceinline__ float dot_row(const X8* f, const char* p, int D, int h) {
+  float s = 0.0f;
+#pragma unroll
+  for (int x = 0; x < DP / 16; ++x)
+    if ((2 * x + h) * 8 < D) {
+      const X8 k = *reinterpret_cast<const X8*>(p + (2 * x + h) * 16);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        s = __builtin_fmaf(static_cast<float>(f[x][e]), static_cast<float>(k[e]), s);
+    }
+  return s + other_half(s);
+}
+
+// acc = acc * f + w * (the row at p), in the columns of a transposed result.
+template <typename T, int DP>
+__device__ __forceinline__ void add_row(f32x16* acc, float f, float w, const char* p, int D, int h) {
+  typedef T x4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const int col = 32 * d + 8 * (i / 4) + 4 * h;
+      if (col >= D) continue;
+      const x4 v = *reinterpret_cast<const x4*>(p + col * 2);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[d][i + e] = acc[d][i + e] * f + w * static_cast<float>(v[e]);
+    }
+}
+
+// Whether a value of this lane's is infinite or NaN.
+template <int DP>
+__device__ __forceinline__ bool not_finite(const f32x16* acc) {
+  float any = 0.0f;
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) any = __builtin_fmaf(acc[d][i], 0.0f, any);  // 0, or NaN
+  return any != 0.0f;
+}
+
+// A wave's queries once more, key by key and only over the keys that each one
+// sees.  The matrix product of a tile that a query sees in part multiplies the
+// values it does not see by 0, and 0 times an infinity or NaN is NaN: a wave
+// that ends with such an output takes this way, so that what a masked value
+// holds never shows.  (Values of finite inputs never come here.)
+template <typename T, int DP, typename X8>
+__device__ __forceinline__ void rows_key_by_key(const X8* qf, const char* kp, int64_t k_row,
+                                                const char* vp, int64_t v_row, int D, float c2,
+                                                int end, int mine, int h, f32x16* o, float* m_out,
+                                                float* sum_out) {
+  float m = -INFINITY, sum = 0.0f;
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d) o[d] = f32x16{};
+#pragma unroll 1
+  for (int j = 0; j < end; ++j, kp += k_row, vp += v_row) {
+    const float s = dot_row<DP>(qf, kp, D, h);
+    if (j >= mine) continue;
+    const float m2 = fmaxf(m, s), base = m2 == -INFINITY ? 0.0f : m2;
+    const float f = exp2_hw((m - base) * c2), p = exp2_hw((s - base) * c2);
+    m = m2;
+    sum = sum * f + p;
+    add_row<T, DP>(o, f, p, vp, D, h);
+  }
+  *m_out = m;
+  *sum_out = sum;
+}
+
+// One block: four waves, 32 queries each, of one list and head (twice four with
+// NS = 2: two groups take alternate tiles of keys, and join their sums through
+// LDS at the end).  Tiles of 64 keys and values go to LDS, the next one while
+// this one is worked on.  Per tile a
 // wave computes K Q^T (a query per lane), the running maximum and sum of its
 // queries in registers, and adds V^T P^T to its outputs, which are rescaled
 // only when a maximum has grown by more than 2^8.  Probabilities are rounded to
@@ -250,6 +322,8 @@ __global__ void __launch_bounds__(kRowWaves * NS * 64, 2) fwd_kernel(const FwdAr
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[d][i] = o[d][i] * fa + room[(2 + 16 * d + i) * 64] * fb;
   }
+  if (a.causal && __any(l < rows && not_finite<DP>(o)))
+    rows_key_by_key<T, DP>(qf, kp, a.k_row, vp, a.v_row, a.D, c2, wave_end, mine, h, o, &m, &sum);
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   store_rows<T, DP>(static_cast<T*>(a.out) + (q_base * a.H + head) * a.D, o, inv, rows, a.H, a.D, l, h);
   if (a.lse != nullptr && h == 0 && l < rows)
@@ -430,6 +504,21 @@ __global__ void __launch_bounds__(kRowWaves * NS * 64, 2) bwd_q_kernel(const Bwd
 #pragma unroll
       for (int i = 0; i < 16; ++i) dq[d][i] += room[(16 * d + i) * 64];
   }
+  if (a.causal && __any(l < rows && not_finite<DP>(dq))) {
+    // As in the forward: keys that a query does not see leave the products.  (The
+    // rows again, for registers' sake.)
+    X8 qr[KS], gr[KS];
+    load_rows<X8, KS>(qr, a.q + q_base * a.q_row + head * a.q_head, rows, a.q_row, a.D, l, h);
+    load_rows<X8, KS>(gr, a.grad + q_base * a.g_row + head * a.g_head, rows, a.g_row, a.D, l, h);
+#pragma unroll
+    for (int d = 0; d < DB; ++d) dq[d] = f32x16{};
+#pragma unroll 1
+    for (int j = 0; j < wave_end; ++j, kp += a.k_row, vp += a.v_row) {
+      const float s = dot_row<DP>(qr, kp, a.D, h), dp = dot_row<DP>(gr, vp, a.D, h);
+      if (j < mine)
+        add_row<T, DP>(dq, 1.0f, exp2_hw(__builtin_fmaf(s, c2, -lse2)) * (dp - delta), kp, a.D, h);
+    }
+  }
   store_rows<T, DP>(static_cast<T*>(a.dq) + (q_base * a.H + head) * a.D, dq, a.scale, rows, a.H, a.D, l, h);
 }
 
@@ -479,7 +568,6 @@ __global__ void __launch_bounds__(kRowWaves * NQ * 64, 2) bwd_kv_kernel(const Bw
   // From the first query that sees a key of the block, to a whole 64.
   const int first = a.causal && tile * BM > shift ? (tile * BM - shift) / 64 * 64 : 0;
   const int per = Lq > first ? (Lq - first + BQ - 1) / BQ : 0;
-  const int64_t steps = static_cast<int64_t>(per) * a.G;
 
   X8 kf[KS], vf[KS];
   load_rows<X8, KS>(kf, a.k + k_base * a.k_row + kvh * a.k_head, keys, a.k_row, a.D, l, h);
@@ -523,7 +611,8 @@ __global__ void __launch_bounds__(kRowWaves * NQ * 64, 2) bwd_kv_kernel(const Bw
       const uint32_t from32 = buf + 32 * b * Ti::kRow;
       const uint32_t ra = opaque(at.row + from32), t0 = opaque(at.tr + from32), t1 = Ti::next8(t0);
       const char* gt = cur + kTileBytes;
-      const char* st = cur + buf + 2 * kTileBytes + (64 * part + 32 * b + 4 * h) * 4;
+      const int lc = lane_again() & 31, h4 = lane_again() >> 5 << 2;
+      const char* st = cur + buf + 2 * kTileBytes + (64 * part + 32 * b + h4) * 4;
       f32x16 s{}, dp{};
 #pragma unroll
       for (int x = 0; x < KS; ++x) s = E::mfma32(lds_read16<X8>(cur + Ti::step2(ra, x)), kf[x], s);
@@ -536,7 +625,7 @@ __global__ void __launch_bounds__(kRowWaves * NQ * 64, 2) bwd_kv_kernel(const Bw
       }
       // Query i0 + r sees key0 + l if r >= key0 + l - shift - i0.
       const bool masked = a.causal && key0 + 31 > i0 + shift;
-      const int from = key0 + l - shift - i0 - 4 * h;
+      const int from = key0 + lc - shift - i0 - h4;
       if (masked) {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
@@ -583,12 +672,12 @@ __global__ void __launch_bounds__(kRowWaves * NQ * 64, 2) bwd_kv_kernel(const Bw
     }
   };
 
-  if (steps > 0) load_tile(0, 0, lds);
-  int g = 0, t = 0;
-  for (int64_t i = 0; i < steps; ++i) {
+  if (per > 0) load_tile(0, 0, lds);
+  uint32_t buf = 0;
+  for (int g = 0, t = 0; per > 0 && g < a.G; buf = kBuf - buf) {
     const int tn = t + 1 < per ? t + 1 : 0, gn = t + 1 < per ? g : g + 1;
     wait_and_barrier<0>();
-    work(t, lds, static_cast<uint32_t>(i & 1) * kBuf, lds + ((i + 1) & 1) * kBuf, gn, tn, i + 1 < steps);
+    work(t, lds, buf, lds + (kBuf - buf), gn, tn, gn < a.G);
     t = tn;
     g = gn;
   }
@@ -616,9 +705,35 @@ __global__ void __launch_bounds__(kRowWaves * NQ * 64, 2) bwd_kv_kernel(const Bw
     }
     if (part == 1) return;
   }
+  // Counted anew: they would take registers through the loop.
+  const int le = lane_again() & 31, he = lane_again() >> 5;
+  if (a.causal && __any(le < keys && (not_finite<DP>(dk) || not_finite<DP>(dv)))) {
+    // As in the forward: queries that do not see a key leave its products.  (The
+    // rows again, for registers' sake.)
+    X8 kr[KS], vr[KS];
+    load_rows<X8, KS>(kr, a.k + k_base * a.k_row + kvh * a.k_head, keys, a.k_row, a.D, le, he);
+    load_rows<X8, KS>(vr, a.v + k_base * a.v_row + kvh * a.v_head, keys, a.v_row, a.D, le, he);
+#pragma unroll
+    for (int d = 0; d < DB; ++d) dk[d] = dv[d] = f32x16{};
+#pragma unroll 1
+    for (int u = 0; u < a.G; ++u) {
+      const int head = kvh * a.G + u;
+#pragma unroll 1
+      for (int i = first; i < Lq; ++i) {
+        const char* qp = a.q + (qs + i) * a.q_row + head * a.q_head;
+        const char* gp = a.grad + (qs + i) * a.g_row + head * a.g_head;
+        const int64_t at_i = int64_t{head} * a.Nq + qs + i;
+        const float s = dot_row<DP>(kr, qp, a.D, he), dp = dot_row<DP>(vr, gp, a.D, he);
+        if (key0 + le > i + shift) continue;
+        const float p = exp2_hw(__builtin_fmaf(s, c2, -a.lse2[at_i]));
+        add_row<T, DP>(dv, 1.0f, p, gp, a.D, he);
+        add_row<T, DP>(dk, 1.0f, p * (dp - a.delta[at_i]), qp, a.D, he);
+      }
+    }
+  }
   const int64_t to = (k_base * a.Hkv + kvh) * a.D;
-  store_rows<T, DP>(static_cast<T*>(a.dk) + to, dk, a.scale, keys, a.Hkv, a.D, l, h);
-  store_rows<T, DP>(static_cast<T*>(a.dv) + to, dv, 1.0f, keys, a.Hkv, a.D, l, h);
+  store_rows<T, DP>(static_cast<T*>(a.dk) + to, dk, a.scale, keys, a.Hkv, a.D, le, he);
+  store_rows<T, DP>(static_cast<T*>(a.dv) + to, dv, 1.0f, keys, a.Hkv, a.D, le, he);
 }
 
 // ---------------------------------------------------------------------------
