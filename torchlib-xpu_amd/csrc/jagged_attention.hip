@@ -14,8 +14,8 @@ namespace {
 
 struct FwdArgs {
   const char *q, *k, *v;           // bytes
-  int64_t q_row, q_head;           // strides in bytes
-  int64_t k_row, k_head, v_row, v_head;
+  uint32_t q_row, k_row, v_row;    // strides in bytes (at most 2^24)
+  int64_t q_head, k_head, v_head;
   const void *q_offsets, *k_offsets;
   int32_t B, Nq, Nk;
   int32_t H, G, D;                 // G query heads per key-value head
@@ -86,13 +86,15 @@ template <int DP, typename X8>
 __device__ __forceinline__ float dot_row(const X8* f, const char* p, int D, int h) {
   float s = 0.0f;
 #pragma unroll
-  for (int x = 0; x < DP / 16; ++x)
+  for (int x = 0; x < DP / 16; ++x) {
     if ((2 * x + h) * 8 < D) {
       const X8 k = *reinterpret_cast<const X8*>(p + (2 * x + h) * 16);
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         s = __builtin_fmaf(static_cast<float>(f[x][e]), static_cast<float>(k[e]), s);
     }
+    asm volatile("" ::: "memory");  // a piece at a time: few registers
+  }
   return s + other_half(s);
 }
 
@@ -109,6 +111,7 @@ __device__ __forceinline__ void add_row(f32x16* acc, float f, float w, const cha
       const x4 v = *reinterpret_cast<const x4*>(p + col * 2);
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[d][i + e] = acc[d][i + e] * f + w * static_cast<float>(v[e]);
+      asm volatile("" ::: "memory");
     }
 }
 
@@ -205,8 +208,8 @@ __global__ void __launch_bounds__(kRowWaves * NS * 64, 2) fwd_kernel(const FwdAr
   __builtin_amdgcn_sched_barrier(0);
 
   typename Ti::template Loader<kBN, kRowWaves * 64> lk, lv;
-  lk.init(tid % (kRowWaves * 64), static_cast<uint32_t>(a.k_row), a.D / 8);
-  lv.init(tid % (kRowWaves * 64), static_cast<uint32_t>(a.v_row), a.D / 8);
+  lk.init(tid % (kRowWaves * 64), a.k_row, a.D / 8);
+  lv.init(tid % (kRowWaves * 64), a.v_row, a.D / 8);
   const char* kp = a.k + int64_t{sk.start} * a.k_row + (head / a.G) * a.k_head;
   const char* vp = a.v + int64_t{sk.start} * a.v_row + (head / a.G) * a.v_head;
   f32x16 o[DB];
@@ -222,9 +225,9 @@ __global__ void __launch_bounds__(kRowWaves * NS * 64, 2) fwd_kernel(const FwdAr
   auto load_tile = [&](int j, char* __restrict__ dst) __attribute__((always_inline)) {
     const int n = rows_left(Lk, j * kBN, kBN);
     lk.load(make_rsrc(kp + static_cast<int64_t>(j) * kBN * a.k_row,
-                      span_bytes(n, static_cast<uint32_t>(a.k_row), a.D * 2)), dst, wave % kRowWaves);
+                      span_bytes(n, a.k_row, a.D * 2)), dst, wave % kRowWaves);
     lv.load(make_rsrc(vp + static_cast<int64_t>(j) * kBN * a.v_row,
-                      span_bytes(n, static_cast<uint32_t>(a.v_row), a.D * 2)),
+                      span_bytes(n, a.v_row, a.D * 2)),
             dst + kTileBytes, wave % kRowWaves);
   };
   auto work = [&](int j, const char* __restrict__ cur, uint32_t buf,
@@ -322,7 +325,7 @@ __global__ void __launch_bounds__(kRowWaves * NS * 64, 2) fwd_kernel(const FwdAr
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[d][i] = o[d][i] * fa + room[(2 + 16 * d + i) * 64] * fb;
   }
-  if (a.causal && __any(l < rows && not_finite<DP>(o)))
+  if (__builtin_expect(a.causal && __any(l < rows && not_finite<DP>(o)), 0))
     rows_key_by_key<T, DP>(qf, kp, a.k_row, vp, a.v_row, a.D, c2, wave_end, mine, h, o, &m, &sum);
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   store_rows<T, DP>(static_cast<T*>(a.out) + (q_base * a.H + head) * a.D, o, inv, rows, a.H, a.D, l, h);
@@ -345,7 +348,8 @@ __global__ void __launch_bounds__(kRowWaves * NS * 64, 2) fwd_kernel(const FwdAr
 
 struct BwdArgs {
   const char *q, *k, *v, *out, *grad;  // bytes; out and grad with q's shape
-  int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, g_row, g_head;
+  uint32_t q_row, k_row, v_row, o_row, g_row;
+  int64_t q_head, k_head, v_head, o_head, g_head;
   const void *q_offsets, *k_offsets;
   int32_t B, Nq, Nk;
   int32_t H, Hkv, G, D;
@@ -358,7 +362,7 @@ struct BwdArgs {
 };
 
 template <typename T, typename I, int DP, int NS>
-__global__ void __launch_bounds__(kRowWaves * NS * 64, 2) bwd_q_kernel(const BwdArgs a) {
+__global__ void __launch_bounds__(kRowWaves * NS * 64, DP <= 64 ? 4 : NS == 1 && DP == 96 ? 3 : 2) bwd_q_kernel(const BwdArgs a) {
   using E = Elem<T>;
   using X8 = typename E::x8;
   using Ti = Tile<DP>;
@@ -422,8 +426,8 @@ __global__ void __launch_bounds__(kRowWaves * NS * 64, 2) bwd_q_kernel(const Bwd
   }
 
   typename Ti::template Loader<kBN, kRowWaves * 64> lk, lv;
-  lk.init(tid % (kRowWaves * 64), static_cast<uint32_t>(a.k_row), a.D / 8);
-  lv.init(tid % (kRowWaves * 64), static_cast<uint32_t>(a.v_row), a.D / 8);
+  lk.init(tid % (kRowWaves * 64), a.k_row, a.D / 8);
+  lv.init(tid % (kRowWaves * 64), a.v_row, a.D / 8);
   const char* kp = a.k + int64_t{sk.start} * a.k_row + (head / a.G) * a.k_head;
   const char* vp = a.v + int64_t{sk.start} * a.v_row + (head / a.G) * a.v_head;
 
@@ -436,14 +440,40 @@ __global__ void __launch_bounds__(kRowWaves * NS * 64, 2) bwd_q_kernel(const Bwd
   auto load_tile = [&](int j, char* __restrict__ dst) __attribute__((always_inline)) {
     const int n = rows_left(Lk, j * kBN, kBN);
     lk.load(make_rsrc(kp + static_cast<int64_t>(j) * kBN * a.k_row,
-                      span_bytes(n, static_cast<uint32_t>(a.k_row), a.D * 2)), dst, wave % kRowWaves);
+                      span_bytes(n, a.k_row, a.D * 2)), dst, wave % kRowWaves);
     lv.load(make_rsrc(vp + static_cast<int64_t>(j) * kBN * a.v_row,
-                      span_bytes(n, static_cast<uint32_t>(a.v_row), a.D * 2)),
+                      span_bytes(n, a.v_row, a.D * 2)),
             dst + kTileBytes, wave % kRowWaves);
   };
   auto work = [&](int j, const char* __restrict__ cur, uint32_t buf,
                   char* __restrict__ next) __attribute__((always_inline)) {
     if (j + NS < tiles) load_tile(j + NS, next);
+    if (j == 0 && wave_end <= kBN) {
+      // These queries see no key past this tile: delta = sum_j p_ij dP_ij in fp32
+      // comes from the tile itself, at the price of its scores once more.  From
+      // the rounded output it is off by that rounding, which shows most where few
+      // keys share a large gradient (256 lists of up to 512: dQ's error against
+      // 64 bits 2.6e-3 -> 2.4e-3, its largest halved).
+      float sum = 0.0f;
+#pragma unroll 1
+      for (int k0 = 0; k0 < wave_end; k0 += 32) {
+        const uint32_t ra = opaque(at.row + buf + k0 * Ti::kRow);
+        f32x16 s{}, dp{};
+#pragma unroll
+        for (int x = 0; x < KS; ++x) {
+          s = E::mfma32(lds_read16<X8>(cur + Ti::step2(ra, x)), qf[x], s);
+          dp = E::mfma32(lds_read16<X8>(cur + kTileBytes + Ti::step2(ra, x)), gf[x], dp);
+        }
+        const int last = mine - k0 - 4 * h;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float w = exp2_hw(__builtin_fmaf(s[i], c2, -lse2)) * dp[i];
+          sum += 8 * (i / 4) + i % 4 >= last ? 0.0f : w;
+        }
+      }
+      delta = sum + other_half(sum);
+      if (h == 0 && l < rows) a.delta[int64_t{head} * a.Nq + q_base + l] = delta;
+    }
 #pragma unroll
     for (int b = 0; b < kBN / 32; ++b) {
       const int k0 = j * kBN + 32 * b;
@@ -504,7 +534,7 @@ __global__ void __launch_bounds__(kRowWaves * NS * 64, 2) bwd_q_kernel(const Bwd
 #pragma unroll
       for (int i = 0; i < 16; ++i) dq[d][i] += room[(16 * d + i) * 64];
   }
-  if (a.causal && __any(l < rows && not_finite<DP>(dq))) {
+  if (__builtin_expect(a.causal && __any(l < rows && not_finite<DP>(dq)), 0)) {
     // As in the forward: keys that a query does not see leave the products.  (The
     // rows again, for registers' sake.)
     X8 qr[KS], gr[KS];
@@ -538,7 +568,12 @@ __global__ void __launch_bounds__(kRowWaves * NQ * 64, 2) bwd_kv_kernel(const Bw
   constexpr int kTileBytes = BQ * DP * 2;
   constexpr int kStat = BQ * 4;
   constexpr int kBuf = 2 * kTileBytes + 2 * kStat;  // Q, dO, lse2, delta
-  __shared__ __attribute__((aligned(1024))) char lds[2 * kBuf];
+  // The last piece of V waits in LDS where the registers run out: a spilled one
+  // is loaded from memory, and its wait is one for the tiles in flight too (4 x
+  // 4096, 16 heads of 128: backward 1047 -> 1021 us).
+  constexpr bool kKeep = DP == 128 && NQ == 2;
+  constexpr int kInRegs = kKeep ? KS - 1 : KS;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * kBuf + (kKeep ? THREADS * 16 : 0)];
   static_assert(NQ == 1 || 2 * kBuf >= BM * DP * 4, "the join's room");
 
   int kvh;
@@ -572,10 +607,11 @@ __global__ void __launch_bounds__(kRowWaves * NQ * 64, 2) bwd_kv_kernel(const Bw
   X8 kf[KS], vf[KS];
   load_rows<X8, KS>(kf, a.k + k_base * a.k_row + kvh * a.k_head, keys, a.k_row, a.D, l, h);
   load_rows<X8, KS>(vf, a.v + k_base * a.v_row + kvh * a.v_head, keys, a.v_row, a.D, l, h);
+  if constexpr (kKeep) *reinterpret_cast<X8*>(lds + 2 * kBuf + tid * 16) = vf[KS - 1];
 
   typename Ti::template Loader<BQ, THREADS> lq, lg;
-  lq.init(tid, static_cast<uint32_t>(a.q_row), a.D / 8);
-  lg.init(tid, static_cast<uint32_t>(a.g_row), a.D / 8);
+  lq.init(tid, a.q_row, a.D / 8);
+  lg.init(tid, a.g_row, a.D / 8);
   const int64_t qs = sq.start;
 
   f32x16 dk[DB], dv[DB];
@@ -589,9 +625,9 @@ __global__ void __launch_bounds__(kRowWaves * NQ * 64, 2) bwd_kv_kernel(const Bw
     const int i0 = first + t * BQ;
     const int n = rows_left(Lq, i0, BQ);
     lq.load(make_rsrc(a.q + (qs + i0) * a.q_row + head * a.q_head,
-                      span_bytes(n, static_cast<uint32_t>(a.q_row), a.D * 2)), dst, wave);
+                      span_bytes(n, a.q_row, a.D * 2)), dst, wave);
     lg.load(make_rsrc(a.grad + (qs + i0) * a.g_row + head * a.g_head,
-                      span_bytes(n, static_cast<uint32_t>(a.g_row), a.D * 2)),
+                      span_bytes(n, a.g_row, a.D * 2)),
             dst + kTileBytes, wave);
     const int64_t s0 = int64_t{head} * a.Nq + qs + i0;
     if (wave < 2 * NQ) {  // 64 values each
@@ -645,7 +681,10 @@ __global__ void __launch_bounds__(kRowWaves * NQ * 64, 2) bwd_kv_kernel(const Bw
       __builtin_amdgcn_sched_barrier(0);
       const uint32_t rb = opaque(at.row + from32);
 #pragma unroll
-      for (int x = 0; x < KS; ++x) dp = E::mfma32(lds_read16<X8>(gt + Ti::step2(rb, x)), vf[x], dp);
+      for (int x = 0; x < kInRegs; ++x) dp = E::mfma32(lds_read16<X8>(gt + Ti::step2(rb, x)), vf[x], dp);
+      if constexpr (kKeep)
+        dp = E::mfma32(lds_read16<X8>(gt + Ti::step2(rb, KS - 1)),
+                       lds_read16<X8>(cur + 2 * kBuf + (wave * 64 + lane_again()) * 16), dp);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
@@ -707,7 +746,7 @@ __global__ void __launch_bounds__(kRowWaves * NQ * 64, 2) bwd_kv_kernel(const Bw
   }
   // Counted anew: they would take registers through the loop.
   const int le = lane_again() & 31, he = lane_again() >> 5;
-  if (a.causal && __any(le < keys && (not_finite<DP>(dk) || not_finite<DP>(dv)))) {
+  if (__builtin_expect(a.causal && __any(le < keys && (not_finite<DP>(dk) || not_finite<DP>(dv))), 0)) {
     // As in the forward: queries that do not see a key leave its products.  (The
     // rows again, for registers' sake.)
     X8 kr[KS], vr[KS];
@@ -723,11 +762,16 @@ __global__ void __launch_bounds__(kRowWaves * NQ * 64, 2) bwd_kv_kernel(const Bw
         const char* qp = a.q + (qs + i) * a.q_row + head * a.q_head;
         const char* gp = a.grad + (qs + i) * a.g_row + head * a.g_head;
         const int64_t at_i = int64_t{head} * a.Nq + qs + i;
-        const float s = dot_row<DP>(kr, qp, a.D, he), dp = dot_row<DP>(vr, gp, a.D, he);
+        const float s = dot_row<DP>(kr, qp, a.D, he);
+        __builtin_amdgcn_sched_barrier(0);
+        const float dp = dot_row<DP>(vr, gp, a.D, he);
+        __builtin_amdgcn_sched_barrier(0);
         if (key0 + le > i + shift) continue;
         const float p = exp2_hw(__builtin_fmaf(s, c2, -a.lse2[at_i]));
         add_row<T, DP>(dv, 1.0f, p, gp, a.D, he);
+        __builtin_amdgcn_sched_barrier(0);
         add_row<T, DP>(dk, 1.0f, p * (dp - a.delta[at_i]), qp, a.D, he);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
@@ -816,11 +860,13 @@ int check_operand(const char* name, const mx_attention_tensor* t, int32_t D, int
              "%s: rows and heads must start at multiples of 16 bytes", name);
   MX_REQUIRE(t->row_stride >= D || N <= 1, "%s: row stride %lld below D = %d", name,
              (long long)t->row_stride, D);
-  MX_REQUIRE(t->row_stride <= (1ll << 23), "%s: row stride %lld above 2^23 elements", name,
+  MX_REQUIRE(t->row_stride >= 0 && t->row_stride <= (1ll << 23), "%s: row stride %lld above 2^23 elements", name,
              (long long)t->row_stride);
   MX_REQUIRE(t->head_stride >= 0, "%s: negative head stride", name);
   return MX_OK;
 }
+
+uint32_t row_bytes(const mx_attention_tensor* t) { return static_cast<uint32_t>(t->row_stride * 2); }
 
 int check_problem(const mx_attention_problem* p) {
   MX_REQUIRE(p != nullptr, "problem is null");
@@ -867,9 +913,9 @@ extern "C" int mx_jagged_attention_forward(const mx_attention_problem* p, const 
   a.q = static_cast<const char*>(q->data);
   a.k = static_cast<const char*>(k->data);
   a.v = static_cast<const char*>(v->data);
-  a.q_row = q->row_stride * 2, a.q_head = q->head_stride * 2;
-  a.k_row = k->row_stride * 2, a.k_head = k->head_stride * 2;
-  a.v_row = v->row_stride * 2, a.v_head = v->head_stride * 2;
+  a.q_row = row_bytes(q), a.q_head = q->head_stride * 2;
+  a.k_row = row_bytes(k), a.k_head = k->head_stride * 2;
+  a.v_row = row_bytes(v), a.v_head = v->head_stride * 2;
   a.q_offsets = p->q_offsets, a.k_offsets = p->k_offsets;
   a.B = static_cast<int32_t>(p->B), a.Nq = static_cast<int32_t>(p->Nq), a.Nk = static_cast<int32_t>(p->Nk);
   a.H = p->H, a.G = p->H / p->Hkv, a.D = p->D;
@@ -912,11 +958,11 @@ extern "C" int mx_jagged_attention_backward(const mx_attention_problem* p, const
   a.v = static_cast<const char*>(v->data);
   a.out = static_cast<const char*>(out->data);
   a.grad = static_cast<const char*>(grad_out->data);
-  a.q_row = q->row_stride * 2, a.q_head = q->head_stride * 2;
-  a.k_row = k->row_stride * 2, a.k_head = k->head_stride * 2;
-  a.v_row = v->row_stride * 2, a.v_head = v->head_stride * 2;
-  a.o_row = out->row_stride * 2, a.o_head = out->head_stride * 2;
-  a.g_row = grad_out->row_stride * 2, a.g_head = grad_out->head_stride * 2;
+  a.q_row = row_bytes(q), a.q_head = q->head_stride * 2;
+  a.k_row = row_bytes(k), a.k_head = k->head_stride * 2;
+  a.v_row = row_bytes(v), a.v_head = v->head_stride * 2;
+  a.o_row = row_bytes(out), a.o_head = out->head_stride * 2;
+  a.g_row = row_bytes(grad_out), a.g_head = grad_out->head_stride * 2;
   a.q_offsets = p->q_offsets, a.k_offsets = p->k_offsets;
   a.B = static_cast<int32_t>(p->B), a.Nq = static_cast<int32_t>(p->Nq), a.Nk = static_cast<int32_t>(p->Nk);
   a.H = p->H, a.Hkv = p->Hkv, a.G = p->H / p->Hkv, a.D = p->D;
