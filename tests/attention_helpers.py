@@ -124,7 +124,8 @@ def check(got, want, tol, what):
     got = np.asarray(got, np.float64)
     assert got.shape == want.shape, (what, got.shape, want.shape)
     assert np.isfinite(got).all() or not np.isfinite(want).all(), f"{what}: not finite"
-    bad = ~(np.abs(got - want) <= tol)
+    with np.errstate(invalid="ignore"):  # infinities on both sides: equal below
+        bad = ~(np.abs(got - want) <= tol)
     bad &= ~((got == want) | (np.isnan(got) & np.isnan(want)))
     if bad.any():
         i = np.unravel_index(np.argmax(np.where(bad, np.abs(got - want) - tol, -np.inf)), got.shape)

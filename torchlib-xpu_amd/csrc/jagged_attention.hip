@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(kRowWaves * NS * 64, 2) fwd_kernel(const FwdAr
   }
   const Span sq = f.own, sk = f.other;
   const int tile = f.tile;
-  if (tile * BM >= sq.len) return;
+  if (tile < 0 || tile * BM >= sq.len) return;  // (below 0: offsets that decrease)
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(kRowWaves * NS * 64, DP <= 64 ? 4 : NS == 1 &&
   }
   const Span sq = f.own, sk = f.other;
   const int tile = f.tile;
-  if (tile * BM >= sq.len) return;
+  if (tile < 0 || tile * BM >= sq.len) return;  // (below 0: offsets that decrease)
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -589,7 +589,7 @@ __global__ void __launch_bounds__(kRowWaves * NQ * 64, 2) bwd_kv_kernel(const Bw
   }
   const Span sk = f.own, sq = f.other;
   const int tile = f.tile;
-  if (tile * BM >= sk.len) return;
+  if (tile < 0 || tile * BM >= sk.len) return;
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -801,7 +801,7 @@ bool split_queries(int64_t Nq, int64_t Nk, int64_t B, int64_t Hkv, int64_t G) {
 
 int blocks_of(int64_t rows, int64_t B, int64_t heads, unsigned* blocks) {
   const int64_t n = tile_turns(rows, B, 128) * heads;
-  MX_REQUIRE(n < (1ll << 31), "too many tiles: %lld", (long long)n);
+  MX_REQUIRE(n < (1ll << 23), "too many tiles: %lld", (long long)n);  // of 512 threads in 32 bits
   *blocks = static_cast<unsigned>(n);
   return MX_OK;
 }
@@ -878,6 +878,7 @@ int check_problem(const mx_attention_problem* p) {
              "more than %d rows or lists", MX_ATTENTION_MAX_ROWS);
   MX_REQUIRE(p->H > 0 && p->Hkv > 0 && p->H % p->Hkv == 0,
              "%d query heads are no multiple of %d key-value heads", p->H, p->Hkv);
+  MX_REQUIRE(static_cast<int64_t>(p->H) * p->D <= (1ll << 23), "rows of %d heads of %d are too wide", p->H, p->D);
   MX_REQUIRE(p->D > 0 && p->D <= MX_ATTENTION_MAX_D && p->D % 8 == 0,
              "head width %d is no multiple of 8 up to %d", p->D, MX_ATTENTION_MAX_D);
   MX_REQUIRE(std::isfinite(p->scale) && p->scale > 0.0f, "scale must be positive and finite");

@@ -250,9 +250,11 @@ __global__ void __launch_bounds__(kStepWaves * 64, 2) step_kernel(const StepArgs
     // the next tile are asked for before this one's keys.
     const int32_t* row = a.c.table + b * a.c.table_row;
     auto entry = [&](int32_t k0, int* slot) {
-      const int32_t key = k0 + (lane & 31);
-      *slot = 0;
-      return key < end ? row[page_of(a.c, key, slot)] : -1;
+      const uint32_t key = k0 + (lane & 31);
+      const uint32_t size = a.c.page_size;
+      const uint32_t e = a.c.page_shift >= 0 ? key >> a.c.page_shift : key / size;
+      *slot = static_cast<int>(key - e * size);
+      return key < static_cast<uint32_t>(end) ? row[e] : -1;
     };
     const int32_t first = t0 * kTileKeys + wave * kStepKeys;
     int slot_next = 0;
@@ -519,7 +521,7 @@ template <typename T, int DP>
 int launch_step(const StepArgs& a, hipStream_t s) {
   const int64_t blocks = static_cast<int64_t>(a.workers > 0 ? a.workers : a.B) * a.Hkv * a.head_blocks;
   const int64_t joins = static_cast<int64_t>(a.B) * a.H;
-  MX_REQUIRE(blocks < (1ll << 31) && joins < (1ll << 31), "too many sequences: %d", a.B);
+  MX_REQUIRE(blocks < (1ll << 22) && joins < (1ll << 22), "too many sequences: %d", a.B);  // threads in 32 bits
   step_kernel<T, DP><<<dim3(static_cast<unsigned>(blocks)), kStepWaves * 64, 0, s>>>(a);
   if (a.workers > 0) {
     const int waves = a.workers / a.B < 8 ? 1 : a.workers / a.B < 32 ? 4 : kJoinMost;
@@ -570,7 +572,7 @@ extern "C" int mx_paged_cache_append(const mx_paged_cache* cache, int32_t dtype,
   a.B = B, a.N = N;
   a.Hkv = Hkv, a.chunks = D / 8;
   const int64_t blocks = mx::ceil_div(N, kAppendWaves);
-  MX_REQUIRE(blocks < (1ll << 31), "too many rows: %lld", (long long)N);
+  MX_REQUIRE(blocks < (1ll << 24), "too many rows: %lld", (long long)N);  // threads in 32 bits
   append_kernel<<<dim3(static_cast<unsigned>(blocks)), kAppendWaves * 64, 0, mx::as_stream(stream)>>>(a);
   MX_LAUNCH_CHECK();
   return MX_OK;
@@ -593,7 +595,7 @@ extern "C" int mx_paged_cache_attention(const mx_paged_cache* cache, int32_t dty
   mx::clear_error();
   if (int rc = check_cache(cache, dtype, Hkv, D)) return rc;
   MX_REQUIRE(B >= 0 && B < (1ll << 31), "%lld sequences", (long long)B);
-  MX_REQUIRE(cache->table_width * cache->page_size < (1ll << 31), "more than 2^31 tokens in a row of the table");
+  MX_REQUIRE(cache->table_width <= (1ll << 30) / cache->page_size, "more than 2^30 tokens in a row of the table");
   MX_REQUIRE(H > 0 && H % Hkv == 0, "%d query heads are no multiple of %d key-value heads", H, Hkv);
   MX_REQUIRE(std::isfinite(scale) && scale > 0.0f, "scale must be positive and finite");
   MX_REQUIRE(lengths_bytes == 4 || lengths_bytes == 8, "lengths_bytes %d", lengths_bytes);
