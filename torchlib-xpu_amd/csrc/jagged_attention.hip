@@ -237,19 +237,17 @@ __global__ void __launch_bounds__(kRowWaves * NS * 64, 2) fwd_kernel(const FwdAr
     if (k0 >= wave_end) return;
     const uint32_t ra = opaque(at.row + buf);
 
-    f32x16 s[kBN / 32];
+    f32x16 s[2]{};
 #pragma unroll
-    for (int b = 0; b < kBN / 32; ++b) {
-      s[b] = f32x16{};
+    for (int x = 0; x < KS; ++x)
 #pragma unroll
-      for (int x = 0; x < KS; ++x)
+      for (int b = 0; b < 2; ++b)  // two chains of products, each the other's wait
         s[b] = E::mfma32(lds_read16<X8>(cur + 32 * b * Ti::kRow + Ti::step2(ra, x)), qf[x], s[b]);
-    }
 
     if (k0 + kBN > all_end) {  // the tile reaches past a query's last key
       const int last = mine - k0 - 4 * h;
 #pragma unroll
-      for (int b = 0; b < kBN / 32; ++b)
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (32 * b + 8 * (i / 4) + i % 4 >= last) s[b][i] = -INFINITY;
@@ -257,7 +255,7 @@ __global__ void __launch_bounds__(kRowWaves * NS * 64, 2) fwd_kernel(const FwdAr
 
     float top = s[0][0];
 #pragma unroll
-    for (int b = 0; b < kBN / 32; ++b)
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
     top = fmaxf(top, other_half(top));
@@ -271,9 +269,9 @@ __global__ void __launch_bounds__(kRowWaves * NS * 64, 2) fwd_kernel(const FwdAr
     }
     const float mc = m == -INFINITY ? 0.0f : m * c2;
 
-    X8 p[kBN / 16];
+    X8 p[4];
 #pragma unroll
-    for (int b = 0; b < kBN / 32; ++b)
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float e = exp2_hw(__builtin_fmaf(s[b][i], c2, -mc));
@@ -283,7 +281,7 @@ __global__ void __launch_bounds__(kRowWaves * NS * 64, 2) fwd_kernel(const FwdAr
 
     const uint32_t t0 = opaque(at.tr + buf), t1 = Ti::next8(t0);
 #pragma unroll
-    for (int x = 0; x < kBN / 16; ++x)
+    for (int x = 0; x < 4; ++x)
 #pragma unroll
       for (int d = 0; d < DB; ++d) {
         const char* f = cur + kTileBytes + 16 * x * Ti::kRow;
@@ -475,7 +473,7 @@ __global__ void __launch_bounds__(kRowWaves * NS * 64, DP <= 64 ? 4 : NS == 1 &&
       if (h == 0 && l < rows) a.delta[int64_t{head} * a.Nq + q_base + l] = delta;
     }
 #pragma unroll
-    for (int b = 0; b < kBN / 32; ++b) {
+    for (int b = 0; b < 2; ++b) {
       const int k0 = j * kBN + 32 * b;
       if (k0 >= wave_end) return;
       const uint32_t ra = opaque(at.row + buf), t0 = opaque(at.tr + buf), t1 = Ti::next8(t0);
