@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(kRowWaves * NS * 64, DP <= 64 ? 4 : NS == 1 &&
   load_rows<X8, KS>(qf, a.q + q_base * a.q_row + head * a.q_head, rows, a.q_row, a.D, l, h);
   load_rows<X8, KS>(gf, a.grad + q_base * a.g_row + head * a.g_head, rows, a.g_row, a.D, l, h);
   float delta = 0.0f, lse2 = 0.0f;
-  {
+  if (wave_end > kBN) {  // else delta comes from the first tile
     X8 of[KS];
     load_rows<X8, KS>(of, a.out + q_base * a.o_row + head * a.o_head, rows, a.o_row, a.D, l, h);
 #pragma unroll
@@ -413,13 +413,13 @@ __global__ void __launch_bounds__(kRowWaves * NS * 64, DP <= 64 ? 4 : NS == 1 &&
       for (int e = 0; e < 8; ++e)
         delta = __builtin_fmaf(static_cast<float>(of[s][e]), static_cast<float>(gf[s][e]), delta);
     delta += other_half(delta);
-    if (l < rows) {
-      const int64_t at = int64_t{head} * a.Nq + q_base + l;
-      lse2 = a.lse[at] * kLog2e;
-      if (h == 0 && group == 0) {
-        a.lse2[at] = lse2;
-        a.delta[at] = delta;
-      }
+  }
+  if (l < rows) {
+    const int64_t at = int64_t{head} * a.Nq + q_base + l;
+    lse2 = a.lse[at] * kLog2e;
+    if (h == 0 && group == 0) {
+      a.lse2[at] = lse2;
+      a.delta[at] = delta;
     }
   }
 
