@@ -77,6 +77,31 @@ def test_long_and_ragged(dev, B):
     run(dev, lengths, 16, 2, 1, 64, "bfloat16")
 
 
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("D", [8, 32, 40, 64, 72, 96, 104, 128])
+def test_widths_in_shares(dev, dtype, D):
+    """More tokens than two wide blocks' tiles: sequences cut anywhere and joined."""
+    run(dev, [1, 0, 31, 1300, 33, 129], 16, 4, 2, D, dtype)
+
+
+@pytest.mark.parametrize("fill", [0.0, float("nan"), float("inf"), -float("inf")])
+def test_what_slots_in_shares_hold(dev, fill):
+    run(dev, [5, 1490, 0, 17], 100, 4, 2, 64, "bfloat16", fill=fill)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("room", [128, 144, 512, 528, 1024, 1040, 4096])
+def test_room_in_the_table(dev, D, room):
+    """The table's width decides how sequences are cut, not what comes out."""
+    kc, vc, table, ks, vs = make_cache([room - 1, 100, room // 2], 16, 2, D, "bfloat16")
+    q = make((3, 6, D), "bfloat16", 9)
+    out = OPS.paged_cache_attention(q.to(dev), kc.to(dev), vc.to(dev), table.to(dev),
+                                    torch.tensor([room - 1, 100, room // 2], device=dev))
+    want, tol = paged_attention(q.double().numpy(), [k.double().numpy() for k in ks],
+                                [v.double().numpy() for v in vs], D ** -0.5, "bfloat16")
+    check(out.double().cpu().numpy(), want, tol, "out")
+
+
 @pytest.mark.parametrize("fill", [0.0, float("nan"), float("inf"), -float("inf")])
 def test_what_slots_without_tokens_hold(dev, fill):
     run(dev, [5, 50, 17], 16, 4, 2, 128, "bfloat16", fill=fill)

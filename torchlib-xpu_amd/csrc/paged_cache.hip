@@ -106,12 +106,14 @@ struct StepArgs {
   int32_t B, H, Hkv, G, D;
   int32_t head_blocks;     // of 16 query heads of a key-value head
   int32_t workers;         // per head block: they share all tiles; 0: a block per sequence
+  int32_t wide;            // a block of 8 or 16 waves per sequence
   float scale;
   void* out;               // [B, H, D]
   float* part;             // [workers, 2, H, D + 2]: sums, then maximum and sum of weights
 };
 
 constexpr int kStepWaves = 4;
+constexpr int wide_waves(int D) { return D <= 64 ? 16 : 8; }  // by the registers
 constexpr int kStepKeys = 32;  // keys of a wave's tile
 
 // N values of 16 bits from global memory.
@@ -130,14 +132,17 @@ __device__ __forceinline__ int64_t shfl64(int64_t v, int lane) {
   return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
 }
 
-// Tokens of sequence b that there are, and its tiles of 128 keys.
+// Tokens of sequence b that there are, and its tiles of 32 keys per wave of a block.
 constexpr int kTileKeys = kStepWaves * kStepKeys;
 
 __device__ __forceinline__ int32_t tokens_of(const StepArgs& a, int32_t b) {
   const int64_t n = ld_index(a.lengths, a.lengths_bytes, b), most = a.c.width * a.c.page_size;
   return static_cast<int32_t>(n < 0 ? 0 : (n < most ? n : most));
 }
-__device__ __forceinline__ int32_t tiles_of(int32_t tokens) { return (tokens + kTileKeys - 1) / kTileKeys; }
+template <int WAVES = kStepWaves>
+__device__ __forceinline__ int32_t tiles_of(int32_t tokens) {
+  return (tokens + WAVES * kStepKeys - 1) / (WAVES * kStepKeys);
+}
 
 // The sequences' tiles end to end are cut into equal shares, one for a worker
 // (and no more than tiles): share w begins at tile w total / shares.  A sequence's tiles may be cut anywhere;
@@ -165,21 +170,22 @@ __device__ __forceinline__ int64_t count_tiles(const StepArgs& a, int32_t b, int
 }
 
 // One block: up to 16 query heads of one key-value head, and a share of its
-// tiles (or one sequence); its waves take 32 of a tile's 128 keys each.  Every
+// tiles (or one sequence); its waves take 32 of a tile's keys each.  Every
 // key and value is read once, straight into registers in the matrix operands'
 // layouts (r = lane % 16, g = lane / 16): 16 keys x 32 columns of K per 16x16x32
 // product, a head per result column; 8 keys and DP / 16 columns of V per lane,
 // transposed in registers.  Probabilities are rounded to the cache's type for
 // the second product; scores, sums and the running maximum are fp32.
-template <typename T, int DP>
-__global__ void __launch_bounds__(kStepWaves * 64, 2) step_kernel(const StepArgs a) {
+template <typename T, int DP, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? 2 : WAVES / 4) step_kernel(const StepArgs a) {
   using E = Elem<T>;
   using X8 = typename E::x8;
+  constexpr int kTile = WAVES * kStepKeys;
   constexpr int KS = DP / 32;  // products along D of a score
   constexpr int EV = DP / 16;  // columns of V per lane
   using VP = typename Piece<EV>::type;
-  __shared__ float sh_o[kStepWaves][16][DP + 1];
-  __shared__ float sh_m[kStepWaves][16], sh_l[kStepWaves][16];
+  __shared__ float sh_o[WAVES][16][DP + 1];
+  __shared__ float sh_m[WAVES][16], sh_l[WAVES][16];
 
   const int heads_all = a.Hkv * a.head_blocks;
   const int hh = blockIdx.x % heads_all, worker = blockIdx.x / heads_all;
@@ -196,9 +202,9 @@ __global__ void __launch_bounds__(kStepWaves * 64, 2) step_kernel(const StepArgs
   // The share: tiles [at, stop) counted from sequence b's first one.
   int32_t b = worker, len;
   int64_t at = 0, stop = 0;
-  if (a.workers == 0) {
+  if (WAVES != kStepWaves || a.workers == 0) {
     len = __builtin_amdgcn_readfirstlane(tokens_of(a, b));
-    stop = len > 0 ? tiles_of(len) : 1;  // an empty sequence is written too
+    stop = len > 0 ? tiles_of<WAVES>(len) : 1;  // an empty sequence is written too
   } else {
     int64_t prior;
     const int64_t total = count_tiles(a, 0, &prior);
@@ -210,7 +216,7 @@ __global__ void __launch_bounds__(kStepWaves * 64, 2) step_kernel(const StepArgs
     for (int32_t i0 = 0; i0 < a.B; i0 += 64) {
       const int32_t i = i0 + lane_id();
       const int32_t tokens = i < a.B ? tokens_of(a, i) : 0;
-      const int32_t upto = wave_prefix(tiles_of(tokens));
+      const int32_t upto = wave_prefix(tiles_of<WAVES>(tokens));
       const int32_t here = readlane_i32(upto, 63);
       if (at >= here) {
         at -= here;
@@ -220,7 +226,7 @@ __global__ void __launch_bounds__(kStepWaves * 64, 2) step_kernel(const StepArgs
       const int l = __builtin_ctzll(__ballot(at < upto));
       b = i0 + l;
       len = readlane_i32(tokens, l);
-      const int32_t skip = readlane_i32(upto, l) - tiles_of(len);
+      const int32_t skip = readlane_i32(upto, l) - tiles_of<WAVES>(len);
       at -= skip;
       stop -= skip;
       break;
@@ -228,9 +234,9 @@ __global__ void __launch_bounds__(kStepWaves * 64, 2) step_kernel(const StepArgs
   }
 
   while (true) {
-    const int32_t n = tiles_of(len);
+    const int32_t n = tiles_of<WAVES>(len);
     const int32_t t0 = static_cast<int32_t>(at), t1 = static_cast<int32_t>(stop < n ? stop : n);
-    const int32_t end = t1 * kTileKeys < len ? t1 * kTileKeys : len;
+    const int32_t end = t1 * kTile < len ? t1 * kTile : len;
 
     X8 qf[KS];
 #pragma unroll
@@ -256,13 +262,13 @@ __global__ void __launch_bounds__(kStepWaves * 64, 2) step_kernel(const StepArgs
       *slot = static_cast<int>(key - e * size);
       return key < static_cast<uint32_t>(end) ? row[e] : -1;
     };
-    const int32_t first = t0 * kTileKeys + wave * kStepKeys;
+    const int32_t first = t0 * kTile + wave * kStepKeys;
     int slot_next = 0;
     int32_t page_next = entry(first, &slot_next);
-    for (int32_t k0 = first; k0 < end; k0 += kTileKeys) {
+    for (int32_t k0 = first; k0 < end; k0 += kTile) {
       const int64_t page = page_next;
       const int slot = slot_next;
-      page_next = entry(k0 + kTileKeys, &slot_next);
+      page_next = entry(k0 + kTile, &slot_next);
       const bool there = page >= 0 && page < a.c.pages;
       const uint32_t seen = static_cast<uint32_t>(__ballot(there));
       const int64_t koff = there ? page * a.c.k_page + slot * a.c.k_slot : 0;
@@ -345,14 +351,14 @@ __global__ void __launch_bounds__(kStepWaves * 64, 2) step_kernel(const StepArgs
       for (int i = 0; i < 4; ++i) sh_o[wave][r][EV * (4 * g + i) + t] = o[t][i];
     __syncthreads();
     const bool whole = t0 == 0 && t1 == n;
-    for (int u = tid; u < heads * a.D; u += kStepWaves * 64) {
+    for (int u = tid; u < heads * a.D; u += WAVES * 64) {
       const int nh = u / a.D, d = u - nh * a.D;
       float mm = sh_m[0][nh];
 #pragma unroll
-      for (int w = 1; w < kStepWaves; ++w) mm = fmaxf(mm, sh_m[w][nh]);
+      for (int w = 1; w < WAVES; ++w) mm = fmaxf(mm, sh_m[w][nh]);
       float acc = 0.0f, l = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kStepWaves; ++w) {
+      for (int w = 0; w < WAVES; ++w) {
         const float f = mm == -INFINITY ? 0.0f : exp2_hw((sh_m[w][nh] - mm) * c2);
         acc += f * sh_o[w][nh][d];
         l += f * sh_l[w][nh];
@@ -471,17 +477,32 @@ __global__ void __launch_bounds__(kJoinMost * 64) join_kernel(const StepArgs a) 
   }
 }
 
-// Workers of a call: two blocks for every CU (64 ragged sequences of up to 4096
-// tokens, 8 x 128: a block per sequence in halves 147 us, shares with one, two
-// and three blocks a CU 119, 106 and 122), or 0, a block per sequence and head,
-// where these are enough to even out by themselves (1024 of up to 200 tokens, 8
-// x 64: 71 us, in shares 108; 256 of up to 2000, 8 x 128: 219, in shares 205)
-// or no sequence has two tiles.
-int32_t plan_workers(int64_t B, int32_t heads, int64_t most) {
-  const int64_t tiles = ceil_div(most, kTileKeys);
-  if (tiles <= 1 || B * heads >= 8 * static_cast<int64_t>(num_cus())) return 0;
-  const int64_t w = ceil_div(static_cast<int64_t>(num_cus()) * 2, heads);
-  return static_cast<int32_t>(w < B * tiles ? w : B * tiles);
+// How a call's sequences are cut.  Times in us, of back-to-back calls with an
+// event on both sides (about 5 of them the launch).
+// - Workers that share all tiles, two blocks for every CU (64 ragged sequences of
+//   up to 4096 tokens, 8 x 128: a block per sequence in halves 147, shares with
+//   one, two and three blocks a CU 119, 106 and 122).  What they leave is joined
+//   by a second launch, which waits for the first.
+// - Where no sequence can have more than two tiles of a wide block (8 or 16
+//   waves), and blocks are few enough to start nearly at once, such a block per
+//   sequence and head instead of the second launch (8 heads of 64: one sequence
+//   of 777 15.2 -> 11.1, of 2048 15.5 -> 17.8; 64 of up to 1024 31.1 -> 27.4; 200
+//   of up to 1024 70.3 -> 70.9; 8 heads of 128: 64 of up to 512 29.6 -> 25.4, 200
+//   57.7 -> 63.4).
+// - A block of four waves per sequence and head where these are enough to even
+//   out by themselves (1024 of up to 200 tokens, 8 x 64: 71, in shares 108; 256 of
+//   up to 2000, 8 x 128: 219, in shares 205) or no sequence has two tiles.
+struct Plan {
+  int32_t workers;  // 0: a block per sequence and head
+  bool wide;
+};
+
+Plan plan_step(int64_t B, int32_t heads, int32_t D, int64_t most) {
+  const int64_t tiles = ceil_div(most, kTileKeys), blocks = B * heads, cus = num_cus();
+  if (tiles <= 1 || blocks >= 8 * cus) return {0, false};
+  if (most <= 2 * wide_waves(D) * kStepKeys && blocks <= 4 * cus) return {0, true};
+  const int64_t w = ceil_div(cus * 2, heads);
+  return {static_cast<int32_t>(w < B * tiles ? w : B * tiles), false};
 }
 
 int32_t head_blocks_of(int32_t H, int32_t Hkv) { return static_cast<int32_t>(ceil_div(H / Hkv, 16)); }
@@ -522,7 +543,10 @@ int launch_step(const StepArgs& a, hipStream_t s) {
   const int64_t blocks = static_cast<int64_t>(a.workers > 0 ? a.workers : a.B) * a.Hkv * a.head_blocks;
   const int64_t joins = static_cast<int64_t>(a.B) * a.H;
   MX_REQUIRE(blocks < (1ll << 22) && joins < (1ll << 22), "too many sequences: %d", a.B);  // threads in 32 bits
-  step_kernel<T, DP><<<dim3(static_cast<unsigned>(blocks)), kStepWaves * 64, 0, s>>>(a);
+  if (a.wide)
+    step_kernel<T, DP, wide_waves(DP)><<<dim3(static_cast<unsigned>(blocks)), wide_waves(DP) * 64, 0, s>>>(a);
+  else
+    step_kernel<T, DP, kStepWaves><<<dim3(static_cast<unsigned>(blocks)), kStepWaves * 64, 0, s>>>(a);
   if (a.workers > 0) {
     const int waves = a.workers / a.B < 8 ? 1 : a.workers / a.B < 32 ? 4 : kJoinMost;
     join_kernel<T><<<dim3(static_cast<unsigned>(joins)), waves * 64, 0, s>>>(a);
@@ -582,8 +606,8 @@ extern "C" size_t mx_paged_cache_attention_workspace_bytes(const mx_paged_cache*
                                                            int32_t H, int32_t Hkv, int32_t D) {
   using namespace mx::attn;
   if (cache == nullptr || B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || D <= 0) return 0;
-  const int64_t workers = plan_workers(B, Hkv * head_blocks_of(H, Hkv), cache->table_width * cache->page_size);
-  return static_cast<size_t>(workers) * 2 * H * (D + 2) * sizeof(float);
+  const Plan plan = plan_step(B, Hkv * head_blocks_of(H, Hkv), D, cache->table_width * cache->page_size);
+  return static_cast<size_t>(plan.workers) * 2 * H * (D + 2) * sizeof(float);
 }
 
 extern "C" int mx_paged_cache_attention(const mx_paged_cache* cache, int32_t dtype,
@@ -615,7 +639,8 @@ extern "C" int mx_paged_cache_attention(const mx_paged_cache* cache, int32_t dty
   a.head_blocks = head_blocks_of(H, Hkv);
   a.scale = scale;
   a.out = out;
-  a.workers = plan_workers(B, Hkv * a.head_blocks, cache->table_width * cache->page_size);
+  const Plan plan = plan_step(B, Hkv * a.head_blocks, D, cache->table_width * cache->page_size);
+  a.workers = plan.workers, a.wide = plan.wide;
   const size_t need = mx_paged_cache_attention_workspace_bytes(cache, B, H, Hkv, D);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return mx::set_error(MX_EWORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
