@@ -632,15 +632,19 @@ typedef struct mx_attention_problem {
 } mx_attention_problem;
 
 /* out: contiguous [Nq, H, D] of the inputs' type; lse (natural logarithm of
- * each query's sum, may be NULL): [H, Nq] fp32. */
+ * each query's sum, may be NULL): [H, Nq] fp32.  The workspaces (device memory
+ * from a multiple of 32 bytes, contents need not be kept between calls) may be
+ * NULL where their size is 0. */
+size_t mx_jagged_attention_forward_workspace_bytes(const mx_attention_problem* p);
 int mx_jagged_attention_forward(const mx_attention_problem* p, const mx_attention_tensor* q,
                                 const mx_attention_tensor* k, const mx_attention_tensor* v,
-                                void* out, float* lse, void* stream);
+                                void* out, float* lse, void* workspace, size_t workspace_bytes,
+                                void* stream);
 
 /* Gradients of the above from its out and lse: contiguous [Nq, H, D] and twice
  * [Nk, Hkv, D], the same bits for the same inputs.  Without dk and dv (both
  * NULL) dq alone. */
-size_t mx_jagged_attention_backward_workspace_bytes(int64_t Nq, int32_t H);
+size_t mx_jagged_attention_backward_workspace_bytes(const mx_attention_problem* p);
 int mx_jagged_attention_backward(const mx_attention_problem* p, const mx_attention_tensor* q,
                                  const mx_attention_tensor* k, const mx_attention_tensor* v,
                                  const mx_attention_tensor* out,

@@ -96,6 +96,22 @@ def test_many_lists(dev, lists, length):
     run(dev, q, k, v, o, o, True, None, "bfloat16", g)
 
 
+@pytest.mark.parametrize("lists,most", [(20, 1000), (70, 260), (1100, 20)])
+@pytest.mark.parametrize("index", [torch.int32, torch.int64])
+@pytest.mark.parametrize("causal", [True, False])
+def test_many_tiles(dev, lists, most, index, causal):
+    """Enough tiles for an order of their own: lists of unlike lengths, rows of no
+    list at both ends, and other lengths for the keys."""
+    rng = np.random.default_rng(lists)
+    nq, nk = rng.integers(0, most + 1, lists), rng.integers(0, most + 1, lists)
+    nq[lists // 2], nk[lists // 3] = 700, 0
+    qo, ko = offsets_of(nq) + 5, offsets_of(nk) + 300
+    Nq, Nk = int(qo[-1]) + 600, int(ko[-1]) + 1
+    q, g = make(Nq, 64, 8, "bfloat16", 1), make(Nq, 64, 8, "bfloat16", 2)
+    k, v = make(Nk, 4, 8, "bfloat16", 3), make(Nk, 4, 8, "bfloat16", 4)
+    run(dev, q, k, v, qo, ko, causal, None, "bfloat16", g, index)
+
+
 @pytest.mark.parametrize("dtype,D", [("float16", 128), ("bfloat16", 128), ("bfloat16", 64)])
 def test_long_lists(dev, dtype, D):
     o = offsets_of([1500, 777])

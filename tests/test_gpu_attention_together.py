@@ -135,7 +135,8 @@ def test_forward_through_ctypes(dev):
     lib.mx_last_error.restype = ctypes.c_char_p
     P = ctypes.c_void_p
     T3 = ctypes.POINTER(Tensor3)
-    lib.mx_jagged_attention_forward.argtypes = [ctypes.POINTER(Problem), T3, T3, T3, P, P, P]
+    lib.mx_jagged_attention_forward.argtypes = [ctypes.POINTER(Problem), T3, T3, T3, P, P, P,
+                                                ctypes.c_size_t, P]
     n, H, Hkv, D = 50, 4, 2, 32
     q, k, v = make((n, H, D), 1), make((n, Hkv, D), 2), make((n, Hkv, D), 3)
     o = np.array([0, 20, 50])
@@ -144,7 +145,7 @@ def test_forward_through_ctypes(dev):
     p = Problem(2, 8, od.data_ptr(), od.data_ptr(), 2, n, n, H, Hkv, D, 1, 0.25)
     args = [Tensor3(x.data_ptr(), x.stride(0), x.stride(1)) for x in (qd, kd, vd)]
     stream = torch.cuda.current_stream().cuda_stream
-    assert lib.mx_jagged_attention_forward(p, *args, out.data_ptr(), lse.data_ptr(), stream) == 0
+    assert lib.mx_jagged_attention_forward(p, *args, out.data_ptr(), lse.data_ptr(), None, 0, stream) == 0
     r = attention(*(x.double().numpy() for x in (q, k, v)), o, o, True, 0.25, "bfloat16")
     check(out.double().cpu().numpy(), r.out, r.out_tol, "out")
     check(lse.double().cpu().numpy(), r.lse, r.lse_tol, "lse")
@@ -153,15 +154,15 @@ def test_forward_through_ctypes(dev):
                        ("B", -1), ("Nq", 2 ** 31)):
         keep = getattr(p, field)
         setattr(p, field, bad)
-        assert lib.mx_jagged_attention_forward(p, *args, out.data_ptr(), lse.data_ptr(), stream) == -1
+        assert lib.mx_jagged_attention_forward(p, *args, out.data_ptr(), lse.data_ptr(), None, 0, stream) == -1
         assert lib.mx_last_error()
         setattr(p, field, keep)
     for bad in (Tensor3(qd.data_ptr() + 2, H * D, D), Tensor3(qd.data_ptr(), D - 8, D),
                 Tensor3(qd.data_ptr(), H * D + 4, D), Tensor3(qd.data_ptr(), 2 ** 24, D), Tensor3(0, H * D, D)):
-        assert lib.mx_jagged_attention_forward(p, bad, args[1], args[2], out.data_ptr(), None, stream) == -1
+        assert lib.mx_jagged_attention_forward(p, bad, args[1], args[2], out.data_ptr(), None, None, 0, stream) == -1
     lib.mx_jagged_attention_backward_workspace_bytes.restype = ctypes.c_size_t
-    lib.mx_jagged_attention_backward_workspace_bytes.argtypes = [ctypes.c_int64, ctypes.c_int32]
-    assert lib.mx_jagged_attention_backward_workspace_bytes(n, H) == n * H * 8
+    lib.mx_jagged_attention_backward_workspace_bytes.argtypes = [ctypes.POINTER(Problem)]
+    assert lib.mx_jagged_attention_backward_workspace_bytes(p) == n * H * 8
     lib.mx_jagged_attention_backward.argtypes = [ctypes.POINTER(Problem), T3, T3, T3, T3, T3, P, P, P, P, P,
                                                  ctypes.c_size_t, P]
     o3 = Tensor3(out.data_ptr(), H * D, D)

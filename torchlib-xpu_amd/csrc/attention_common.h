@@ -380,6 +380,23 @@ __device__ __forceinline__ bool find_ranked(const I* own, const I* other, int32_
   return true;
 }
 
+// A turn worked out beforehand (plan_kernel): tile < 0 is a turn without work.
+struct alignas(32) Turn {
+  Span own, other;
+  int32_t tile;
+  int32_t pad[3];
+};
+
+__device__ __forceinline__ bool find_planned(const Turn* turns, int32_t n, int32_t turn, Found* f) {
+  const Turn* t = turns + rotated(turn, n);
+  const i32x4 s = *reinterpret_cast<const i32x4*>(t);
+  const int32_t tile = __builtin_amdgcn_readfirstlane(t->tile);
+  f->own = {__builtin_amdgcn_readfirstlane(s[0]), __builtin_amdgcn_readfirstlane(s[1])};
+  f->other = {__builtin_amdgcn_readfirstlane(s[2]), __builtin_amdgcn_readfirstlane(s[3])};
+  f->tile = tile;
+  return tile >= 0;
+}
+
 inline int64_t tile_turns(int64_t N, int64_t B, int bm) { return N / bm + B + 2; }
 
 }  // namespace attn

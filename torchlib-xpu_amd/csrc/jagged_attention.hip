@@ -12,6 +12,87 @@ namespace mx {
 namespace attn {
 namespace {
 
+constexpr int kBN = 64;        // keys per tile
+constexpr int kRowWaves = 4;   // waves of 32 queries: tiles of 128
+constexpr int kRowShift = 7;
+
+struct PlanArgs {
+  const void *q_offsets, *k_offsets;
+  int32_t B, Nq, Nk, causal;
+  Turn* turns[2];                  // of the queries' tiles and the keys' tiles
+  int32_t n[2];
+};
+
+// The order of a launch's tiles where lists are many and long: list by list, those
+// with the most partners first (a block's time is its tile's length: the longest
+// must not start last), a list's tiles one after another, as they read the same
+// keys.  Block 0 orders the queries' tiles, block 1 the keys'.  The lists are
+// counted into bins by the leading bits of their partners' number (exponent and 5
+// more: 3%), whose sums are the bins' first turns; order within a bin is as it
+// comes, which decides when a tile is worked on, never what comes out.
+constexpr int kPlanThreads = 1024;  // and as many bins
+
+template <typename I>
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
+  __shared__ int32_t bins[kPlanThreads], sums[kPlanThreads / 64];
+  const bool keys = blockIdx.x == 1;
+  const I* own = static_cast<const I*>(keys ? a.k_offsets : a.q_offsets);
+  const I* other = static_cast<const I*>(keys ? a.q_offsets : a.k_offsets);
+  const int32_t N = keys ? a.Nk : a.Nq, Nother = keys ? a.Nq : a.Nk;
+  Turn* turns = a.turns[blockIdx.x];
+  const int32_t most = a.n[blockIdx.x];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+
+  struct List { Span own, other; int32_t tiles, bin; };
+  auto list = [&](int32_t i) {
+    List x{};
+    if (i > a.B + 1) return x;
+    const int32_t s = list_start(own, a.B, N, i), e = list_start(own, a.B, N, i + 1);
+    const int32_t os = list_start(other, a.B, Nother, i), oe = list_start(other, a.B, Nother, i + 1);
+    x.own = {s, e > s ? e - s : 0};
+    x.other = {os, i > 0 && i <= a.B && oe > os ? oe - os : 0};
+    x.tiles = (x.own.len + 127) >> kRowShift;
+    // 2^0 .. 2^22 partners: bins 736 .. 1 from the end.
+    const int32_t bits = static_cast<int32_t>(__float_as_uint(static_cast<float>(x.other.len)) >> 18) - (127 << 5) + 1;
+    x.bin = kPlanThreads - 1 - (bits > 0 ? bits : 0);
+    return x;
+  };
+
+  bins[tid] = 0;
+  const List first = list(tid);
+  __syncthreads();
+  for (int32_t i = tid; i <= a.B + 1; i += kPlanThreads) {
+    const List x = i == tid ? first : list(i);
+    if (x.tiles > 0) atomicAdd(&bins[x.bin], x.tiles);
+  }
+  __syncthreads();
+  const int32_t here = bins[tid];
+  int32_t before = wave_prefix(here);
+  if (lane == 63) sums[wave] = before;
+  __syncthreads();
+  int32_t total = 0;
+  for (int w = 0; w < kPlanThreads / 64; ++w) {
+    if (w == wave) before += total;
+    total += sums[w];
+  }
+  bins[tid] = before - here;
+  __syncthreads();
+  for (int32_t i = tid; i <= a.B + 1; i += kPlanThreads) {
+    const List x = i == tid ? first : list(i);
+    if (x.tiles == 0) continue;
+    const int32_t at = atomicAdd(&bins[x.bin], x.tiles);
+    for (int32_t t = 0; t < x.tiles; ++t) {
+      if (static_cast<uint32_t>(at + t) >= static_cast<uint32_t>(most)) break;  // offsets that decrease: more tiles than turns
+      Turn w{};
+      w.own = x.own;
+      w.other = x.other;
+      w.tile = keys || !a.causal ? t : x.tiles - 1 - t;
+      turns[at + t] = w;
+    }
+  }
+  for (int64_t t = int64_t{total < 0 ? 0 : total} + tid; t < most; t += kPlanThreads) turns[t].tile = -1;
+}
+
 struct FwdArgs {
   const char *q, *k, *v;           // bytes
   uint32_t q_row, k_row, v_row;    // strides in bytes (at most 2^24)
@@ -21,6 +102,8 @@ struct FwdArgs {
   int32_t H, G, D;                 // G query heads per key-value head
   int32_t causal;
   int32_t ranked;                  // find_ranked finds the tiles
+  const Turn* turns;               // find_planned does, among n_turns, if not null
+  int32_t n_turns;
   float scale;
   void* out;                       // [Nq, H, D]
   float* lse;                      // [H, Nq] or null
@@ -75,10 +158,6 @@ __device__ __forceinline__ void load_rows(X8* f, const char* base, int rows, int
   }
 }
 
-
-constexpr int kBN = 64;        // keys per tile
-constexpr int kRowWaves = 4;   // waves of 32 queries: tiles of 128
-constexpr int kRowShift = 7;
 
 // This lane's row f (its half of the columns) times the row at p, summed over
 // both half-waves.
@@ -176,7 +255,9 @@ __global__ void __launch_bounds__(kRowWaves * NS * 64, 2) fwd_kernel(const FwdAr
   const I* qo = static_cast<const I*>(a.q_offsets);
   const I* ko = static_cast<const I*>(a.k_offsets);
   Found f;
-  if (a.ranked) {
+  if (a.turns != nullptr) {
+    if (!find_planned(a.turns, a.n_turns, turn, &f)) return;
+  } else if (a.ranked) {
     if (!find_ranked<true>(qo, ko, a.B, a.Nq, a.Nk, kRowShift, a.causal != 0, turn, &f)) return;
   } else {
     if (!find_list<true>(qo, ko, a.B, a.Nq, a.Nk, kRowShift, turn, &f)) return;
@@ -353,6 +434,8 @@ struct BwdArgs {
   int32_t H, Hkv, G, D;
   int32_t causal;
   int32_t ranked;                  // find_ranked finds the tiles
+  const Turn *q_turns, *k_turns;   // find_planned does, if not null
+  int32_t n_q_turns, n_k_turns;
   float scale;
   const float* lse;                    // [H, Nq]
   float *lse2, *delta;                 // [H, Nq], workspace
@@ -374,7 +457,9 @@ __global__ void __launch_bounds__(kRowWaves * NS * 64, DP <= 64 ? 4 : NS == 1 &&
   const I* qo = static_cast<const I*>(a.q_offsets);
   const I* ko = static_cast<const I*>(a.k_offsets);
   Found f;
-  if (a.ranked) {
+  if (a.q_turns != nullptr) {
+    if (!find_planned(a.q_turns, a.n_q_turns, turn, &f)) return;
+  } else if (a.ranked) {
     if (!find_ranked<true>(qo, ko, a.B, a.Nq, a.Nk, kRowShift, a.causal != 0, turn, &f)) return;
   } else {
     if (!find_list<true>(qo, ko, a.B, a.Nq, a.Nk, kRowShift, turn, &f)) return;
@@ -580,7 +665,9 @@ __global__ void __launch_bounds__(kRowWaves * NQ * 64, 2) bwd_kv_kernel(const Bw
   const I* qo = static_cast<const I*>(a.q_offsets);
   const I* ko = static_cast<const I*>(a.k_offsets);
   Found f;
-  if (a.ranked) {
+  if (a.k_turns != nullptr) {
+    if (!find_planned(a.k_turns, a.n_k_turns, turn, &f)) return;
+  } else if (a.ranked) {
     if (!find_ranked<false>(ko, qo, a.B, a.Nk, a.Nq, kRowShift, a.causal != 0, turn, &f)) return;
   } else {
     if (!find_list<false>(ko, qo, a.B, a.Nk, a.Nq, kRowShift, turn, &f)) return;
@@ -893,13 +980,64 @@ int32_t ranked_tiles(const mx_attention_problem* p) {
          ceil_div(p->Nq, 128) * p->H > 2 * num_cus();
 }
 
+// Tiles in an order worked out by a launch of its own (about 6 us), where
+// find_ranked does not serve.  In us, without and with it: ragged lists gain, lists
+// of one length pay for the launch.  8 heads of 64, lists of 1 to 1000: 62 with 2
+// key-value heads backward 208 -> 184, forward 55.3 -> 53.9; 32 of them backward
+// 103 -> 92; 60 of 1 to 500: 71 -> 65, forward 27 -> 30; 128 of 1 to 2000: forward
+// 306 -> 291; 1000 of 100: forward 189 -> 130, backward 513 -> 348; 100 of 512:
+// forward 63 -> 66, backward 213 -> 216; 32 of 512, heads of 96: 122 -> 128.
+bool planned_tiles(const mx_attention_problem* p, bool backward) {
+  return p->B > 0 && !ranked_tiles(p) && ceil_div(p->Nq, 128) * p->H > (backward ? 2 : 16) * num_cus();
+}
+
+size_t turns_bytes(int64_t N, int64_t B) { return static_cast<size_t>(tile_turns(N, B, 128)) * sizeof(Turn); }
+
+// Each query's lse and delta, up to where turns may begin.
+size_t stats_bytes(const mx_attention_problem* p) {
+  return (static_cast<size_t>(p->Nq) * p->H * 2 * sizeof(float) + alignof(Turn) - 1) / alignof(Turn) * alignof(Turn);
+}
+
+int check_workspace(const void* workspace, size_t bytes, size_t need) {
+  if (need > 0 && (workspace == nullptr || bytes < need))
+    return mx::set_error(MX_EWORKSPACE, "workspace of %zu bytes, %zu needed", bytes, need);
+  MX_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % alignof(Turn) == 0, "workspace must start at a multiple of %zu bytes",
+             alignof(Turn));
+  return MX_OK;
+}
+
+// Writes the orders: of the queries' tiles to `turns`, and of the keys' tiles
+// after them if `keys`.
+int plan(const mx_attention_problem* p, Turn* turns, bool keys, hipStream_t stream) {
+  PlanArgs a{};
+  a.q_offsets = p->q_offsets, a.k_offsets = p->k_offsets;
+  a.B = static_cast<int32_t>(p->B), a.Nq = static_cast<int32_t>(p->Nq), a.Nk = static_cast<int32_t>(p->Nk);
+  a.causal = p->causal;
+  a.n[0] = static_cast<int32_t>(tile_turns(p->Nq, p->B, 128));
+  a.n[1] = static_cast<int32_t>(tile_turns(p->Nk, p->B, 128));
+  a.turns[0] = turns;
+  a.turns[1] = turns + a.n[0];
+  const dim3 grid(keys ? 2 : 1);
+  if (p->index_bytes == 8) plan_kernel<int64_t><<<grid, kPlanThreads, 0, stream>>>(a);
+  else plan_kernel<int32_t><<<grid, kPlanThreads, 0, stream>>>(a);
+  MX_LAUNCH_CHECK();
+  return MX_OK;
+}
+
 }  // namespace
 }  // namespace attn
 }  // namespace mx
 
+extern "C" size_t mx_jagged_attention_forward_workspace_bytes(const mx_attention_problem* p) {
+  using namespace mx::attn;
+  if (check_problem(p) != MX_OK || p->Nq == 0 || !planned_tiles(p, false)) return 0;
+  return turns_bytes(p->Nq, p->B);
+}
+
 extern "C" int mx_jagged_attention_forward(const mx_attention_problem* p, const mx_attention_tensor* q,
                                            const mx_attention_tensor* k, const mx_attention_tensor* v,
-                                           void* out, float* lse, void* stream) {
+                                           void* out, float* lse, void* workspace,
+                                           size_t workspace_bytes, void* stream) {
   using namespace mx::attn;
   mx::clear_error();
   if (int rc = check_problem(p)) return rc;
@@ -908,6 +1046,8 @@ extern "C" int mx_jagged_attention_forward(const mx_attention_problem* p, const 
   if (int rc = check_operand("v", v, p->D, p->Nk)) return rc;
   if (p->Nq == 0) return MX_OK;
   MX_REQUIRE(out != nullptr && reinterpret_cast<uintptr_t>(out) % 16 == 0, "out must be 16-byte aligned");
+  const size_t need = mx_jagged_attention_forward_workspace_bytes(p);
+  if (int rc = check_workspace(workspace, workspace_bytes, need)) return rc;
   FwdArgs a{};
   a.q = static_cast<const char*>(q->data);
   a.k = static_cast<const char*>(k->data);
@@ -922,12 +1062,21 @@ extern "C" int mx_jagged_attention_forward(const mx_attention_problem* p, const 
   a.ranked = ranked_tiles(p);
   a.out = out, a.lse = lse;
   const hipStream_t s = mx::as_stream(stream);
+  if (need > 0) {
+    Turn* turns = static_cast<Turn*>(workspace);
+    if (int rc = plan(p, turns, false, s)) return rc;
+    a.turns = turns;
+    a.n_turns = static_cast<int32_t>(tile_turns(p->Nq, p->B, 128));
+  }
   return p->dtype == MX_DTYPE_BF16 ? MX_ATTN_DISPATCH(launch_fwd, __bf16, a, p->index_bytes, s)
                                    : MX_ATTN_DISPATCH(launch_fwd, _Float16, a, p->index_bytes, s);
 }
 
-extern "C" size_t mx_jagged_attention_backward_workspace_bytes(int64_t Nq, int32_t H) {
-  return Nq > 0 && H > 0 ? static_cast<size_t>(Nq) * H * 2 * sizeof(float) : 0;
+extern "C" size_t mx_jagged_attention_backward_workspace_bytes(const mx_attention_problem* p) {
+  using namespace mx::attn;
+  if (check_problem(p) != MX_OK) return 0;
+  const size_t stats = stats_bytes(p);
+  return planned_tiles(p, true) ? stats + turns_bytes(p->Nq, p->B) + turns_bytes(p->Nk, p->B) : stats;
 }
 
 extern "C" int mx_jagged_attention_backward(const mx_attention_problem* p, const mx_attention_tensor* q,
@@ -948,9 +1097,8 @@ extern "C" int mx_jagged_attention_backward(const mx_attention_problem* p, const
   MX_REQUIRE((dk == nullptr) == (dv == nullptr), "dk and dv: both or neither");
   for (const void* x : {dq, dk, dv})
     MX_REQUIRE(reinterpret_cast<uintptr_t>(x) % 16 == 0, "gradients must be 16-byte aligned");
-  const size_t need = mx_jagged_attention_backward_workspace_bytes(p->Nq, p->H);
-  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
-    return mx::set_error(MX_EWORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  if (int rc = check_workspace(workspace, workspace_bytes, mx_jagged_attention_backward_workspace_bytes(p)))
+    return rc;
   BwdArgs a{};
   a.q = static_cast<const char*>(q->data);
   a.k = static_cast<const char*>(k->data);
@@ -972,6 +1120,14 @@ extern "C" int mx_jagged_attention_backward(const mx_attention_problem* p, const
   a.delta = a.lse2 + p->Nq * p->H;
   a.dq = dq, a.dk = dk, a.dv = dv;
   const hipStream_t s = mx::as_stream(stream);
+  if (planned_tiles(p, true)) {
+    Turn* turns = reinterpret_cast<Turn*>(static_cast<char*>(workspace) + stats_bytes(p));
+    if (int rc = plan(p, turns, dk != nullptr, s)) return rc;
+    a.n_q_turns = static_cast<int32_t>(tile_turns(p->Nq, p->B, 128));
+    a.n_k_turns = static_cast<int32_t>(tile_turns(p->Nk, p->B, 128));
+    a.q_turns = turns;
+    a.k_turns = turns + a.n_q_turns;
+  }
   return p->dtype == MX_DTYPE_BF16 ? MX_ATTN_DISPATCH(launch_bwd, __bf16, a, p->index_bytes, s)
                                    : MX_ATTN_DISPATCH(launch_bwd, _Float16, a, p->index_bytes, s);
 }

@@ -2027,8 +2027,12 @@ Tensor run_jagged_attention(const Tensor& q, const Tensor& k, const Tensor& v,
   pack_attention(q, k, v, q_offsets, k_offsets, causal, scale, c);
   Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
   if (lse != nullptr) *lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
+  const size_t ws_bytes = mx_jagged_attention_forward_workspace_bytes(&c.p);
+  Tensor ws;
+  if (ws_bytes > 0) ws = at::empty({static_cast<int64_t>(ws_bytes)}, q.options().dtype(at::kByte));
   MX_CALL(mx_jagged_attention_forward(&c.p, &c.q, &c.k, &c.v, out.data_ptr(),
-                                      lse != nullptr ? lse->data_ptr<float>() : nullptr, stream_of(q)));
+                                      lse != nullptr ? lse->data_ptr<float>() : nullptr,
+                                      ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, stream_of(q)));
   return out;
 }
 
@@ -2074,7 +2078,7 @@ std::tuple<Tensor, Tensor, Tensor> run_jagged_attention_backward(
     dk = at::empty(k.sizes(), opts);
     dv = at::empty(k.sizes(), opts);
   }
-  const size_t ws_bytes = mx_jagged_attention_backward_workspace_bytes(q.size(0), c.p.H);
+  const size_t ws_bytes = mx_jagged_attention_backward_workspace_bytes(&c.p);
   Tensor ws = at::empty({static_cast<int64_t>(ws_bytes)}, q.options().dtype(at::kByte));
   MX_CALL(mx_jagged_attention_backward(
       &c.p, &c.q, &c.k, &c.v, &o, &g, lse.data_ptr<float>(), dq.data_ptr(),
