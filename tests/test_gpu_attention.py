@@ -112,6 +112,19 @@ def test_many_tiles(dev, lists, most, index, causal):
     run(dev, q, k, v, qo, ko, causal, None, "bfloat16", g, index)
 
 
+@pytest.mark.parametrize("H,Hkv", [(8, 1), (3, 3)])
+@pytest.mark.parametrize("D", [24, 64, 96, 128])
+@pytest.mark.parametrize("causal", [True, False])
+def test_shared_out_queries(dev, H, Hkv, D, causal):
+    """Few keys under many queries: each key's gradients are sums of several
+    shares, some of them empty, some lists without queries or keys."""
+    qo, ko = offsets_of([0, 1, 900, 70, 300]) + 2, offsets_of([40, 3, 500, 0, 310]) + 1
+    Nq, Nk = int(qo[-1]) + 3, int(ko[-1]) + 5
+    q, g = make(Nq, H, D, "float16", 1), make(Nq, H, D, "float16", 2)
+    k, v = make(Nk, Hkv, D, "float16", 3), make(Nk, Hkv, D, "float16", 4)
+    run(dev, q, k, v, qo, ko, causal, None, "float16", g)
+
+
 @pytest.mark.parametrize("dtype,D", [("float16", 128), ("bfloat16", 128), ("bfloat16", 64)])
 def test_long_lists(dev, dtype, D):
     o = offsets_of([1500, 777])

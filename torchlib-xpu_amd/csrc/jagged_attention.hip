@@ -7,6 +7,7 @@
 //   s_ij = scale q_i.k_j,  lse_i = log sum_j exp(s_ij),  p_ij = exp(s_ij - lse_i),
 //   o_i = sum_j p_ij v_j;   a query that sees no key has o_i = 0, lse_i = -inf.
 #include "attention_common.h"
+#include <algorithm>
 
 namespace mx {
 namespace attn {
@@ -145,6 +146,21 @@ __device__ __forceinline__ void store_rows(void* base, const f32x16* acc, float 
     }
 }
 
+// The same unscaled in fp32, at `base` of a contiguous [.., heads, D].
+template <int DP>
+__device__ __forceinline__ void store_sums(float* base, const f32x16* acc, int rows, int heads, int D,
+                                           int l, int h) {
+  if (l >= rows) return;
+  float* row = base + int64_t{l} * heads * D + 4 * h;
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const int col = 32 * d + 8 * (i / 4);
+      if (col < D) *reinterpret_cast<f32x4*>(row + col) = f32x4{acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]};
+    }
+}
+
 // Row l of a 32-row tile as the B operand: 8 columns per step.
 template <typename X8, int KS>
 __device__ __forceinline__ void load_rows(X8* f, const char* base, int rows, int64_t stride, int D,
@@ -235,11 +251,22 @@ __device__ __forceinline__ void rows_key_by_key(const X8* qf, const char* kp, in
 // One block: four waves, 32 queries each, of one list and head (twice four with
 // NS = 2: two groups take alternate tiles of keys, and join their sums through
 // LDS at the end).  Tiles of 64 keys and values go to LDS, the next one while
-// this one is worked on.  Per tile a
-// wave computes K Q^T (a query per lane), the running maximum and sum of its
-// queries in registers, and adds V^T P^T to its outputs, which are rescaled
-// only when a maximum has grown by more than 2^8.  Probabilities are rounded to
-// the input type for the second product; sums, maxima and outputs are fp32.
+// this one is worked on.  Per tile a wave computes K Q^T (a query per lane, so
+// that its probabilities are the next product's operand as they stand), the
+// running maximum m and sum of exp(s - m) of its queries in registers, and adds
+// V^T P^T to its outputs; outputs and sum are multiplied by exp(m - m') only when
+// a maximum has grown by more than 2^8 (until then exp(s - m) <= 2^8).
+// Probabilities are rounded to the input type for the second product, whose
+// matrix instruction takes no wider one; sums, maxima and outputs are fp32.
+//
+// Bound: long lists by the issue of the matrix products and of the softmax's
+// vector instructions between them (2 lists of 8192, 16 heads of 128 over 4:
+// 548 us, 1.0 PFLOP/s of the visible pairs, matrix pipes busy for half the cycles,
+// no LDS conflicts, 0.3 TB/s); many short ones by latency: to a block's first
+// tile it is 4 to 5 us (the list, then queries and keys), of a life of 8 to 16
+// (64 lists of 1 to 1000, 8 heads of 64 over 2: 51 us, 1.6 TB/s; 256 lists of up
+// to 512, 8 heads of 96: 41 us).  Hence four waves and two tiles in turn: 3 or
+// 4 blocks a CU; three tiles, or one or two waves a block, were slower.
 template <typename T, typename I, int DP, int NS>
 __global__ void __launch_bounds__(kRowWaves * NS * 64, 2) fwd_kernel(const FwdArgs a) {
   using E = Elem<T>;
@@ -440,8 +467,17 @@ struct BwdArgs {
   const float* lse;                    // [H, Nq]
   float *lse2, *delta;                 // [H, Nq], workspace
   void *dq, *dk, *dv;                  // contiguous
+  int32_t shares;                      // of a key tile's queries (bwd_kv_kernel)
+  float* sums;                         // [shares, 2, Nk, Hkv, D], workspace if shares > 1
 };
 
+// The queries' launch: tiles as in the forward.  A wave keeps Q and dO of its 32
+// queries as operands and dQ as sums; per tile it computes S and dP with a query
+// per lane and adds K^T dS^T.  Where all keys of a query fit one tile, delta is
+// sum_j p_ij dP_ij from there (exact to the rounding of P) and the output is not
+// read; else it is dO.o.  Bound as the forward's (4 lists of 4096, 16 heads of 128
+// over 4: 409 us, 1.0 PFLOP/s, matrix pipes 53%; 256 lists of up to 512, 8 heads
+// of 96: 50 us).
 template <typename T, typename I, int DP, int NS>
 __global__ void __launch_bounds__(kRowWaves * NS * 64, DP <= 64 ? 4 : NS == 1 && DP == 96 ? 3 : 2) bwd_q_kernel(const BwdArgs a) {
   using E = Elem<T>;
@@ -641,7 +677,10 @@ __global__ void __launch_bounds__(kRowWaves * NS * 64, DP <= 64 ? 4 : NS == 1 &&
 // LDS at the end).  Queries and dO go through LDS with their lse and delta;
 // scores come out with a key per lane.  D = 128 takes 192 registers for K, V,
 // dK and dV: scores are used up before dP is computed, which leaves two waves
-// per SIMD.
+// per SIMD.  Bound: the matrix products' issue and the LDS reads that feed them
+// with only two waves to hide either (4 lists of 4096, 16 heads of 128 over 4:
+// 610 us, 0.9 PFLOP/s, matrix pipes 44%); short lists by latency as above (256
+// lists of up to 512, 8 heads of 96: 63 us).
 template <typename T, typename I, int DP, int NQ>
 __global__ void __launch_bounds__(kRowWaves * NQ * 64, 2) bwd_kv_kernel(const BwdArgs a) {
   using E = Elem<T>;
@@ -688,6 +727,10 @@ __global__ void __launch_bounds__(kRowWaves * NQ * 64, 2) bwd_kv_kernel(const Bw
   // From the first query that sees a key of the block, to a whole 64.
   const int first = a.causal && tile * BM > shift ? (tile * BM - shift) / 64 * 64 : 0;
   const int per = Lq > first ? (Lq - first + BQ - 1) / BQ : 0;
+  // This share's blocks of BQ queries, counted through the group's heads.
+  const int share = blockIdx.y;
+  const int begin = static_cast<int>(int64_t{per} * a.G * share / a.shares);
+  const int end = static_cast<int>(int64_t{per} * a.G * (share + 1) / a.shares);
 
   X8 kf[KS], vf[KS];
   load_rows<X8, KS>(kf, a.k + k_base * a.k_row + kvh * a.k_head, keys, a.k_row, a.D, l, h);
@@ -796,14 +839,17 @@ __global__ void __launch_bounds__(kRowWaves * NQ * 64, 2) bwd_kv_kernel(const Bw
     }
   };
 
-  if (per > 0) load_tile(0, 0, lds);
   uint32_t buf = 0;
-  for (int g = 0, t = 0; per > 0 && g < a.G; buf = kBuf - buf) {
-    const int tn = t + 1 < per ? t + 1 : 0, gn = t + 1 < per ? g : g + 1;
-    wait_and_barrier<0>();
-    work(t, lds, buf, lds + (kBuf - buf), gn, tn, gn < a.G);
-    t = tn;
-    g = gn;
+  if (begin < end) {
+    int g = begin / per, t = begin - g * per;
+    load_tile(g, t, lds);
+    for (int left = end - begin; left > 0; --left, buf = kBuf - buf) {
+      const int tn = t + 1 < per ? t + 1 : 0, gn = t + 1 < per ? g : g + 1;
+      wait_and_barrier<0>();
+      work(t, lds, buf, lds + (kBuf - buf), gn, tn, left > 1);
+      t = tn;
+      g = gn;
+    }
   }
 
   if constexpr (NQ == 2) {
@@ -840,10 +886,11 @@ __global__ void __launch_bounds__(kRowWaves * NQ * 64, 2) bwd_kv_kernel(const Bw
 #pragma unroll
     for (int d = 0; d < DB; ++d) dk[d] = dv[d] = f32x16{};
 #pragma unroll 1
-    for (int u = 0; u < a.G; ++u) {
-      const int head = kvh * a.G + u;
+    for (int u = begin; u < end; ++u) {
+      const int head = kvh * a.G + u / per;
+      const int i0 = first + u % per * BQ, i1 = min_of(i0 + BQ, Lq);
 #pragma unroll 1
-      for (int i = first; i < Lq; ++i) {
+      for (int i = i0; i < i1; ++i) {
         const char* qp = a.q + (qs + i) * a.q_row + head * a.q_head;
         const char* gp = a.grad + (qs + i) * a.g_row + head * a.g_head;
         const int64_t at_i = int64_t{head} * a.Nq + qs + i;
@@ -861,14 +908,39 @@ __global__ void __launch_bounds__(kRowWaves * NQ * 64, 2) bwd_kv_kernel(const Bw
     }
   }
   const int64_t to = (k_base * a.Hkv + kvh) * a.D;
+  if (a.shares > 1) {
+    const int64_t all = int64_t{a.Nk} * a.Hkv * a.D;
+    store_sums<DP>(a.sums + 2 * share * all + to, dk, keys, a.Hkv, a.D, le, he);
+    store_sums<DP>(a.sums + (2 * share + 1) * all + to, dv, keys, a.Hkv, a.D, le, he);
+    return;
+  }
   store_rows<T, DP>(static_cast<T*>(a.dk) + to, dk, a.scale, keys, a.Hkv, a.D, le, he);
   store_rows<T, DP>(static_cast<T*>(a.dv) + to, dv, 1.0f, keys, a.Hkv, a.D, le, he);
+}
+
+// dK and dV from their shares' sums, added in the shares' order, four values a
+// thread.  Bound: reading the sums, which the caches still hold.
+template <typename T>
+__global__ void __launch_bounds__(256) join_shares_kernel(const BwdArgs a) {
+  typedef T x4 __attribute__((ext_vector_type(4)));
+  const int64_t all = int64_t{a.Nk} * a.Hkv * a.D;
+  const int64_t i = (int64_t{blockIdx.x} * 256 + threadIdx.x) * 4;
+  if (i >= all) return;
+  const bool v = blockIdx.y == 1;
+  const float* p = a.sums + (v ? all : 0) + i;
+  f32x4 sum{};
+#pragma unroll 4
+  for (int s = 0; s < a.shares; ++s) sum += *reinterpret_cast<const f32x4*>(p + 2 * s * all);
+  const float scale = v ? 1.0f : a.scale;
+  x4 w;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = static_cast<T>(sum[e] * scale);
+  *reinterpret_cast<x4*>(static_cast<T*>(v ? a.dv : a.dk) + i) = w;
 }
 
 // ---------------------------------------------------------------------------
 // Launches
 // ---------------------------------------------------------------------------
-
 
 // Waves beyond a block's four where the launch's tiles of 128 rows do not fill
 // the chip, on lists long enough to share out.  Times in us, 8 heads of 128:
@@ -882,6 +954,26 @@ bool split_keys(int64_t Nq, int64_t Nk, int64_t B, int64_t H) {
 }
 bool split_queries(int64_t Nq, int64_t Nk, int64_t B, int64_t Hkv, int64_t G) {
   return B > 0 && ceil_div(Nk, 128) * Hkv <= 2 * num_cus() && Nq / B * G >= 1024;
+}
+
+// Shares of a key tile's queries where the tiles leave part of the chip idle, joined
+// by a third launch: up to two blocks of four waves, or one of eight, for every CU,
+// and two tiles of queries in each share of a list of mean length.  Whole
+// backward in us, without and with them (more than 4, 8 or 16 shares once the chip
+// is full gain no more): one list of 1059, 8 heads of 128 over 1: 291 -> 74; 4096,
+// 8 of 64 over 1: 632 -> 154; 4096, 16 of 128 over 2: 1026 -> 404; 2 of 400, 8 of
+// 64 over 1: 86 -> 35; 4 of 1 to 1000, 4 heads of 96: 70 -> 60; 2 of 300, 2 heads
+// of 128: 42 -> 39; with four tiles a share at least 8 of 1 to 500, 8 of 64 over 1,
+// 52, with two 42, with one 44.
+int32_t query_shares(const mx_attention_problem* p) {
+  if (p->B == 0 || p->Nk == 0) return 1;
+  const int64_t G = p->H / p->Hkv, blocks = ceil_div(p->Nk, 128) * p->Hkv;
+  const bool two = split_queries(p->Nq, p->Nk, p->B, p->Hkv, G);
+  const int64_t room = (two ? 1 : 2) * static_cast<int64_t>(num_cus()) / blocks;
+  const int64_t work = p->Nq / p->B * G / (two ? 256 : 128);
+  const int64_t n = std::min<int64_t>({room, work, 16});
+
+  return n > 1 ? static_cast<int32_t>(n) : 1;
 }
 
 int blocks_of(int64_t rows, int64_t B, int64_t heads, unsigned* blocks) {
@@ -915,10 +1007,15 @@ int launch_bwd(const BwdArgs& a, hipStream_t stream) {
       bwd_q_kernel<T, I, DP, 1><<<dim3(qblocks), 256, 0, stream>>>(a);
   }
   if (a.Nk > 0 && a.dk != nullptr) {
+    const dim3 grid(kblocks, a.shares);
     if (split_queries(a.Nq, a.Nk, a.B, a.Hkv, a.G))
-      bwd_kv_kernel<T, I, DP, 2><<<dim3(kblocks), 512, 0, stream>>>(a);
+      bwd_kv_kernel<T, I, DP, 2><<<grid, 512, 0, stream>>>(a);
     else
-      bwd_kv_kernel<T, I, DP, 1><<<dim3(kblocks), 256, 0, stream>>>(a);
+      bwd_kv_kernel<T, I, DP, 1><<<grid, 256, 0, stream>>>(a);
+    if (a.shares > 1) {
+      const int64_t n = ceil_div(int64_t{a.Nk} * a.Hkv * a.D, 1024);
+      join_shares_kernel<T><<<dim3(static_cast<unsigned>(n), 2), 256, 0, stream>>>(a);
+    }
   }
   MX_LAUNCH_CHECK();
   return MX_OK;
@@ -998,6 +1095,11 @@ size_t stats_bytes(const mx_attention_problem* p) {
   return (static_cast<size_t>(p->Nq) * p->H * 2 * sizeof(float) + alignof(Turn) - 1) / alignof(Turn) * alignof(Turn);
 }
 
+// The backward's workspace: stats, turns, the shares' sums.
+size_t sums_at(const mx_attention_problem* p) {
+  return stats_bytes(p) + (planned_tiles(p, true) ? turns_bytes(p->Nq, p->B) + turns_bytes(p->Nk, p->B) : 0);
+}
+
 int check_workspace(const void* workspace, size_t bytes, size_t need) {
   if (need > 0 && (workspace == nullptr || bytes < need))
     return mx::set_error(MX_EWORKSPACE, "workspace of %zu bytes, %zu needed", bytes, need);
@@ -1075,8 +1177,10 @@ extern "C" int mx_jagged_attention_forward(const mx_attention_problem* p, const 
 extern "C" size_t mx_jagged_attention_backward_workspace_bytes(const mx_attention_problem* p) {
   using namespace mx::attn;
   if (check_problem(p) != MX_OK) return 0;
-  const size_t stats = stats_bytes(p);
-  return planned_tiles(p, true) ? stats + turns_bytes(p->Nq, p->B) + turns_bytes(p->Nk, p->B) : stats;
+  size_t n = sums_at(p);
+  const int64_t shares = query_shares(p);
+  if (shares > 1) n += static_cast<size_t>(shares) * 2 * p->Nk * p->Hkv * p->D * sizeof(float);
+  return n;
 }
 
 extern "C" int mx_jagged_attention_backward(const mx_attention_problem* p, const mx_attention_tensor* q,
@@ -1120,6 +1224,8 @@ extern "C" int mx_jagged_attention_backward(const mx_attention_problem* p, const
   a.delta = a.lse2 + p->Nq * p->H;
   a.dq = dq, a.dk = dk, a.dv = dv;
   const hipStream_t s = mx::as_stream(stream);
+  a.shares = query_shares(p);
+  a.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + sums_at(p));
   if (planned_tiles(p, true)) {
     Turn* turns = reinterpret_cast<Turn*>(static_cast<char*>(workspace) + stats_bytes(p));
     if (int rc = plan(p, turns, dk != nullptr, s)) return rc;
