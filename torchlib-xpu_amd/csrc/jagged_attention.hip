@@ -943,14 +943,19 @@ __global__ void __launch_bounds__(256) join_shares_kernel(const BwdArgs a) {
 // ---------------------------------------------------------------------------
 
 // Waves beyond a block's four where the launch's tiles of 128 rows do not fill
-// the chip, on lists long enough to share out.  Times in us, 8 heads of 128:
-//   forward, key tiles over two groups: 1 list of 4096 94 -> 78, 16 lists of 128
-//   queries and 1128 keys 34.4 -> 32.5; 4 lists of 2048 (512 tiles) 58 -> 60;
-//   backward's keys, queries over two groups (whole backward): 1 x 4096
-//   310 -> 258, 4 x 2048 (512 tiles) 184 -> 173, 6 x 2048 211 -> 233, 16 x 512
+// the chip, on lists long enough to share out.  Times in us:
+//   key tiles over two groups, forward: 1 list of 4096, 8 heads of 128 (256 tiles)
+//   94 -> 78; 16 lists of 128 queries and 1128 keys, 8 of 128, 34.4 -> 32.5; 1 of
+//   5282, 8 of 64 (336 tiles) 84 -> 67; 2 of 4096 (512 tiles) 82 -> 73, 8 of 128
+//   121 -> 94; 4 of 2048 (512 tiles) 45.2 -> 41.6, 8 of 128 65.6 -> 68.3; 8 of 1024
+//   (512 tiles), 8 of 128, 38.6 -> 48.4;
+//   backward's keys, queries over two groups (whole backward), 8 heads of 128: 1 x
+//   4096 310 -> 258, 4 x 2048 (512 tiles) 184 -> 173, 6 x 2048 211 -> 233, 16 x 512
 //   (512 tiles) 71 -> 81, the same with 2 key-value heads 127 -> 101.
 bool split_keys(int64_t Nq, int64_t Nk, int64_t B, int64_t H) {
-  return B > 0 && ceil_div(Nq, 128) * H <= num_cus() && Nk / B >= 512;
+  if (B == 0) return false;
+  const int64_t tiles = ceil_div(Nq, 128) * H, mean = Nk / B, cus = num_cus();
+  return (2 * tiles <= 3 * cus && mean >= 512) || (tiles <= 2 * cus && mean >= 4096);
 }
 bool split_queries(int64_t Nq, int64_t Nk, int64_t B, int64_t Hkv, int64_t G) {
   return B > 0 && ceil_div(Nk, 128) * Hkv <= 2 * num_cus() && Nq / B * G >= 1024;
