@@ -261,11 +261,11 @@ __device__ __forceinline__ void rows_key_by_key(const X8* qf, const char* kp, in
 //
 // Bound: long lists by the issue of the matrix products and of the softmax's
 // vector instructions between them (2 lists of 8192, 16 heads of 128 over 4:
-// 548 us, 1.0 PFLOP/s of the visible pairs, matrix pipes busy for half the cycles,
+// 518 to 548 us, 1.0 PFLOP/s of the visible pairs, matrix pipes busy for half the cycles,
 // no LDS conflicts, 0.3 TB/s); many short ones by latency: to a block's first
 // tile it is 4 to 5 us (the list, then queries and keys), of a life of 8 to 16
-// (64 lists of 1 to 1000, 8 heads of 64 over 2: 51 us, 1.6 TB/s; 256 lists of up
-// to 512, 8 heads of 96: 41 us).  Hence four waves and two tiles in turn: 3 or
+// (64 lists of 0 to 1000, 8 heads of 64 over 2: 48 to 51 us, 1.6 TB/s; 256 lists of
+// up to 512, 8 heads of 96: 41 us).  Hence four waves and two tiles in turn: 3 or
 // 4 blocks a CU; three tiles, or one or two waves a block, were slower.
 template <typename T, typename I, int DP, int NS>
 __global__ void __launch_bounds__(kRowWaves * NS * 64, 2) fwd_kernel(const FwdArgs a) {
