@@ -112,6 +112,17 @@ def test_many_tiles(dev, lists, most, index, causal):
     run(dev, q, k, v, qo, ko, causal, None, "bfloat16", g, index)
 
 
+@pytest.mark.parametrize("Hkv", [16, 32, 64])
+@pytest.mark.parametrize("causal", [True, False])
+def test_heads_of_a_block(dev, Hkv, causal):
+    """Four, two and one query heads of a block, on tiles found by rank: more
+    keys than queries, fewer, and a single query."""
+    qo, ko = offsets_of([400, 1, 330, 410]), offsets_of([900, 1300, 300, 1200])
+    q, g = make(int(qo[-1]), 64, 8, "bfloat16", 1), make(int(qo[-1]), 64, 8, "bfloat16", 2)
+    k, v = make(int(ko[-1]), Hkv, 8, "bfloat16", 3), make(int(ko[-1]), Hkv, 8, "bfloat16", 4)
+    run(dev, q, k, v, qo, ko, causal, None, "bfloat16", g)
+
+
 @pytest.mark.parametrize("H,Hkv", [(8, 1), (3, 3)])
 @pytest.mark.parametrize("D", [24, 64, 96, 128])
 @pytest.mark.parametrize("causal", [True, False])

@@ -14,7 +14,7 @@ namespace attn {
 namespace {
 
 constexpr int kBN = 64;        // keys per tile
-constexpr int kRowWaves = 4;   // waves of 32 queries: tiles of 128
+constexpr int kRowWaves = 4;   // waves of 32 queries: tiles of 128, of one head
 constexpr int kRowShift = 7;
 
 struct PlanArgs {
@@ -22,6 +22,7 @@ struct PlanArgs {
   int32_t B, Nq, Nk, causal;
   Turn* turns[2];                  // of the queries' tiles and the keys' tiles
   int32_t n[2];
+  int32_t shift[2];                // log2 of a tile's rows
 };
 
 // The order of a launch's tiles where lists are many and long: list by list, those
@@ -41,7 +42,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
   const I* other = static_cast<const I*>(keys ? a.q_offsets : a.k_offsets);
   const int32_t N = keys ? a.Nk : a.Nq, Nother = keys ? a.Nq : a.Nk;
   Turn* turns = a.turns[blockIdx.x];
-  const int32_t most = a.n[blockIdx.x];
+  const int32_t most = a.n[blockIdx.x], shift = a.shift[blockIdx.x];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
 
   struct List { Span own, other; int32_t tiles, bin; };
@@ -52,7 +53,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
     const int32_t os = list_start(other, a.B, Nother, i), oe = list_start(other, a.B, Nother, i + 1);
     x.own = {s, e > s ? e - s : 0};
     x.other = {os, i > 0 && i <= a.B && oe > os ? oe - os : 0};
-    x.tiles = (x.own.len + 127) >> kRowShift;
+    x.tiles = (x.own.len + (1 << shift) - 1) >> shift;
     // 2^0 .. 2^22 partners: bins 736 .. 1 from the end.
     const int32_t bits = static_cast<int32_t>(__float_as_uint(static_cast<float>(x.other.len)) >> 18) - (127 << 5) + 1;
     x.bin = kPlanThreads - 1 - (bits > 0 ? bits : 0);
@@ -102,6 +103,7 @@ struct FwdArgs {
   int32_t B, Nq, Nk;
   int32_t H, G, D;                 // G query heads per key-value head
   int32_t causal;
+  int32_t pack;                    // log2 of the heads of a block
   int32_t ranked;                  // find_ranked finds the tiles
   const Turn* turns;               // find_planned does, among n_turns, if not null
   int32_t n_turns;
@@ -248,7 +250,8 @@ __device__ __forceinline__ void rows_key_by_key(const X8* qf, const char* kp, in
   *sum_out = sum;
 }
 
-// One block: four waves, 32 queries each, of one list and head (twice four with
+// One block: four waves, 32 queries each, of one list and one head, or on short
+// lists of two or four heads that share their keys (twice four waves with
 // NS = 2: two groups take alternate tiles of keys, and join their sums through
 // LDS at the end).  Tiles of 64 keys and values go to LDS, the next one while
 // this one is worked on.  Per tile a wave computes K Q^T (a query per lane, so
@@ -261,7 +264,7 @@ __device__ __forceinline__ void rows_key_by_key(const X8* qf, const char* kp, in
 //
 // Bound: long lists by the issue of the matrix products and of the softmax's
 // vector instructions between them (2 lists of 8192, 16 heads of 128 over 4:
-// 518 to 548 us, 1.0 PFLOP/s of the visible pairs, matrix pipes busy for half the cycles,
+// 518 to 566 us, 1.0 PFLOP/s of the visible pairs, matrix pipes busy for half the cycles,
 // no LDS conflicts, 0.3 TB/s); many short ones by latency: to a block's first
 // tile it is 4 to 5 us (the list, then queries and keys), of a life of 8 to 16
 // (64 lists of 0 to 1000, 8 heads of 64 over 2: 48 to 51 us, 1.6 TB/s; 256 lists of
@@ -272,32 +275,35 @@ __global__ void __launch_bounds__(kRowWaves * NS * 64, 2) fwd_kernel(const FwdAr
   using E = Elem<T>;
   using X8 = typename E::x8;
   using Ti = Tile<DP>;
-  constexpr int KS = DP / 16, DB = DP / 32, BM = kRowWaves * 32;
+  constexpr int KS = DP / 16, DB = DP / 32;
   constexpr int kTileBytes = kBN * DP * 2;
   __shared__ __attribute__((aligned(1024))) char lds[NS * 4 * kTileBytes];  // K0 V0 K1 V1 per group
 
   int head;
   int turn;
-  head_and_turn(blockIdx.x, a.H, &head, &turn);
+  head_and_turn(blockIdx.x, a.H >> a.pack, &head, &turn);
   const I* qo = static_cast<const I*>(a.q_offsets);
   const I* ko = static_cast<const I*>(a.k_offsets);
   Found f;
   if (a.turns != nullptr) {
     if (!find_planned(a.turns, a.n_turns, turn, &f)) return;
   } else if (a.ranked) {
-    if (!find_ranked<true>(qo, ko, a.B, a.Nq, a.Nk, kRowShift, a.causal != 0, turn, &f)) return;
+    if (!find_ranked<true>(qo, ko, a.B, a.Nq, a.Nk, kRowShift - a.pack, a.causal != 0, turn, &f)) return;
   } else {
-    if (!find_list<true>(qo, ko, a.B, a.Nq, a.Nk, kRowShift, turn, &f)) return;
+    if (!find_list<true>(qo, ko, a.B, a.Nq, a.Nk, kRowShift - a.pack, turn, &f)) return;
   }
   const Span sq = f.own, sk = f.other;
   const int tile = f.tile;
+  const int BM = kRowWaves * 32 >> a.pack;      // the tile's queries
   if (tile < 0 || tile * BM >= sq.len) return;  // (below 0: offsets that decrease)
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, l = lane & 31, h = lane >> 5;
   const int group = wave / kRowWaves;                   // of the key tiles j with j % NS == group
-  const int row0 = tile * BM + wave % kRowWaves * 32;  // the wave's first query in the list
+  const int per_head = kRowWaves >> a.pack, sub = wave % kRowWaves;  // waves
+  head = (head << a.pack) + (sub >> (2 - a.pack));
+  const int row0 = tile * BM + (sub & (per_head - 1)) * 32;  // the wave's first query in the list
   const int64_t q_base = sq.start + row0;
   const int rows = rows_left(sq.len, row0, 32);
   const int Lk = sk.len;
@@ -460,6 +466,7 @@ struct BwdArgs {
   int32_t B, Nq, Nk;
   int32_t H, Hkv, G, D;
   int32_t causal;
+  int32_t pack;                    // log2 of the heads of a block (queries' launch)
   int32_t ranked;                  // find_ranked finds the tiles
   const Turn *q_turns, *k_turns;   // find_planned does, if not null
   int32_t n_q_turns, n_k_turns;
@@ -483,32 +490,35 @@ __global__ void __launch_bounds__(kRowWaves * NS * 64, DP <= 64 ? 4 : NS == 1 &&
   using E = Elem<T>;
   using X8 = typename E::x8;
   using Ti = Tile<DP>;
-  constexpr int KS = DP / 16, DB = DP / 32, BM = kRowWaves * 32;
+  constexpr int KS = DP / 16, DB = DP / 32;
   constexpr int kTileBytes = kBN * DP * 2;
   __shared__ __attribute__((aligned(1024))) char lds[NS * 4 * kTileBytes];
 
   int head;
   int turn;
-  head_and_turn(blockIdx.x, a.H, &head, &turn);
+  head_and_turn(blockIdx.x, a.H >> a.pack, &head, &turn);
   const I* qo = static_cast<const I*>(a.q_offsets);
   const I* ko = static_cast<const I*>(a.k_offsets);
   Found f;
   if (a.q_turns != nullptr) {
     if (!find_planned(a.q_turns, a.n_q_turns, turn, &f)) return;
   } else if (a.ranked) {
-    if (!find_ranked<true>(qo, ko, a.B, a.Nq, a.Nk, kRowShift, a.causal != 0, turn, &f)) return;
+    if (!find_ranked<true>(qo, ko, a.B, a.Nq, a.Nk, kRowShift - a.pack, a.causal != 0, turn, &f)) return;
   } else {
-    if (!find_list<true>(qo, ko, a.B, a.Nq, a.Nk, kRowShift, turn, &f)) return;
+    if (!find_list<true>(qo, ko, a.B, a.Nq, a.Nk, kRowShift - a.pack, turn, &f)) return;
   }
   const Span sq = f.own, sk = f.other;
   const int tile = f.tile;
+  const int BM = kRowWaves * 32 >> a.pack;      // the tile's queries
   if (tile < 0 || tile * BM >= sq.len) return;  // (below 0: offsets that decrease)
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, l = lane & 31, h = lane >> 5;
   const int group = wave / kRowWaves;                   // of the key tiles j with j % NS == group
-  const int row0 = tile * BM + wave % kRowWaves * 32;  // the wave's first query in the list
+  const int per_head = kRowWaves >> a.pack, sub = wave % kRowWaves;  // waves
+  head = (head << a.pack) + (sub >> (2 - a.pack));
+  const int row0 = tile * BM + (sub & (per_head - 1)) * 32;  // the wave's first query in the list
   const int64_t q_base = sq.start + row0;
   const int rows = rows_left(sq.len, row0, 32);
   const int Lk = sk.len;
@@ -981,8 +991,23 @@ int32_t query_shares(const mx_attention_problem* p) {
   return n > 1 ? static_cast<int32_t>(n) : 1;
 }
 
-int blocks_of(int64_t rows, int64_t B, int64_t heads, unsigned* blocks) {
-  const int64_t n = tile_turns(rows, B, 128) * heads;
+// Query heads (log2) that a block of the queries' launches takes, of those that
+// share a key-value head: its four waves have 32 queries of four heads, 64 of two
+// or 128 of one, and read the same keys.  Short lists leave fewer waves without a
+// query; long ones start more blocks that must find their tile.  In us, one head
+// and as many as there are: 117 lists of 27 with 249 keys, 16 heads of 128 over 4:
+// forward 32.5 -> 21.8, with the backward 114 -> 87; 200 of 1 to 60, 8 of 64 over
+// 2: 12.4 -> 9.0; 173 of 1 to 344, 4 of 80 over 1, with the backward 116 -> 105; 32
+// of 1 to 600, 8 of 96 over 4: 22.6 -> 21.8; 64 of 1 to 1000, 8 of 64 over 2: 48.5
+// -> 49.4; 16 of 512, 8 of 128 over 2: 23.0 -> 24.7; 2 of 8192: the same.
+int heads_packed(const mx_attention_problem* p) {
+  const int32_t G = p->H / p->Hkv;
+  if (p->Nq > 384 * p->B) return 0;
+  return G % 4 == 0 ? 2 : G % 2 == 0 ? 1 : 0;
+}
+
+int blocks_of(int64_t rows, int64_t B, int64_t heads, int pack, unsigned* blocks) {
+  const int64_t n = tile_turns(rows, B, 128 >> pack) * (heads >> pack);
   MX_REQUIRE(n < (1ll << 23), "too many tiles: %lld", (long long)n);  // of 512 threads in 32 bits
   *blocks = static_cast<unsigned>(n);
   return MX_OK;
@@ -991,7 +1016,7 @@ int blocks_of(int64_t rows, int64_t B, int64_t heads, unsigned* blocks) {
 template <typename T, typename I, int DP>
 int launch_fwd(const FwdArgs& a, hipStream_t stream) {
   unsigned blocks;
-  if (int rc = blocks_of(a.Nq, a.B, a.H, &blocks)) return rc;
+  if (int rc = blocks_of(a.Nq, a.B, a.H, a.pack, &blocks)) return rc;
   if (split_keys(a.Nq, a.Nk, a.B, a.H))
     fwd_kernel<T, I, DP, 2><<<dim3(blocks), 512, 0, stream>>>(a);
   else
@@ -1003,8 +1028,8 @@ int launch_fwd(const FwdArgs& a, hipStream_t stream) {
 template <typename T, typename I, int DP>
 int launch_bwd(const BwdArgs& a, hipStream_t stream) {
   unsigned qblocks, kblocks;
-  if (int rc = blocks_of(a.Nq, a.B, a.H, &qblocks)) return rc;
-  if (int rc = blocks_of(a.Nk, a.B, a.Hkv, &kblocks)) return rc;
+  if (int rc = blocks_of(a.Nq, a.B, a.H, a.pack, &qblocks)) return rc;
+  if (int rc = blocks_of(a.Nk, a.B, a.Hkv, 0, &kblocks)) return rc;
   if (a.Nq > 0) {
     if (split_keys(a.Nq, a.Nk, a.B, a.H))
       bwd_q_kernel<T, I, DP, 2><<<dim3(qblocks), 512, 0, stream>>>(a);
@@ -1093,7 +1118,9 @@ bool planned_tiles(const mx_attention_problem* p, bool backward) {
   return p->B > 0 && !ranked_tiles(p) && ceil_div(p->Nq, 128) * p->H > (backward ? 2 : 16) * num_cus();
 }
 
-size_t turns_bytes(int64_t N, int64_t B) { return static_cast<size_t>(tile_turns(N, B, 128)) * sizeof(Turn); }
+// Turns of the queries' and of the keys' tiles.
+int64_t q_turns(const mx_attention_problem* p) { return tile_turns(p->Nq, p->B, 128 >> heads_packed(p)); }
+int64_t k_turns(const mx_attention_problem* p) { return tile_turns(p->Nk, p->B, 128); }
 
 // Each query's lse and delta, up to where turns may begin.
 size_t stats_bytes(const mx_attention_problem* p) {
@@ -1102,7 +1129,7 @@ size_t stats_bytes(const mx_attention_problem* p) {
 
 // The backward's workspace: stats, turns, the shares' sums.
 size_t sums_at(const mx_attention_problem* p) {
-  return stats_bytes(p) + (planned_tiles(p, true) ? turns_bytes(p->Nq, p->B) + turns_bytes(p->Nk, p->B) : 0);
+  return stats_bytes(p) + (planned_tiles(p, true) ? static_cast<size_t>(q_turns(p) + k_turns(p)) * sizeof(Turn) : 0);
 }
 
 int check_workspace(const void* workspace, size_t bytes, size_t need) {
@@ -1120,8 +1147,9 @@ int plan(const mx_attention_problem* p, Turn* turns, bool keys, hipStream_t stre
   a.q_offsets = p->q_offsets, a.k_offsets = p->k_offsets;
   a.B = static_cast<int32_t>(p->B), a.Nq = static_cast<int32_t>(p->Nq), a.Nk = static_cast<int32_t>(p->Nk);
   a.causal = p->causal;
-  a.n[0] = static_cast<int32_t>(tile_turns(p->Nq, p->B, 128));
-  a.n[1] = static_cast<int32_t>(tile_turns(p->Nk, p->B, 128));
+  a.n[0] = static_cast<int32_t>(q_turns(p));
+  a.n[1] = static_cast<int32_t>(k_turns(p));
+  a.shift[0] = kRowShift - heads_packed(p), a.shift[1] = kRowShift;
   a.turns[0] = turns;
   a.turns[1] = turns + a.n[0];
   const dim3 grid(keys ? 2 : 1);
@@ -1138,7 +1166,7 @@ int plan(const mx_attention_problem* p, Turn* turns, bool keys, hipStream_t stre
 extern "C" size_t mx_jagged_attention_forward_workspace_bytes(const mx_attention_problem* p) {
   using namespace mx::attn;
   if (check_problem(p) != MX_OK || p->Nq == 0 || !planned_tiles(p, false)) return 0;
-  return turns_bytes(p->Nq, p->B);
+  return static_cast<size_t>(q_turns(p)) * sizeof(Turn);
 }
 
 extern "C" int mx_jagged_attention_forward(const mx_attention_problem* p, const mx_attention_tensor* q,
@@ -1166,6 +1194,7 @@ extern "C" int mx_jagged_attention_forward(const mx_attention_problem* p, const 
   a.B = static_cast<int32_t>(p->B), a.Nq = static_cast<int32_t>(p->Nq), a.Nk = static_cast<int32_t>(p->Nk);
   a.H = p->H, a.G = p->H / p->Hkv, a.D = p->D;
   a.causal = p->causal, a.scale = p->scale;
+  a.pack = heads_packed(p);
   a.ranked = ranked_tiles(p);
   a.out = out, a.lse = lse;
   const hipStream_t s = mx::as_stream(stream);
@@ -1173,7 +1202,7 @@ extern "C" int mx_jagged_attention_forward(const mx_attention_problem* p, const 
     Turn* turns = static_cast<Turn*>(workspace);
     if (int rc = plan(p, turns, false, s)) return rc;
     a.turns = turns;
-    a.n_turns = static_cast<int32_t>(tile_turns(p->Nq, p->B, 128));
+    a.n_turns = static_cast<int32_t>(q_turns(p));
   }
   return p->dtype == MX_DTYPE_BF16 ? MX_ATTN_DISPATCH(launch_fwd, __bf16, a, p->index_bytes, s)
                                    : MX_ATTN_DISPATCH(launch_fwd, _Float16, a, p->index_bytes, s);
@@ -1223,6 +1252,7 @@ extern "C" int mx_jagged_attention_backward(const mx_attention_problem* p, const
   a.B = static_cast<int32_t>(p->B), a.Nq = static_cast<int32_t>(p->Nq), a.Nk = static_cast<int32_t>(p->Nk);
   a.H = p->H, a.Hkv = p->Hkv, a.G = p->H / p->Hkv, a.D = p->D;
   a.causal = p->causal, a.scale = p->scale;
+  a.pack = heads_packed(p);
   a.ranked = ranked_tiles(p);
   a.lse = lse;
   a.lse2 = static_cast<float*>(workspace);
@@ -1234,8 +1264,8 @@ extern "C" int mx_jagged_attention_backward(const mx_attention_problem* p, const
   if (planned_tiles(p, true)) {
     Turn* turns = reinterpret_cast<Turn*>(static_cast<char*>(workspace) + stats_bytes(p));
     if (int rc = plan(p, turns, dk != nullptr, s)) return rc;
-    a.n_q_turns = static_cast<int32_t>(tile_turns(p->Nq, p->B, 128));
-    a.n_k_turns = static_cast<int32_t>(tile_turns(p->Nk, p->B, 128));
+    a.n_q_turns = static_cast<int32_t>(q_turns(p));
+    a.n_k_turns = static_cast<int32_t>(k_turns(p));
     a.q_turns = turns;
     a.k_turns = turns + a.n_q_turns;
   }
