@@ -210,11 +210,12 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? 2 : WAVES / 
   const char* vb = a.c.v + kvh * a.c.v_head;
 
   // The share: tiles [at, stop) counted from sequence b's first one.
+  const bool shared = WAVES == kStepWaves && a.workers > 0;
   int32_t b = worker, len;
   int64_t at = 0, stop = 0;
-  if (WAVES != kStepWaves || a.workers == 0) {
+  if (!shared) {
     len = __builtin_amdgcn_readfirstlane(tokens_of(a, b));
-    stop = len > 0 ? tiles_of<WAVES>(len) : 1;  // an empty sequence is written too
+    stop = tiles_of<WAVES>(len);  // 0 for an empty one: its one pass writes the zeros
   } else {
     int64_t prior;
     const int64_t total = count_tiles(a, 0, &prior);
@@ -386,7 +387,7 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? 2 : WAVES / 
         }
       }
     }
-    if (stop <= n) return;
+    if (!shared || stop <= n) return;  // a block per sequence never leaves its own
     // The next sequence that has tokens.
     stop -= n;
     at = 0;
