@@ -623,8 +623,8 @@ typedef struct mx_attention_tensor {
 typedef struct mx_attention_problem {
   int32_t dtype;          /* MX_DTYPE_F16 or MX_DTYPE_BF16 */
   int32_t index_bytes;    /* of the offsets: 4 or 8 */
-  const void* q_offsets;  /* [B + 1], non-decreasing */
-  const void* k_offsets;  /* [B + 1] */
+  const void* q_offsets;  /* [B + 1], non-decreasing (one entry where B is 0) */
+  const void* k_offsets;  /* [B + 1]; NULL, as q_offsets, only without lists and rows */
   int64_t B, Nq, Nk;      /* lists, query rows, key rows */
   int32_t H, Hkv, D;
   int32_t causal;

@@ -1094,7 +1094,9 @@ int check_problem(const mx_attention_problem* p) {
   MX_REQUIRE(p->D > 0 && p->D <= MX_ATTENTION_MAX_D && p->D % 8 == 0,
              "head width %d is no multiple of 8 up to %d", p->D, MX_ATTENTION_MAX_D);
   MX_REQUIRE(std::isfinite(p->scale) && p->scale > 0.0f, "scale must be positive and finite");
-  MX_REQUIRE(p->B == 0 || (p->q_offsets != nullptr && p->k_offsets != nullptr), "offsets are null");
+  // Without lists too, rows lie before or after the one entry, which the kernels read.
+  MX_REQUIRE((p->q_offsets != nullptr && p->k_offsets != nullptr) || (p->B == 0 && p->Nq == 0 && p->Nk == 0),
+             "offsets are null");
   return MX_OK;
 }
 
