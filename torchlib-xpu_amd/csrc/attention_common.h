@@ -36,6 +36,7 @@ struct Elem;
 template <>
 struct Elem<__bf16> {
   using x8 = bf16x8;
+  static constexpr bool kNarrow = false;  // the range of fp32
   static __device__ __forceinline__ f32x16 mfma32(x8 a, x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
@@ -47,6 +48,7 @@ struct Elem<__bf16> {
 template <>
 struct Elem<_Float16> {
   using x8 = f16x8;
+  static constexpr bool kNarrow = true;  // up to 65504
   static __device__ __forceinline__ f32x16 mfma32(x8 a, x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }

@@ -227,7 +227,8 @@ __device__ __forceinline__ bool not_finite(const f32x16* acc) {
 // sees.  The matrix product of a tile that a query sees in part multiplies the
 // values it does not see by 0, and 0 times an infinity or NaN is NaN: a wave
 // that ends with such an output takes this way, so that what a masked value
-// holds never shows.  (Values of finite inputs never come here.)
+// holds never shows.  (Finite inputs never come here, in the backward as long as
+// scores stay below 2^30: an fp32 lse no longer tells probabilities apart there.)
 template <typename T, int DP, typename X8>
 __device__ __forceinline__ void rows_key_by_key(const X8* qf, const char* kp, int64_t k_row,
                                                 const char* vp, int64_t v_row, int D, float c2,
@@ -458,6 +459,39 @@ __global__ void __launch_bounds__(kRowWaves * NS * 64, 2) fwd_kernel(const FwdAr
 // in both, seven products where five would do, which is less than what summing
 // dQ over key tiles through memory costs.
 
+// dS goes into a matrix product in the input type, and fp16 ends at 65504, which
+// finite gradients' dS can pass (dO of 5e3 and v of 4 in 128 columns give dP of
+// 2e5; scale, and small q and k, may bring the gradients back into range).  So for
+// fp16 a column (a query of the first launch, a key of the second) of 32 rows of dS
+// is looked at before its rounding, and where one passes the range the column's
+// dS is multiplied from there on by a power of two that brings it below 2^15, and
+// what has been summed of it by the same: exact, until the caller divides the sums
+// by it.  Such a factor f leaves dS with 11 bits down to 2^-14 / f, which is 2^-28
+// of the column's largest or less.  It waits in LDS (`mine`, of this lane): in the
+// ordinary case, fitted == false, only the maxima of |dS| and a vote are spent (4
+// lists of 4096, 16 heads of 128 over 4, fp16: backward 1024 -> 1040 us; 64 of 0 to
+// 1000, 8 of 64 over 2: 184 -> 189; one of 1024, 8 of 128: 65, and 73 where columns
+// need factors).
+// Returns whether the wave's columns have factors.
+template <int DB>
+__device__ __forceinline__ bool fit_range(f32x16& ds, f32x16* acc, float* mine, bool fitted) {
+  float top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(ds[i]));
+  if (__builtin_expect(!fitted && !__any(top > 65504.0f), 1)) return false;
+  const float before = fitted ? *mine : 1.0f;
+  float f = before;
+  top = fmaxf(top, other_half(top));  // the column's other 16 rows
+  // An infinity is one of the inputs' and stays one.
+  if (top * f > 65504.0f && top < INFINITY) f = __builtin_ldexpf(1.0f, 15 - __builtin_amdgcn_frexp_expf(top));
+  const float r = f / before;
+#pragma unroll
+  for (int d = 0; d < DB; ++d) acc[d] *= r;
+  ds *= f;
+  *mine = f;
+  return true;
+}
+
 struct BwdArgs {
   const char *q, *k, *v, *out, *grad;  // bytes; out and grad with q's shape
   uint32_t q_row, k_row, v_row, o_row, g_row;
@@ -492,7 +526,7 @@ __global__ void __launch_bounds__(kRowWaves * NS * 64, DP <= 64 ? 4 : NS == 1 &&
   using Ti = Tile<DP>;
   constexpr int KS = DP / 16, DB = DP / 32;
   constexpr int kTileBytes = kBN * DP * 2;
-  __shared__ __attribute__((aligned(1024))) char lds[NS * 4 * kTileBytes];
+  __shared__ __attribute__((aligned(1024))) char lds[NS * 4 * kTileBytes + (E::kNarrow ? kRowWaves * NS * 64 * 4 : 0)];
 
   int head;
   int turn;
@@ -563,6 +597,8 @@ __global__ void __launch_bounds__(kRowWaves * NS * 64, DP <= 64 ? 4 : NS == 1 &&
   f32x16 dq[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) dq[d] = f32x16{};
+  bool fitted = false;  // fit_range, and where this lane's factor is
+  auto factor = [&] { return reinterpret_cast<float*>(lds + NS * 4 * kTileBytes) + wave * 64 + lane_again(); };
   const float c2 = a.scale * kLog2e;
   const Places<DP> at(lane, 0);
 
@@ -625,6 +661,7 @@ __global__ void __launch_bounds__(kRowWaves * NS * 64, DP <= 64 ? 4 : NS == 1 &&
         for (int i = 0; i < 16; ++i)
           if (8 * (i / 4) + i % 4 >= last) s[i] = 0.0f;
       }
+      if constexpr (E::kNarrow) fitted = fit_range<DB>(s, dq, factor(), fitted);
       X8 ds[2];
 #pragma unroll
       for (int i = 0; i < 16; ++i) ds[i / 8][i % 8] = static_cast<T>(s[i]);
@@ -645,9 +682,14 @@ __global__ void __launch_bounds__(kRowWaves * NS * 64, DP <= 64 ? 4 : NS == 1 &&
     wait_and_barrier<0>();
     work(j, mine_lds, (t & 1) * 2 * kTileBytes, mine_lds + ((t + 1) & 1) * 2 * kTileBytes);
   }
+  if (E::kNarrow && fitted) {
+    const float inv = 1.0f / *factor();
+#pragma unroll
+    for (int d = 0; d < DB; ++d) dq[d] *= inv;
+  }
 
   if constexpr (NS == 2) {
-    static_assert(sizeof(lds) >= kRowWaves * 64 * 16 * DB * 4, "the join's room");
+    static_assert(NS * 4 * kTileBytes >= kRowWaves * 64 * 16 * DB * 4, "the join's room");
     float* room = reinterpret_cast<float*>(lds) + wave % kRowWaves * 64 * 16 * DB + lane;
     wait_and_barrier<0>();
     if (group == 1) {
@@ -705,7 +747,8 @@ __global__ void __launch_bounds__(kRowWaves * NQ * 64, 2) bwd_kv_kernel(const Bw
   // 4096, 16 heads of 128: backward 1047 -> 1021 us).
   constexpr bool kKeep = DP == 128 && NQ == 2;
   constexpr int kInRegs = kKeep ? KS - 1 : KS;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * kBuf + (kKeep ? THREADS * 16 : 0)];
+  constexpr int kFactors = 2 * kBuf + (kKeep ? THREADS * 16 : 0);
+  __shared__ __attribute__((aligned(1024))) char lds[kFactors + (E::kNarrow ? THREADS * 4 : 0)];
   static_assert(NQ == 1 || 2 * kBuf >= BM * DP * 4, "the join's room");
 
   int kvh;
@@ -755,6 +798,8 @@ __global__ void __launch_bounds__(kRowWaves * NQ * 64, 2) bwd_kv_kernel(const Bw
   f32x16 dk[DB], dv[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) dk[d] = dv[d] = f32x16{};
+  bool fitted = false;  // fit_range, and where this lane's factor is
+  auto factor = [&] { return reinterpret_cast<float*>(lds + kFactors) + wave * 64 + lane_again(); };
   const float c2 = a.scale * kLog2e;
   const Places<DP> at(lane, 64 * part);
 
@@ -835,6 +880,7 @@ __global__ void __launch_bounds__(kRowWaves * NQ * 64, 2) bwd_kv_kernel(const Bw
         for (int i = 0; i < 16; ++i)
           if (8 * (i / 4) + i % 4 < from) dp[i] = 0.0f;
       }
+      if constexpr (E::kNarrow) fitted = fit_range<DB>(dp, dk, factor(), fitted);
       X8 ds[2];
 #pragma unroll
       for (int i = 0; i < 16; ++i) ds[i / 8][i % 8] = static_cast<T>(dp[i]);
@@ -860,6 +906,11 @@ __global__ void __launch_bounds__(kRowWaves * NQ * 64, 2) bwd_kv_kernel(const Bw
       t = tn;
       g = gn;
     }
+  }
+  if (E::kNarrow && fitted) {
+    const float inv = 1.0f / *factor();
+#pragma unroll
+    for (int d = 0; d < DB; ++d) dk[d] *= inv;
   }
 
   if constexpr (NQ == 2) {
