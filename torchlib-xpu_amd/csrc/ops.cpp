@@ -2192,6 +2192,18 @@ void paged_cache_append(const Tensor& k, const Tensor& v, const Tensor& offsets,
                                 starts.data_ptr(), index_bytes_of(starts, "starts"), stream_of(k)));
 }
 
+// The append as autograd sees it: the caches' versions move on, so that a backward
+// that has saved one of them notices.
+void paged_cache_append_inplace(const Tensor& k, const Tensor& v, const Tensor& offsets, const Tensor& starts,
+                                const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table) {
+  {
+    at::AutoDispatchBelowADInplaceOrView g;
+    paged_cache_append(k, v, offsets, starts, k_cache, v_cache, page_table);
+  }
+  for (const Tensor* t : {&k_cache, &v_cache})
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();  // (inference tensors keep none)
+}
+
 Tensor paged_cache_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache,
                              const Tensor& page_table, const Tensor& lengths,
                              std::optional<double> scale) {
@@ -2486,6 +2498,10 @@ TORCH_LIBRARY_IMPL(mx_fbgemm, CUDA, m) {
   m.impl("jagged_attention_backward", TORCH_FN(mx_ops::jagged_attention_backward));
   m.impl("paged_cache_append", TORCH_FN(mx_ops::paged_cache_append));
   m.impl("paged_cache_attention", TORCH_FN(mx_ops::paged_cache_attention));
+}
+
+TORCH_LIBRARY_IMPL(mx_fbgemm, ADInplaceOrView, m) {
+  m.impl("paged_cache_append", TORCH_FN(mx_ops::paged_cache_append_inplace));
 }
 
 TORCH_LIBRARY_IMPL(mx_fbgemm, Autograd, m) {
