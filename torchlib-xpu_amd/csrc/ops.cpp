@@ -14,6 +14,7 @@
 // are registered: CPU tensors raise the dispatcher's NotImplementedError.
 #include <ATen/ATen.h>
 #include <ATen/hip/HIPGeneratorImpl.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -2129,6 +2130,10 @@ class JaggedAttention : public torch::autograd::Function<JaggedAttention> {
 Tensor jagged_attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v,
                                  const Tensor& q_offsets, const std::optional<Tensor>& k_offsets,
                                  bool causal, std::optional<double> scale) {
+  // Below, a tangent would be dropped without a word.
+  TORCH_CHECK_NOT_IMPLEMENTED(!c10::AutogradState::get_tls_state().get_fw_grad_mode() ||
+                                  !(q._fw_grad(0).defined() || k._fw_grad(0).defined() || v._fw_grad(0).defined()),
+                              "jagged_attention has no forward-mode derivative");
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
     return JaggedAttention::apply(q, k, v, q_offsets, k_offsets, causal, scale);
   at::AutoDispatchBelowADInplaceOrView g;
