@@ -23,7 +23,10 @@ class PagedSequenceCache:
     ([pages, page_size, heads, head_dim] fp16 or bf16, the heads' widths a
     multiple of 8 up to 128).
 
-    The host keeps lengths and free pages, so no call waits for the device.
+    The host keeps lengths and free pages, and what it tells the device goes through
+    pinned memory, so no call waits for the device.  Nor can a call be captured in
+    a graph, as its numbers are the host's: ``paged_cache_append`` and
+    ``paged_cache_attention`` with numbers on the device can.
     Sequences are named by the number ``add`` gives; calls take any of them in
     any order, each at most once."""
 
@@ -83,6 +86,7 @@ class PagedSequenceCache:
         self._distinct(sequences)
         if not sequences:
             return
+        self._not_captured()
         starts = [self._lengths[s] for s in sequences]
         self._reserve(sequences, [a + n for a, n in zip(starts, counts)])
         # Offsets and starts in one copy to the device.
@@ -101,6 +105,7 @@ class PagedSequenceCache:
         self._distinct(sequences)
         if q.size(0) != len(sequences):
             raise ValueError(f"q has {q.size(0)} rows for {len(sequences)} sequences")
+        self._not_captured()
         lengths = self._to_device([self._lengths[s] for s in sequences])
         return torch.ops.mx_fbgemm.paged_cache_attention(q, self.k, self.v, self._rows(sequences),
                                                          lengths, scale)
@@ -118,8 +123,18 @@ class PagedSequenceCache:
         if len(set(sequences)) != len(sequences):
             raise ValueError("a sequence is named twice")
 
+    def _not_captured(self) -> None:
+        """A replay would copy from pinned memory that holds other numbers by then."""
+        if self._table.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("PagedSequenceCache's calls cannot be captured in a graph")
+
     def _to_device(self, numbers: list[int]) -> torch.Tensor:
-        return torch.tensor(numbers, dtype=torch.int32).to(self._table.device)
+        """The numbers on the device, enqueued: from pinned memory, which torch's host
+        allocator keeps until the copy has run (one from pageable memory would wait
+        for all work of the stream)."""
+        device = self._table.device
+        pinned = device.type == "cuda"
+        return torch.tensor(numbers, dtype=torch.int32, pin_memory=pinned).to(device, non_blocking=pinned)
 
     def _rows(self, sequences: Sequence[int]) -> torch.Tensor:
         """The table's rows of the sequences, as wide as their longest."""
