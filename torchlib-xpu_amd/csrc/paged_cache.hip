@@ -504,8 +504,12 @@ __global__ void __launch_bounds__(kJoinMost * 64) join_kernel(const StepArgs a) 
 //   of up to 1024 70.3 -> 70.9; 8 heads of 128: 64 of up to 512 29.6 -> 25.4, 200
 //   57.7 -> 63.4).
 // - A block of four waves per sequence and head where these are enough to even
-//   out by themselves (1024 of up to 200 tokens, 8 x 64: 71, in shares 108; 256 of
-//   up to 2000, 8 x 128: 219, in shares 205) or no sequence has two tiles.
+//   out by themselves, or no sequence has two tiles.  The host knows no lengths, and
+//   lengths decide: this way gains where they are alike or short (1024 of up to 200
+//   tokens, 8 x 64: 72, in shares 110; 256 of 8192, 8 x 64: 903, in shares 1000; 512
+//   of 1 to 1000 by their logarithm, 4 x 64: 38, in shares 41) and loses where few are
+//   long (256 of up to 2000, 8 x 128: 211, in shares 201; by their logarithm 90, in
+//   shares 70; up to 8192 by their logarithm 298, in shares 184).
 struct Plan {
   int32_t workers;  // 0: a block per sequence and head
   bool wide;
