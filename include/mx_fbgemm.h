@@ -690,6 +690,63 @@ int mx_paged_cache_attention(const mx_paged_cache* cache, int32_t dtype,
                              int32_t D, const void* lengths, int32_t lengths_bytes, float scale,
                              void* out, void* workspace, size_t workspace_bytes, void* stream);
 
+/* A 4-bit cache (`bits` 4 below) has, for a head's D values, a row of D / 2 + 4
+ * bytes: codes 0..15, the even element in the low half of a byte, then scale and
+ * bias in fp16; value = scale * code + bias.  A head's row is quantized as
+ * mx_quantize_fused_nbit_rowwise does it: bias the row's smallest value in fp16, scale
+ * (largest - bias) / 15 in fp16 (1 where that is 0), codes rounded to nearest.
+ * mx_paged_cache's strides count bytes then (multiples of 4), and k and v are
+ * 4-byte aligned. */
+
+/* Angles of the positions: table is fp32 [positions, pairs, 2] (cosine, sine),
+ * 16-byte aligned.  A head's first 2 * pairs values turn (pairs a multiple of 4),
+ * in pairs (i, i + pairs), or (2 i, 2 i + 1) where interleaved:
+ * (x1, x2) -> (x1 c - x2 s, x2 c + x1 s), each operation rounded to fp32. */
+typedef struct mx_rotary {
+  const float* table;
+  int64_t positions;
+  int32_t pairs;
+  int32_t interleaved;
+} mx_rotary;
+
+/* Rotates the heads of x (strided [N, H, D]): row offsets[b] + i is at position
+ * starts[b] + i (starts NULL: i); with `inverse` by the negative angles (the
+ * gradient).  out: contiguous [N, H, D].  A row of no list gives zeros; of a row whose
+ * position has no entry in the table, the values that would turn are NaN. */
+int mx_jagged_rotary(int32_t dtype, const mx_attention_tensor* x, int64_t N, int32_t H, int32_t D,
+                     const mx_rotary* rotary, int32_t inverse, int64_t B, const void* offsets,
+                     int32_t offsets_bytes, const void* starts, int32_t starts_bytes, void* out,
+                     void* stream);
+
+/* mx_paged_cache_append into a cache of 16 or 4 bits, with the keys rotated on
+ * the way (rotary may be NULL: they are not), and the queries of the same rows
+ * (strided [N, H, D], H 0: none) rotated into q_out, contiguous, as
+ * mx_jagged_rotary does.  A token whose position has no entry in the table is
+ * dropped. */
+int mx_paged_cache_append_rows(const mx_paged_cache* cache, int32_t bits, int32_t dtype, int32_t H,
+                               int32_t Hkv, int32_t D, const mx_attention_tensor* q,
+                               const mx_attention_tensor* k, const mx_attention_tensor* v,
+                               const mx_rotary* rotary, int64_t N, int64_t B, const void* offsets,
+                               int32_t offsets_bytes, const void* starts, int32_t starts_bytes,
+                               void* q_out, void* stream);
+
+/* mx_paged_cache_attention over a 4-bit cache; dtype is that of q and out. */
+size_t mx_paged_cache_attention_int4_workspace_bytes(const mx_paged_cache* cache, int64_t B,
+                                                     int32_t H, int32_t Hkv, int32_t D);
+int mx_paged_cache_attention_int4(const mx_paged_cache* cache, int32_t dtype,
+                                  const mx_attention_tensor* q, int64_t B, int32_t H, int32_t Hkv,
+                                  int32_t D, const void* lengths, int32_t lengths_bytes,
+                                  float scale, void* out, void* workspace, size_t workspace_bytes,
+                                  void* stream);
+
+/* The tokens of lists out of a cache of 16 or 4 bits, packed: row offsets[b] + i
+ * of k_out and v_out (contiguous [N, Hkv, D] of dtype; with 16 bits the cache's)
+ * is token i of sequence b.  Rows of no list, and tokens without a page, give
+ * zeros. */
+int mx_paged_cache_gather(const mx_paged_cache* cache, int32_t bits, int32_t dtype, int32_t Hkv,
+                          int32_t D, int64_t N, int64_t B, const void* offsets,
+                          int32_t offsets_bytes, void* k_out, void* v_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

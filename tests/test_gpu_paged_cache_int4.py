@@ -1,0 +1,217 @@
+"""Attention of one token per sequence over a cache of 4-bit rows, against its
+float64 definition."""
+
+import numpy as np
+import pytest
+import torch
+
+from attention_helpers import check
+from rows_helpers import attention4, make, page_table, rows4
+
+pytestmark = pytest.mark.gpu
+
+OPS = torch.ops.mx_fbgemm
+
+
+def make_cache(lengths, page, Hkv, D, seed=0, fill=None, width=None, values=None):
+    """Sequences' rows laid into pages in a random order.  Slots and pages of no token
+    hold random bytes, their scale and bias `fill`."""
+    table, pages = page_table(lengths, page, seed, width=width)
+    g = torch.Generator().manual_seed(seed)
+    caches, lists = [], []
+    for which in range(2):
+        c = torch.randint(0, 256, (pages, page, Hkv, D // 2 + 4), generator=g, dtype=torch.uint8)
+        if fill is not None:
+            c[..., -4:] = torch.full((2,), fill, dtype=torch.float16).view(torch.uint8)
+        rows = []
+        for b, n in enumerate(lengths):
+            x = values(which, b, n) if values else make((n, Hkv, D), torch.float32, seed + 2 * b + which + 1)
+            r = rows4(x) if n else torch.zeros((0, Hkv, D // 2 + 4), dtype=torch.uint8)
+            rows.append(r)
+            t = torch.arange(n)
+            c[table[b, t // page].long(), t % page] = r
+        caches.append(c), lists.append(rows)
+    return caches[0], caches[1], table, lists[0], lists[1]
+
+
+def run(dev, lengths, page, H, Hkv, D, dtype, index=torch.int32, scale=None, q=None, **kw):
+    print(f"[case] {len(lengths)} lists up to {max(lengths)} page={page} H={H}/{Hkv} D={D} {dtype}", flush=True)
+    kc, vc, table, ks, vs = make_cache(lengths, page, Hkv, D, **kw)
+    if q is None:
+        q = make((len(lengths), H, D), dtype, 99)
+    out = OPS.paged_cache_attention(q.to(dev), kc.to(dev), vc.to(dev), table.to(dev),
+                                    torch.tensor(lengths, device=dev, dtype=index), scale)
+    want, tol = attention4(q.double().numpy(), ks, vs, scale if scale is not None else D ** -0.5, dtype)
+    check(out.double().cpu().numpy(), want, tol, "out")
+    return out
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("D", [8, 16, 24, 32, 40, 48, 64, 72, 80, 96, 104, 120, 128])
+def test_widths(dev, dtype, D):
+    run(dev, [1, 0, 31, 32, 33, 200], 16, 4, 2, D, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("D", [8, 24, 32, 40, 64, 72, 96, 104, 128])
+def test_widths_in_shares(dev, dtype, D):
+    """More tokens than two wide blocks' tiles: sequences cut anywhere and joined."""
+    run(dev, [1, 0, 31, 1300, 33, 129], 16, 4, 2, D, dtype)
+
+
+@pytest.mark.parametrize("page", [1, 3, 8, 16, 33, 64, 100, 256])
+def test_page_sizes(dev, page):
+    run(dev, [1, 97, 300, 128], page, 4, 4, 64, "bfloat16", torch.int64)
+
+
+@pytest.mark.parametrize("H,Hkv", [(1, 1), (2, 1), (16, 1), (17, 1), (40, 2), (24, 8)])
+def test_grouped_heads(dev, H, Hkv):
+    run(dev, [65, 5], 16, H, Hkv, 32, "float16", scale=0.3)
+
+
+@pytest.mark.parametrize("B", [1, 3, 300])
+def test_long_and_ragged(dev, B):
+    rng = np.random.default_rng(B)
+    lengths = [int(x) for x in rng.integers(0, 120, B)]
+    lengths[0] = 5000 if B < 300 else 700
+    run(dev, lengths, 16, 2, 1, 64, "bfloat16")
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("room", [128, 144, 512, 528, 1024, 1040, 4096])
+def test_room_in_the_table(dev, D, room):
+    """The table's width decides how sequences are cut, not what comes out."""
+    run(dev, [room - 1, 100, room // 2], 16, 6, 2, D, "float16")
+
+
+@pytest.mark.parametrize("lengths", [[5, 50, 17], [5, 1490, 0, 17]])
+@pytest.mark.parametrize("fill", [0.0, float("nan"), float("inf"), -float("inf")])
+def test_what_slots_without_tokens_hold(dev, fill, lengths):
+    run(dev, lengths, 100, 4, 2, 128, "bfloat16", fill=fill)
+    run(dev, lengths, 100, 4, 2, 128, "float16", fill=fill)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_rows_far_from_zero(dev, dtype):
+    """Biases that outweigh the codes, constant rows, small and large scales."""
+    def values(which, b, n):
+        x = make((n, 2, 64), torch.float32, 7 * b + which)
+        return [x * 0.01 + 20.0, x * 0 + 3.0, x * 1e-4, x * 50][b]
+    run(dev, [70, 40, 300, 33], 16, 4, 2, 64, dtype, values=values)
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e-6, 300.0, 3e4])
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_sizes_of_queries(dev, dtype, size):
+    """Queries far from order one; large ones make one token win."""
+    q = (make((3, 4, 64), torch.float32, 5) * size).clamp(-65000, 65000).to(getattr(torch, dtype))
+    run(dev, [70, 40, 300], 16, 4, 2, 64, dtype, q=q, scale=1.0 / max(size, 1e-6) if size > 1 else None)
+
+
+def test_one_head_of_many_lists(dev):
+    run(dev, [i % 130 for i in range(2100)], 16, 2, 1, 32, "bfloat16")
+
+
+def test_lengths_past_the_table_and_below_zero(dev):
+    kc, vc, table, ks, vs = make_cache([32, 32, 20], 16, 1, 32)
+    q = make((3, 2, 32), "float16", 1).to(dev)
+    args = (q, kc.to(dev), vc.to(dev), table.to(dev))
+    want = OPS.paged_cache_attention(*args, torch.tensor([32, 32, 0], device=dev))
+    got = OPS.paged_cache_attention(*args, torch.tensor([1000, 32, -7], device=dev))
+    assert torch.equal(got, want) and torch.count_nonzero(got[2]) == 0
+
+
+def test_bad_table_entries_are_absent_tokens(dev):
+    kc, vc, table, ks, vs = make_cache([48, 48], 16, 1, 32)
+    q = make((2, 2, 32), "float16", 1)
+    lengths = torch.tensor([48, 48], device=dev)
+    for bad in (-1, kc.size(0), 2 ** 31 - 1, -2 ** 31):
+        t = table.clone()
+        t[0, 1] = bad
+        t[1] = bad
+        out = OPS.paged_cache_attention(q.to(dev), kc.to(dev), vc.to(dev), t.to(dev), lengths)
+        keep = [*range(16), *range(32, 48)]
+        want, tol = attention4(q[:1].double().numpy(), [ks[0][keep]], [vs[0][keep]], 32 ** -0.5, "float16")
+        check(out[:1].double().cpu().numpy(), want, tol, "out")
+        assert torch.count_nonzero(out[1]) == 0
+
+
+@pytest.mark.parametrize("D", [32, 64, 72, 128])
+def test_strided_caches(dev, D):
+    """Keys and values interleaved in one buffer, heads before slots, rows at any
+    multiple of 4 bytes, tables and queries that are views: the same bits."""
+    lengths = [70, 9]
+    kc, vc, table, ks, vs = make_cache(lengths, 16, 2, D)
+    q = make((2, 8, D), "bfloat16", 5).to(dev)
+    n = torch.tensor(lengths, device=dev)
+    table, kd, vd = table.to(dev), kc.to(dev), vc.to(dev)
+    want = OPS.paged_cache_attention(q, kd, vd, table, n)
+    both = torch.stack([kd, vd], 1)
+    assert torch.equal(OPS.paged_cache_attention(q, both[:, 0], both[:, 1], table, n), want)
+    hk, hv = (x.transpose(1, 2).contiguous().transpose(1, 2) for x in (kd, vd))
+    assert torch.equal(OPS.paged_cache_attention(q, hk, hv, table, n), want)
+    row = kd.size(3)
+    for pad in (4, 12, 16):
+        wk, wv = (torch.full((*x.shape[:3], row + pad), 255, dtype=torch.uint8, device=dev) for x in (kd, vd))
+        wk[..., pad:], wv[..., :row] = kd, vd
+        assert torch.equal(OPS.paged_cache_attention(q, wk[..., pad:], wv[..., :row], table, n), want)
+    wide = torch.zeros((2, 5), dtype=torch.int32, device=dev)
+    wide[:, : table.size(1)] = table
+    assert torch.equal(OPS.paged_cache_attention(q, kd, vd, torch.cat([wide, wide], 1)[:, :5], n), want)
+    qt = q.transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(OPS.paged_cache_attention(qt, kd, vd, table, n), want)
+
+
+def test_the_cache_ends_with_its_last_row(dev):
+    """Rows at the very end of an allocation: nothing behind them is read into a
+    result (the bytes behind are all ones, a NaN in scale and bias)."""
+    for D in (8, 40, 72, 128):
+        kc, vc, table, ks, vs = make_cache([16], 16, 1, D, width=1)
+        row = D // 2 + 4
+        pool = torch.full((kc.numel() + 4096,), 255, dtype=torch.uint8, device=dev)
+        pool[: kc.numel()] = kc.reshape(-1).to(dev)
+        view = pool[: kc.numel()].view(kc.shape)
+        last = torch.tensor([[kc.size(0) - 1]], dtype=torch.int32, device=dev)
+        view[-1] = kc[int(table[0, 0])].to(dev)
+        q = make((1, 2, D), "bfloat16", 3)
+        out = OPS.paged_cache_attention(q.to(dev), view, vc.to(dev)[int(table[0, 0])].expand(kc.shape).contiguous(), last,
+                                        torch.tensor([16], device=dev))
+        want, tol = attention4(q.double().numpy(), ks, vs, D ** -0.5, "bfloat16")
+        check(out.double().cpu().numpy(), want, tol, f"out D={D} row={row}")
+
+
+def test_the_same_bits_every_time(dev):
+    kc, vc, table, ks, vs = make_cache([3000, 17, 900], 16, 2, 64)
+    q = make((3, 4, 64), "float16", 1).to(dev)
+    args = (q, kc.to(dev), vc.to(dev), table.to(dev), torch.tensor([3000, 17, 900], device=dev))
+    want = OPS.paged_cache_attention(*args)
+    for _ in range(5):
+        assert torch.equal(OPS.paged_cache_attention(*args), want)
+
+
+def test_empty(dev):
+    kc = torch.zeros((0, 16, 2, 20), dtype=torch.uint8, device=dev)
+    q = make((2, 2, 32), "float16", 0).to(dev)
+    n = torch.tensor([5, 5], device=dev)
+    for W in (0, 3):
+        table = torch.zeros((2, W), dtype=torch.int32, device=dev)
+        assert torch.count_nonzero(OPS.paged_cache_attention(q, kc, kc, table, n)) == 0
+    kc = torch.zeros((2, 16, 2, 20), dtype=torch.uint8, device=dev)
+    table = torch.zeros((0, 1), dtype=torch.int32, device=dev)
+    assert OPS.paged_cache_attention(q[:0], kc, kc, table, n[:0]).shape == (0, 2, 32)
+
+
+def test_refusals(dev):
+    kc = torch.zeros((2, 16, 2, 20), dtype=torch.uint8, device=dev)  # D 32
+    q = torch.zeros((3, 4, 32), dtype=torch.float16, device=dev)
+    table = torch.zeros((3, 1), dtype=torch.int32, device=dev)
+    n = torch.ones(3, dtype=torch.int64, device=dev)
+    h = torch.zeros((2, 16, 2, 32), dtype=torch.float16, device=dev)
+    big = torch.zeros((2, 16, 2, 72), dtype=torch.uint8, device=dev)
+    for args in [(q.float(), kc, kc, table, n), (q[:, :3], kc, kc, table, n), (q[:, :, :16], kc, kc, table, n),
+                 (q, kc[..., :18], kc[..., :18], table, n), (q, kc, kc[:1], table, n), (q, kc, h, table, n),
+                 (q, kc[..., :4], kc[..., :4], table, n), (q, big, big, table, n), (q, kc.char(), kc.char(), table, n),
+                 (q, kc.transpose(2, 3), kc.transpose(2, 3), table, n), (q, kc.cpu(), kc, table, n),
+                 (q, kc, kc, table, n, 0.0), (q, kc, kc, table, n.float()), (q, kc[0], kc[0], table, n)]:
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            OPS.paged_cache_attention(*args)

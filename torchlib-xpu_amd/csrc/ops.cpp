@@ -2140,26 +2140,41 @@ Tensor jagged_attention_autograd(const Tensor& q, const Tensor& k, const Tensor&
   return jagged_attention_plain(q, k, v, q_offsets, k_offsets, causal, scale);
 }
 
-mx_paged_cache pack_cache(const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table) {
+// A cache as the kernels take it: [pages, page_size, heads, D] of 16-bit values, or
+// [pages, page_size, heads, D / 2 + 4] bytes, rows of 4 bits.
+struct CacheCall {
+  mx_paged_cache c{};
+  int32_t bits = 16;
+  int64_t heads = 0, D = 0;
+};
+
+CacheCall pack_cache(const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table) {
   check_gpu(k_cache, "k_cache");
   check_arg(v_cache, k_cache, "v_cache", false);
   check_arg(page_table, k_cache, "page_table", false);
-  attention_dtype(k_cache, "k_cache");
+  CacheCall r;
+  if (k_cache.scalar_type() == at::kByte) r.bits = 4;
+  else TORCH_CHECK(k_cache.scalar_type() == at::kHalf || k_cache.scalar_type() == at::kBFloat16,
+                   "k_cache must be float16, bfloat16 or uint8 (rows of 4 bits), got ", k_cache.scalar_type());
   TORCH_CHECK(k_cache.dim() == 4, "k_cache must be [pages, page_size, heads, D], got ", k_cache.sizes());
   TORCH_CHECK(k_cache.sizes() == v_cache.sizes() && k_cache.scalar_type() == v_cache.scalar_type(),
               "k_cache and v_cache must have one shape and type");
-  check_head_width(k_cache.size(3));
+  r.heads = k_cache.size(2);
+  r.D = r.bits == 16 ? k_cache.size(3) : 2 * (k_cache.size(3) - 4);
+  check_head_width(r.D);
   TORCH_CHECK(k_cache.size(1) >= 1 && k_cache.size(1) < (1ll << 31) && k_cache.size(2) >= 1,
               "page_size and heads must be positive, got ", k_cache.sizes());
+  const int64_t step = r.bits == 16 ? 8 : 4;  // elements
+  const uintptr_t align = r.bits == 16 ? 16 : 4;
   for (const Tensor* t : {&k_cache, &v_cache})
-    TORCH_CHECK(t->stride(3) == 1 && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0 &&
-                    t->stride(0) % 8 == 0 && t->stride(1) % 8 == 0 && t->stride(2) % 8 == 0,
-                "the caches' rows must be contiguous and start at multiples of 16 bytes, got strides ",
+    TORCH_CHECK(t->stride(3) == 1 && reinterpret_cast<uintptr_t>(t->data_ptr()) % align == 0 &&
+                    t->stride(0) % step == 0 && t->stride(1) % step == 0 && t->stride(2) % step == 0,
+                "the caches' rows must be contiguous and start at multiples of ", align, " bytes, got strides ",
                 t->strides());
   TORCH_CHECK(page_table.scalar_type() == at::kInt && page_table.dim() == 2 &&
                   (page_table.size(1) <= 1 || page_table.stride(1) == 1),
               "page_table must be int32 [sequences, pages of a sequence] with contiguous rows");
-  mx_paged_cache c{};
+  mx_paged_cache& c = r.c;
   c.k = k_cache.data_ptr();
   c.v = v_cache.data_ptr();
   c.k_page_stride = k_cache.stride(0), c.k_slot_stride = k_cache.stride(1), c.k_head_stride = k_cache.stride(2);
@@ -2169,7 +2184,32 @@ mx_paged_cache pack_cache(const Tensor& k_cache, const Tensor& v_cache, const Te
   c.table = page_table.data_ptr<int32_t>();
   c.table_row_stride = page_table.stride(0);
   c.table_width = page_table.size(1);
-  return c;
+  return r;
+}
+
+// Rows that go into a cache or attend to it: of its type, or of either 16-bit type
+// over rows of 4 bits.
+void check_cache_rows(const Tensor& t, const Tensor& like, const CacheCall& c, const char* name) {
+  if (c.bits == 4) attention_dtype(like, name);
+  check_rows(t, like, name);
+}
+
+// Offsets and starts of the lists that a page table has.
+void check_lists(const Tensor& offsets, const Tensor& starts, const Tensor& like, int64_t B) {
+  check_arg(offsets, like, "offsets", true);
+  check_arg(starts, like, "starts", true);
+  TORCH_CHECK(offsets.dim() == 1 && offsets.numel() == B + 1, "offsets must have ", B + 1, " entries, got ",
+              offsets.sizes());
+  TORCH_CHECK(starts.dim() == 1 && starts.numel() == B, "starts must have ", B, " entries, got ", starts.sizes());
+}
+
+void check_appended(const Tensor& k, const Tensor& v, const Tensor& k_cache, const CacheCall& c) {
+  const Tensor& like = c.bits == 16 ? k_cache : k;
+  check_cache_rows(k, like, c, "k");
+  check_cache_rows(v, like, c, "v");
+  TORCH_CHECK(k.sizes() == v.sizes(), "k ", k.sizes(), " and v ", v.sizes(), " must have one shape");
+  TORCH_CHECK(k.size(1) == c.heads && k.size(2) == c.D, "k is ", k.sizes(), " but the cache holds ", c.heads,
+              " heads of ", c.D);
 }
 
 void paged_cache_append(const Tensor& k, const Tensor& v, const Tensor& offsets, const Tensor& starts,
@@ -2177,36 +2217,189 @@ void paged_cache_append(const Tensor& k, const Tensor& v, const Tensor& offsets,
   check_gpu(k, "k");
   c10::OptionalDeviceGuard guard(k.device());
   check_arg(k_cache, k, "k_cache", false);
-  const mx_paged_cache c = pack_cache(k_cache, v_cache, page_table);
-  check_rows(k, k_cache, "k");
-  check_rows(v, k_cache, "v");
-  TORCH_CHECK(k.sizes() == v.sizes(), "k ", k.sizes(), " and v ", v.sizes(), " must have one shape");
-  TORCH_CHECK(k.size(1) == k_cache.size(2) && k.size(2) == k_cache.size(3), "k is ", k.sizes(),
-              " but the cache holds ", k_cache.size(2), " heads of ", k_cache.size(3));
-  check_arg(offsets, k, "offsets", true);
-  check_arg(starts, k, "starts", true);
+  const CacheCall c = pack_cache(k_cache, v_cache, page_table);
+  check_appended(k, v, k_cache, c);
   const int64_t B = page_table.size(0);
-  TORCH_CHECK(offsets.dim() == 1 && offsets.numel() == B + 1, "offsets must have ", B + 1, " entries, got ",
-              offsets.sizes());
-  TORCH_CHECK(starts.dim() == 1 && starts.numel() == B, "starts must have ", B, " entries, got ", starts.sizes());
+  check_lists(offsets, starts, k, B);
   Tensor kk, kv;
   const mx_attention_tensor ko = attention_operand(k, kk), vo = attention_operand(v, kv);
-  MX_CALL(mx_paged_cache_append(&c, mx_dtype_of(k.scalar_type()), static_cast<int32_t>(k.size(1)),
-                                static_cast<int32_t>(k.size(2)), &ko, &vo, k.size(0), B,
-                                offsets.data_ptr(), index_bytes_of(offsets, "offsets"),
-                                starts.data_ptr(), index_bytes_of(starts, "starts"), stream_of(k)));
+  const int32_t heads = static_cast<int32_t>(c.heads), D = static_cast<int32_t>(c.D);
+  if (c.bits == 16)
+    MX_CALL(mx_paged_cache_append(&c.c, mx_dtype_of(k.scalar_type()), heads, D, &ko, &vo, k.size(0), B,
+                                  offsets.data_ptr(), index_bytes_of(offsets, "offsets"),
+                                  starts.data_ptr(), index_bytes_of(starts, "starts"), stream_of(k)));
+  else
+    MX_CALL(mx_paged_cache_append_rows(&c.c, c.bits, mx_dtype_of(k.scalar_type()), 0, heads, D, nullptr, &ko, &vo,
+                                       nullptr, k.size(0), B, offsets.data_ptr(),
+                                       index_bytes_of(offsets, "offsets"), starts.data_ptr(),
+                                       index_bytes_of(starts, "starts"), nullptr, stream_of(k)));
 }
 
-// The append as autograd sees it: the caches' versions move on, so that a backward
-// that has saved one of them notices.
+// An append moves the caches' versions on, so that a backward that has saved one
+// of them notices.
+void bump_versions(const Tensor& k_cache, const Tensor& v_cache) {
+  for (const Tensor* t : {&k_cache, &v_cache})
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();  // (inference tensors keep none)
+}
+
+// The append as autograd sees it.
 void paged_cache_append_inplace(const Tensor& k, const Tensor& v, const Tensor& offsets, const Tensor& starts,
                                 const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table) {
   {
     at::AutoDispatchBelowADInplaceOrView g;
     paged_cache_append(k, v, offsets, starts, k_cache, v_cache, page_table);
   }
-  for (const Tensor* t : {&k_cache, &v_cache})
-    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();  // (inference tensors keep none)
+  bump_versions(k_cache, v_cache);
+}
+
+// The angles of the positions, [positions, pairs, 2] fp32, for heads of width D.
+mx_rotary rotary_operand(const Tensor& table, const Tensor& like, int64_t D, bool interleaved, Tensor& keep) {
+  check_arg(table, like, "table", false);
+  TORCH_CHECK(table.scalar_type() == at::kFloat && table.dim() == 3 && table.size(2) == 2,
+              "table must be float32 [positions, pairs, 2], got ", table.scalar_type(), " ", table.sizes());
+  TORCH_CHECK(table.size(1) > 0 && table.size(1) % 4 == 0 && 2 * table.size(1) <= D, "table has ", table.size(1),
+              " pairs: twice their number must be a multiple of 8 up to the head width ", D);
+  TORCH_CHECK(table.size(0) < (1ll << 31), "table has too many positions: ", table.size(0));
+  const bool ready = table.is_contiguous() && reinterpret_cast<uintptr_t>(table.data_ptr()) % 16 == 0;
+  keep = ready ? table : table.clone(at::MemoryFormat::Contiguous);
+  return {keep.data_ptr<float>(), keep.size(0), static_cast<int32_t>(keep.size(1)), interleaved ? 1 : 0};
+}
+
+Tensor run_jagged_rotary(const Tensor& x, const Tensor& offsets, const Tensor& table,
+                         const std::optional<Tensor>& starts, bool interleaved, bool inverse) {
+  check_gpu(x, "x");
+  c10::OptionalDeviceGuard guard(x.device());
+  check_rows(x, x, "x");
+  const int32_t dtype = attention_dtype(x, "x");
+  check_head_width(x.size(2));
+  TORCH_CHECK(x.size(1) < (1 << 20), "too many heads: ", x.size(1));
+  check_arg(offsets, x, "offsets", false);
+  TORCH_CHECK(offsets.dim() == 1 && offsets.numel() >= 1, "offsets must be 1-D with at least one entry");
+  const int64_t B = offsets.numel() - 1;
+  const int32_t offsets_bytes = index_bytes_of(offsets, "offsets");
+  const Tensor o = offsets.contiguous();
+  Tensor first, angles, rows;
+  if (starts.has_value() && starts->defined()) {
+    check_arg(*starts, x, "starts", false);
+    TORCH_CHECK(starts->dim() == 1 && starts->numel() == B, "starts must have ", B, " entries, got ",
+                starts->sizes());
+    index_bytes_of(*starts, "starts");
+    first = starts->contiguous();
+  }
+  const mx_rotary r = rotary_operand(table, x, x.size(2), interleaved, angles);
+  const mx_attention_tensor xo = attention_operand(x, rows);
+  Tensor out = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+  const bool has = first.defined() && B > 0;
+  MX_CALL(mx_jagged_rotary(dtype, &xo, x.size(0), static_cast<int32_t>(x.size(1)), static_cast<int32_t>(x.size(2)),
+                           &r, inverse ? 1 : 0, B, o.data_ptr(), offsets_bytes, has ? first.data_ptr() : nullptr,
+                           has ? index_bytes_of(first, "starts") : 0, out.data_ptr(), stream_of(x)));
+  return out;
+}
+
+Tensor jagged_rotary_plain(const Tensor& x, const Tensor& offsets, const Tensor& table,
+                           const std::optional<Tensor>& starts, bool interleaved) {
+  return run_jagged_rotary(x, offsets, table, starts, interleaved, false);
+}
+
+Tensor jagged_rotary_backward(const Tensor& grad_output, const Tensor& offsets, const Tensor& table,
+                              const std::optional<Tensor>& starts, bool interleaved) {
+  return run_jagged_rotary(grad_output, offsets, table, starts, interleaved, true);
+}
+
+// Linear in x: its gradient is the rotation back, which has a gradient of its own.
+class JaggedRotary : public torch::autograd::Function<JaggedRotary> {
+ public:
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& offsets, const Tensor& table,
+                        const std::optional<Tensor>& starts, bool interleaved, bool inverse) {
+    at::AutoDispatchBelowADInplaceOrView g;
+    const bool has = starts.has_value() && starts->defined();
+    ctx->save_for_backward({offsets, table, has ? *starts : Tensor()});
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["inverse"] = inverse;
+    return run_jagged_rotary(x, offsets, table, starts, interleaved, inverse);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list r(6);
+    if (!grads[0].defined() || !ctx->needs_input_grad(0)) return r;
+    const auto s = ctx->get_saved_variables();
+    const std::optional<Tensor> starts = s[2].defined() ? std::optional<Tensor>(s[2]) : std::nullopt;
+    const bool interleaved = ctx->saved_data["interleaved"].toBool(), inverse = ctx->saved_data["inverse"].toBool();
+    if (at::GradMode::is_enabled() && grads[0].requires_grad())
+      r[0] = JaggedRotary::apply(grads[0], s[0], s[1], starts, interleaved, !inverse);
+    else
+      r[0] = run_jagged_rotary(grads[0], s[0], s[1], starts, interleaved, !inverse);
+    return r;
+  }
+};
+
+Tensor rotary_autograd(const Tensor& x, const Tensor& offsets, const Tensor& table,
+                       const std::optional<Tensor>& starts, bool interleaved, bool inverse) {
+  // Below, a tangent would be dropped without a word.
+  TORCH_CHECK_NOT_IMPLEMENTED(!c10::AutogradState::get_tls_state().get_fw_grad_mode() ||
+                                  !(x._fw_grad(0).defined() || table._fw_grad(0).defined()),
+                              "jagged_rotary has no forward-mode derivative");
+  TORCH_CHECK(!at::GradMode::is_enabled() || !table.requires_grad(), "jagged_rotary has no gradient of its table");
+  if (at::GradMode::is_enabled() && x.requires_grad())
+    return JaggedRotary::apply(x, offsets, table, starts, interleaved, inverse);
+  at::AutoDispatchBelowADInplaceOrView g;
+  return run_jagged_rotary(x, offsets, table, starts, interleaved, inverse);
+}
+
+Tensor jagged_rotary_autograd(const Tensor& x, const Tensor& offsets, const Tensor& table,
+                              const std::optional<Tensor>& starts, bool interleaved) {
+  return rotary_autograd(x, offsets, table, starts, interleaved, false);
+}
+
+Tensor jagged_rotary_backward_autograd(const Tensor& grad_output, const Tensor& offsets, const Tensor& table,
+                                       const std::optional<Tensor>& starts, bool interleaved) {
+  return rotary_autograd(grad_output, offsets, table, starts, interleaved, true);
+}
+
+Tensor paged_cache_append_rotary(const std::optional<Tensor>& q, const Tensor& k, const Tensor& v,
+                                 const Tensor& offsets, const Tensor& starts, const Tensor& table,
+                                 const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table,
+                                 bool interleaved) {
+  check_gpu(k, "k");
+  c10::OptionalDeviceGuard guard(k.device());
+  check_arg(k_cache, k, "k_cache", false);
+  const CacheCall c = pack_cache(k_cache, v_cache, page_table);
+  check_appended(k, v, k_cache, c);
+  const int64_t B = page_table.size(0), N = k.size(0);
+  check_lists(offsets, starts, k, B);
+  const bool has = q.has_value() && q->defined();
+  if (has) {
+    check_rows(*q, k, "q");
+    TORCH_CHECK(q->size(0) == N && q->size(2) == c.D, "q is ", q->sizes(), " but k has ", N, " rows of width ", c.D);
+    TORCH_CHECK(q->size(1) < (1 << 20), "too many heads: ", q->size(1));
+  }
+  const int64_t H = has ? q->size(1) : 0;
+  Tensor angles, kq, kk, kv;
+  const mx_rotary r = rotary_operand(table, k, c.D, interleaved, angles);
+  const mx_attention_tensor ko = attention_operand(k, kk), vo = attention_operand(v, kv);
+  const mx_attention_tensor qo = H > 0 ? attention_operand(*q, kq) : mx_attention_tensor{};
+  Tensor out = at::empty({N, H, c.D}, k.options().memory_format(at::MemoryFormat::Contiguous));
+  MX_CALL(mx_paged_cache_append_rows(&c.c, c.bits, mx_dtype_of(k.scalar_type()), static_cast<int32_t>(H),
+                                     static_cast<int32_t>(c.heads), static_cast<int32_t>(c.D),
+                                     H > 0 ? &qo : nullptr, &ko, &vo, &r, N, B, offsets.data_ptr(),
+                                     index_bytes_of(offsets, "offsets"), starts.data_ptr(),
+                                     index_bytes_of(starts, "starts"), out.data_ptr(), stream_of(k)));
+  return out;
+}
+
+Tensor paged_cache_append_rotary_inplace(const std::optional<Tensor>& q, const Tensor& k, const Tensor& v,
+                                         const Tensor& offsets, const Tensor& starts, const Tensor& table,
+                                         const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table,
+                                         bool interleaved) {
+  // The rotated queries would come back without their graph.
+  TORCH_CHECK(!at::GradMode::is_enabled() || !(q.has_value() && q->defined() && q->requires_grad()),
+              "paged_cache_append_rotary has no gradient: call it under torch.no_grad(), or jagged_rotary");
+  Tensor out;
+  {
+    at::AutoDispatchBelowADInplaceOrView g;
+    out = paged_cache_append_rotary(q, k, v, offsets, starts, table, k_cache, v_cache, page_table, interleaved);
+  }
+  bump_versions(k_cache, v_cache);
+  return out;
 }
 
 Tensor paged_cache_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache,
@@ -2215,10 +2408,10 @@ Tensor paged_cache_attention(const Tensor& q, const Tensor& k_cache, const Tenso
   check_gpu(q, "q");
   c10::OptionalDeviceGuard guard(q.device());
   check_arg(k_cache, q, "k_cache", false);
-  const mx_paged_cache c = pack_cache(k_cache, v_cache, page_table);
-  check_rows(q, k_cache, "q");
-  const int64_t B = q.size(0), H = q.size(1), D = q.size(2), Hkv = k_cache.size(2);
-  TORCH_CHECK(D == k_cache.size(3), "q has head width ", D, " but the cache ", k_cache.size(3));
+  const CacheCall c = pack_cache(k_cache, v_cache, page_table);
+  check_cache_rows(q, c.bits == 16 ? k_cache : q, c, "q");
+  const int64_t B = q.size(0), H = q.size(1), D = q.size(2), Hkv = c.heads;
+  TORCH_CHECK(D == c.D, "q has head width ", D, " but the cache ", c.D);
   TORCH_CHECK(H > 0 && H % Hkv == 0 && H < (1 << 20), "q has ", H, " heads, which is no multiple of the ", Hkv,
               " key-value heads");
   TORCH_CHECK(page_table.size(0) == B, "page_table has ", page_table.size(0), " rows but q ", B);
@@ -2228,16 +2421,41 @@ Tensor paged_cache_attention(const Tensor& q, const Tensor& k_cache, const Tenso
   Tensor keep;
   const mx_attention_tensor qo = attention_operand(q, keep);
   Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
-  const size_t ws_bytes = mx_paged_cache_attention_workspace_bytes(
-      &c, B, static_cast<int32_t>(H), static_cast<int32_t>(Hkv), static_cast<int32_t>(D));
+  const auto bytes_of = c.bits == 16 ? mx_paged_cache_attention_workspace_bytes
+                                     : mx_paged_cache_attention_int4_workspace_bytes;
+  const auto attend = c.bits == 16 ? mx_paged_cache_attention : mx_paged_cache_attention_int4;
+  const size_t ws_bytes = bytes_of(&c.c, B, static_cast<int32_t>(H), static_cast<int32_t>(Hkv), static_cast<int32_t>(D));
   Tensor ws;
   if (ws_bytes > 0) ws = at::empty({static_cast<int64_t>(ws_bytes)}, q.options().dtype(at::kByte));
-  MX_CALL(mx_paged_cache_attention(&c, mx_dtype_of(q.scalar_type()), &qo, B, static_cast<int32_t>(H),
-                                   static_cast<int32_t>(Hkv), static_cast<int32_t>(D),
-                                   lengths.data_ptr(), index_bytes_of(lengths, "lengths"),
-                                   attention_scale(scale, D), out.data_ptr(),
-                                   ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, stream_of(q)));
+  MX_CALL(attend(&c.c, mx_dtype_of(q.scalar_type()), &qo, B, static_cast<int32_t>(H), static_cast<int32_t>(Hkv),
+                 static_cast<int32_t>(D), lengths.data_ptr(), index_bytes_of(lengths, "lengths"),
+                 attention_scale(scale, D), out.data_ptr(), ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes,
+                 stream_of(q)));
   return out;
+}
+
+std::tuple<Tensor, Tensor> paged_cache_gather(const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table,
+                                              const Tensor& offsets, int64_t total,
+                                              std::optional<at::ScalarType> dtype) {
+  check_gpu(k_cache, "k_cache");
+  c10::OptionalDeviceGuard guard(k_cache.device());
+  const CacheCall c = pack_cache(k_cache, v_cache, page_table);
+  const at::ScalarType type = dtype.value_or(c.bits == 16 ? k_cache.scalar_type() : at::kBFloat16);
+  TORCH_CHECK(type == at::kHalf || type == at::kBFloat16, "dtype must be float16 or bfloat16, got ", type);
+  TORCH_CHECK(c.bits == 4 || type == k_cache.scalar_type(), "the cache is ", k_cache.scalar_type(),
+              " but dtype ", type);
+  const int64_t B = page_table.size(0);
+  check_arg(offsets, k_cache, "offsets", true);
+  TORCH_CHECK(offsets.dim() == 1 && offsets.numel() == B + 1, "offsets must have ", B + 1, " entries, got ",
+              offsets.sizes());
+  TORCH_CHECK(total >= 0, "total must not be negative, got ", total);
+  const auto opts = k_cache.options().dtype(type).memory_format(at::MemoryFormat::Contiguous);
+  Tensor k = at::empty({total, c.heads, c.D}, opts), v = at::empty({total, c.heads, c.D}, opts);
+  MX_CALL(mx_paged_cache_gather(&c.c, c.bits, mx_dtype_of(type), static_cast<int32_t>(c.heads),
+                                static_cast<int32_t>(c.D), total, B, offsets.data_ptr(),
+                                index_bytes_of(offsets, "offsets"), k.data_ptr(), v.data_ptr(),
+                                stream_of(k_cache)));
+  return {k, v};
 }
 
 }  // namespace mx_ops
@@ -2495,6 +2713,15 @@ TORCH_LIBRARY(mx_fbgemm, m) {
         "Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor page_table) -> ()");
   m.def("paged_cache_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor page_table, "
         "Tensor lengths, float? scale=None) -> Tensor");
+  m.def("jagged_rotary(Tensor x, Tensor offsets, Tensor table, Tensor? starts=None, "
+        "bool interleaved=False) -> Tensor");
+  m.def("jagged_rotary_backward(Tensor grad_output, Tensor offsets, Tensor table, Tensor? starts=None, "
+        "bool interleaved=False) -> Tensor");
+  m.def("paged_cache_append_rotary(Tensor? q, Tensor k, Tensor v, Tensor offsets, Tensor starts, "
+        "Tensor table, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor page_table, "
+        "bool interleaved=False) -> Tensor");
+  m.def("paged_cache_gather(Tensor k_cache, Tensor v_cache, Tensor page_table, Tensor offsets, "
+        "int total, ScalarType? dtype=None) -> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(mx_fbgemm, CUDA, m) {
@@ -2503,12 +2730,19 @@ TORCH_LIBRARY_IMPL(mx_fbgemm, CUDA, m) {
   m.impl("jagged_attention_backward", TORCH_FN(mx_ops::jagged_attention_backward));
   m.impl("paged_cache_append", TORCH_FN(mx_ops::paged_cache_append));
   m.impl("paged_cache_attention", TORCH_FN(mx_ops::paged_cache_attention));
+  m.impl("jagged_rotary", TORCH_FN(mx_ops::jagged_rotary_plain));
+  m.impl("jagged_rotary_backward", TORCH_FN(mx_ops::jagged_rotary_backward));
+  m.impl("paged_cache_append_rotary", TORCH_FN(mx_ops::paged_cache_append_rotary));
+  m.impl("paged_cache_gather", TORCH_FN(mx_ops::paged_cache_gather));
 }
 
 TORCH_LIBRARY_IMPL(mx_fbgemm, ADInplaceOrView, m) {
   m.impl("paged_cache_append", TORCH_FN(mx_ops::paged_cache_append_inplace));
+  m.impl("paged_cache_append_rotary", TORCH_FN(mx_ops::paged_cache_append_rotary_inplace));
 }
 
 TORCH_LIBRARY_IMPL(mx_fbgemm, Autograd, m) {
   m.impl("jagged_attention", TORCH_FN(mx_ops::jagged_attention_autograd));
+  m.impl("jagged_rotary", TORCH_FN(mx_ops::jagged_rotary_autograd));
+  m.impl("jagged_rotary_backward", TORCH_FN(mx_ops::jagged_rotary_backward_autograd));
 }

@@ -32,7 +32,7 @@ OPS_LIB = LIB_DIR / "mx_fbgemm_ops.so"
 
 HIP_SOURCES = ["abi.hip", "jagged.hip", "tbe_fwd.hip", "tbe_bwd.hip", "nbit_fwd.hip",
                "nbit_nobag.hip", "bounds_check.hip", "codec.hip", "vbe.hip", "sparse_ops.hip",
-               "jagged_attention.hip", "paged_cache.hip"]
+               "jagged_attention.hip", "paged_cache.hip", "paged_cache_int4.hip", "paged_rows.hip"]
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 ARCH = "gfx950"
 
