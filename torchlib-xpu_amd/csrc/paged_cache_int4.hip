@@ -7,6 +7,8 @@
 //   out = sum_j p_j s_j e_j + sum_j p_j f_j,   p = softmax(score):
 // the matrix products run on the codes themselves, scale and bias enter once per
 // token.
+#include <type_traits>
+
 #include "paged_common.h"
 #include "row_codec.h"
 
@@ -15,14 +17,23 @@ namespace attn {
 namespace {
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
 // 128 + c as bf16 (exponent 7, seven bits of mantissa): a code in the low bits of
-// each half of a word, in one instruction for two.
-__device__ __forceinline__ uint32_t codes2(uint32_t w) { return (w & 0x000f000fu) | 0x43004300u; }
+// each half of a word, in one instruction for two (the compiler knows neither
+// constant, or it would take two instructions with a literal each).
+struct Codes {
+  uint32_t mask, one28;
+  __device__ __forceinline__ Codes() {
+    asm("s_mov_b32 %0, 0x000f000f" : "=s"(mask));
+    asm("v_mov_b32 %0, 0x43004300" : "=v"(one28));
+  }
+  __device__ __forceinline__ int two(uint32_t w) const { return static_cast<int>((w & mask) | one28); }
+};
 constexpr float kOffset = 136.0f;  // 128 + c - 136 = c - 8
 
 __device__ __forceinline__ bf16x8 splat(float v) {
@@ -38,6 +49,26 @@ __device__ __forceinline__ uint32_t load_codes(const char* p) {
   else return *reinterpret_cast<const uint8_t*>(p);
 }
 
+// KS words from a multiple of 4 bytes.
+template <int KS>
+__device__ __forceinline__ void load_words(const char* p, uint32_t (&w)[KS]) {
+  if constexpr (KS == 1) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else {
+    typedef uint32_t V __attribute__((ext_vector_type(KS), aligned(4)));
+    const V v = *reinterpret_cast<const V*>(p);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) w[s] = v[s];
+  }
+}
+
+// A wave's 32 keys as they lie in memory: codes of two keys (a quarter of the row
+// each) and of eight values (EV columns each), and a row's scale and bias.
+template <int KS>
+struct Tile4 {
+  uint32_t k[2][KS], v[8], tail, seen;
+};
+
 // One block: up to 16 query heads of one key-value head, and a share of its
 // tiles (or one sequence), as attention over a 16-bit cache; its waves take 32
 // of a tile's keys each.  Codes go straight into registers and become bf16
@@ -46,8 +77,8 @@ __device__ __forceinline__ uint32_t load_codes(const char* p) {
 // which come out as one operand each of DP / 16 products.  The integers are
 // 128 + c; -136 times the other operand's sum starts each product off, so that
 // what is summed is c - 8 and no more than a tile's offset ever stands in a sum.
-// fp16 queries (and, for them, probabilities) are split into two bf16 parts.
-template <typename T, int DP, int WAVES>
+// fp16 queries, and p_j s_j, are split into two bf16 parts.
+template <typename T, int DP, int WAVES, bool P16>
 __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? 2 : WAVES / 4) step4_kernel(const StepArgs a) {
   using E = Elem<T>;
   constexpr bool kSplit = E::kNarrow;
@@ -70,6 +101,16 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? 2 : WAVES / 
   const char* kb = a.c.k + kvh * a.c.k_head;
   const char* vb = a.c.v + kvh * a.c.v_head;
   const int words = a.D / 8, tail = a.D / 2;
+  const Codes codes;
+  // The lane's place in a row of codes: words word0.. of a key, the byte of its
+  // first column of a value (past the row's end: the first, of a column unused).
+  const int word0 = KS * g < words - KS ? KS * g : words - KS;
+  const int column = EV * r < a.D ? EV * r / 2 : 0;
+  // And among 16 rows of a page.
+  const int64_t k_at = r * a.c.k_slot + word0 * 4, tail_at = r * (g < 2 ? a.c.k_slot : a.c.v_slot) + tail;
+  int64_t v_at[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v_at[i] = (4 * g + i) * a.c.v_slot + column;
 
   // The share: tiles [at, stop) counted from sequence b's first one.
   const bool shared = WAVES == kStepWaves && a.workers > 0;
@@ -88,13 +129,15 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? 2 : WAVES / 
     const int32_t end = t1 * kTile < len ? t1 * kTile : len;
 
     // Queries in the codes' order: a word's halves hold codes 0 4, 1 5, 2 6, 3 7.
+    // A row's end may cut its quarters short: they begin early enough then, and
+    // what another quarter has too meets zeros.
     bf16x8 qf[KS], ql[KS];
     f32x4 total{};
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      const int word = KS * g + s;
+      const int word = word0 + s;
       i32x4 w{};
-      if (r < heads && word < words)
+      if (r < heads && word >= KS * g)
         w = *reinterpret_cast<const i32x4*>(a.q + b * a.q_row + (head0 + r) * a.q_head + word * 16);
       const typename E::x8 x = __builtin_bit_cast(typename E::x8, w);
 #pragma unroll
@@ -114,52 +157,59 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? 2 : WAVES / 
     for (int t = 0; t < EV; ++t) o[t] = f32x4{};
 
     const int32_t* row = a.c.table + b * a.c.table_row;
-    auto entry = [&](int32_t k0, int* slot) {
-      const uint32_t key = k0 + (lane & 31);
-      const uint32_t size = a.c.page_size;
-      const uint32_t e = a.c.page_shift >= 0 ? key >> a.c.page_shift : key / size;
-      *slot = static_cast<int>(key - e * size);
-      return key < static_cast<uint32_t>(end) ? row[e] : -1;
-    };
-    const int32_t first = t0 * kTile + wave * kStepKeys;
-    int slot_next = 0;
-    int32_t page_next = entry(first, &slot_next);
-    for (int32_t k0 = first; k0 < end; k0 += kTile) {
-      const int64_t page = page_next;
-      const int slot = slot_next;
-      page_next = entry(k0 + kTile, &slot_next);
-      const bool there = page >= 0 && page < a.c.pages;
-      const uint32_t seen = static_cast<uint32_t>(__ballot(there));
-      const int64_t koff = there ? page * a.c.k_page + slot * a.c.k_slot : 0;
-      const int64_t voff = there ? page * a.c.v_page + slot * a.c.v_slot : 0;
-
-      // Scale and bias: lanes 0..31 of the keys, 32..63 of the values.
-      uint32_t sb = 0;
-      if (there) sb = *reinterpret_cast<const uint32_t*>((lane < 32 ? kb + koff : vb + voff) + tail);
-      uint32_t kw[2][KS];
+    // Asks for the rows of 32 keys from k0 on.  Those of no token are read from
+    // wherever is safe: what they hold never shows.
+    auto load = [&](int32_t k0, Tile4<KS>* x) {
+      if constexpr (P16) {
+        // 16 keys from a multiple of 16 are in one page: addresses are the wave's.
+        const char *ka[2], *va[2];
+        x->seen = 0;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const char* p = kb + shfl64(koff, 16 * u + r) + KS * g * 4;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          kw[u][s] = 0;
-          if (KS * g + s < words) kw[u][s] = reinterpret_cast<const uint32_t*>(p)[s];
+        for (int u = 0; u < 2; ++u) {
+          const int32_t key = k0 + 16 * u;
+          const uint32_t size = a.c.page_size;
+          const uint32_t e = a.c.page_shift >= 0 ? static_cast<uint32_t>(key) >> a.c.page_shift : key / size;
+          const int32_t slot = key - e * size;
+          int32_t page = key < end ? load_scalar(row + e) : -1;
+          const bool there = page >= 0 && page < a.c.pages;
+          page = there ? page : 0;
+          const int left = end - key;
+          x->seen |= there ? (left >= 16 ? 0xffffu : (1u << left) - 1u) << (16 * u) : 0u;
+          ka[u] = kb + page * a.c.k_page + (there ? slot : 0) * a.c.k_slot;
+          va[u] = vb + page * a.c.v_page + (there ? slot : 0) * a.c.v_slot;
         }
-      }
-      uint32_t vw[8];
+        const char* t = g == 0 ? ka[0] : g == 1 ? ka[1] : g == 2 ? va[0] : va[1];
+        x->tail = *reinterpret_cast<const uint32_t*>(t + tail_at);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int nk = 16 * (i / 4) + 4 * g + i % 4;
-        const char* p = vb + shfl64(voff, nk);
-        vw[i] = 0;
-        if (EV * r < a.D && ((seen >> nk) & 1)) vw[i] = load_codes<EV>(p + EV * r / 2);
+        for (int u = 0; u < 2; ++u) {
+          load_words<KS>(ka[u] + k_at, x->k[u]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x->v[4 * u + i] = load_codes<EV>(va[u] + v_at[i]);
+        }
+      } else {
+        const uint32_t key = k0 + (lane & 31), size = a.c.page_size;
+        const uint32_t e = a.c.page_shift >= 0 ? key >> a.c.page_shift : key / size;
+        const int64_t page = key < static_cast<uint32_t>(end) ? row[e] : -1;
+        const bool there = page >= 0 && page < a.c.pages;
+        x->seen = static_cast<uint32_t>(__ballot(there));
+        const int32_t slot = key - e * size;
+        const int64_t koff = there ? page * a.c.k_page + slot * a.c.k_slot : 0;
+        const int64_t voff = there ? page * a.c.v_page + slot * a.c.v_slot : 0;
+        x->tail = *reinterpret_cast<const uint32_t*>((lane < 32 ? kb + koff : vb + voff) + tail);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) load_words<KS>(kb + shfl64(koff, 16 * u + r) + word0 * 4, x->k[u]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          x->v[i] = load_codes<EV>(vb + shfl64(voff, 16 * (i / 4) + 4 * g + i % 4) + column);
       }
-
+    };
+    auto sum_up = [&](const Tile4<KS>& x) {
+      const uint32_t seen = x.seen;
       {
         RowCodec<4, false> codec;
-        codec.load(reinterpret_cast<const uint8_t*>(&sb));
+        codec.load(reinterpret_cast<const uint8_t*>(&x.tail));
         const float f = __builtin_fmaf(8.0f, codec.scale, codec.bias);
-        sh_tail[wave][lane >> 5][lane & 31] = there ? f32x2{codec.scale, f} : f32x2{};
+        sh_tail[wave][lane >> 5][lane & 31] = (seen >> (lane & 31)) & 1 ? f32x2{codec.scale, f} : f32x2{};
       }
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
@@ -176,20 +226,21 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? 2 : WAVES / 
 
       f32x4 s[2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        s[u] = f32x4{start, start, start, start};
+      for (int u = 0; u < 2; ++u) s[u] = f32x4{start, start, start, start};
 #pragma unroll
-        for (int x = 0; x < KS; ++x) {
-          const uint32_t w = kw[u][x];
-          const i32x4 c = {static_cast<int>(codes2(w)), static_cast<int>(codes2(w >> 4)),
-                           static_cast<int>(codes2(w >> 8)), static_cast<int>(codes2(w >> 12))};
-          s[u] = mfma(__builtin_bit_cast(bf16x8, c), qf[x], s[u]);
-          if constexpr (kSplit) s[u] = mfma(__builtin_bit_cast(bf16x8, c), ql[x], s[u]);
+      for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint32_t w = x.k[u][i];
+          const bf16x8 c = __builtin_bit_cast(
+              bf16x8, i32x4{codes.two(w), codes.two(w >> 4), codes.two(w >> 8), codes.two(w >> 12)});
+          s[u] = mfma(c, qf[i], s[u]);
+          if constexpr (kSplit) s[u] = mfma(c, ql[i], s[u]);
         }
-      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) s[i / 4][i % 4] = __builtin_fmaf(kt[i][0], s[i / 4][i % 4], kt[i][1] * qsum);
       if (seen != 0xffffffffu) {
+        asm volatile("" ::: "memory");  // a branch: hardly any tile comes here
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -210,33 +261,54 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? 2 : WAVES / 
         m = m2;
       }
       const float mc = m == -INFINITY ? 0.0f : m * c2;
-      bf16x8 p, pl;
+      f32x8 ps;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float e = exp2_hw(__builtin_fmaf(s[i / 4][i % 4], c2, -mc));
         sum += e;
         add = __builtin_fmaf(e, vt[i][1], add);
-        const float ps = e * vt[i][0];
-        p[i] = static_cast<__bf16>(ps);
-        if constexpr (kSplit) pl[i] = static_cast<__bf16>(ps - static_cast<float>(p[i]));
+        ps[i] = e * vt[i][0];
       }
+      const bf16x8 p = __builtin_convertvector(ps, bf16x8);
+      const bf16x8 pl = __builtin_convertvector(ps - __builtin_convertvector(p, f32x8), bf16x8);
+      const bf16x8 minus = splat(-kOffset);
 #pragma unroll
-      for (int t = 0; t < EV; ++t) {
-        // Columns EV r + t of the eight keys, two to a word.
-        i32x4 c;
+      for (int t = 0; t < EV; ++t) o[t] = mfma(minus, p, o[t]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t w = t < 4 ? (vw[2 * i] & 0xffffu) | (vw[2 * i + 1] << 16)
-                                   : (vw[2 * i] >> 16) | (vw[2 * i + 1] & 0xffff0000u);
-          c[i] = codes2(w >> (4 * (t & 3)));
+      for (int t = 0; t < EV; ++t) o[t] = mfma(minus, pl, o[t]);
+      // Columns EV r + t of the eight keys, two to a word.
+      constexpr int kHalves = EV == 8 ? 2 : 1, kColumns = EV == 8 ? 4 : EV;
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          w[i] = __builtin_amdgcn_perm(x.v[2 * i + 1], x.v[2 * i], h == 0 ? 0x05040100u : 0x07060302u);
+#pragma unroll
+        for (int t = 0; t < kColumns; ++t) {
+          i32x4 c;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) c[i] = codes.two(w[i] >> (4 * t));
+          const bf16x8 y = __builtin_bit_cast(bf16x8, c);
+          o[4 * h + t] = mfma(y, p, o[4 * h + t]);
+          o[4 * h + t] = mfma(y, pl, o[4 * h + t]);
         }
-        const bf16x8 x = __builtin_bit_cast(bf16x8, c);
-        o[t] = mfma(splat(-kOffset), p, o[t]);
-        o[t] = mfma(x, p, o[t]);
-        if constexpr (kSplit) {
-          o[t] = mfma(splat(-kOffset), pl, o[t]);
-          o[t] = mfma(x, pl, o[t]);
-        }
+      }
+    };
+    // A tile's rows are asked for one tile ahead.
+    int32_t k0 = t0 * kTile + wave * kStepKeys;
+    if (k0 < end) {
+      Tile4<KS> x0, x1;
+      load(k0, &x0);
+      while (true) {
+        if (k0 + kTile < end) load(k0 + kTile, &x1);
+        sum_up(x0);
+        k0 += kTile;
+        if (k0 >= end) break;
+        if (k0 + kTile < end) load(k0 + kTile, &x0);
+        sum_up(x1);
+        k0 += kTile;
+        if (k0 >= end) break;
       }
     }
 
@@ -282,10 +354,14 @@ int launch_step(const StepArgs& a, hipStream_t s) {
   const int64_t blocks = static_cast<int64_t>(a.workers > 0 ? a.workers : a.B) * a.Hkv * a.head_blocks;
   const int64_t joins = static_cast<int64_t>(a.B) * a.H;
   MX_REQUIRE(blocks < (1ll << 22) && joins < (1ll << 22), "too many sequences: %d", a.B);  // threads in 32 bits
-  if (a.wide)
-    step4_kernel<T, DP, wide_waves(DP)><<<dim3(static_cast<unsigned>(blocks)), wide_waves(DP) * 64, 0, s>>>(a);
-  else
-    step4_kernel<T, DP, kStepWaves><<<dim3(static_cast<unsigned>(blocks)), kStepWaves * 64, 0, s>>>(a);
+  auto launch = [&](auto p16) {
+    constexpr bool P16 = decltype(p16)::value;
+    const dim3 grid(static_cast<unsigned>(blocks));
+    if (a.wide) step4_kernel<T, DP, wide_waves(DP), P16><<<grid, wide_waves(DP) * 64, 0, s>>>(a);
+    else step4_kernel<T, DP, kStepWaves, P16><<<grid, kStepWaves * 64, 0, s>>>(a);
+  };
+  if (a.c.page_size % 16 == 0) launch(std::true_type{});
+  else launch(std::false_type{});
   if (a.workers > 0) {
     const int waves = a.workers / a.B < 8 ? 1 : a.workers / a.B < 32 ? 4 : kJoinMost;
     join_kernel<T><<<dim3(static_cast<unsigned>(joins)), waves * 64, 0, s>>>(a);
