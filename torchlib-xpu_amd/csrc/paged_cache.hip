@@ -111,18 +111,20 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? 2 : WAVES / 
 
   // The share: tiles [at, stop) counted from sequence b's first one.
   const bool shared = WAVES == kStepWaves && a.workers > 0;
+  Cursor cursor;
   int32_t b = worker, len;
   int64_t at = 0, stop = 0;
   if (!shared) {
     len = __builtin_amdgcn_readfirstlane(tokens_of(a, b));
     stop = tiles_of<WAVES>(len);  // 0 for an empty one: its one pass writes the zeros
-  } else if (!find_share(a, worker, &b, &len, &at, &stop)) {
-    return;
+  } else {
+    if (!find_share(a, worker, &cursor, &at, &stop)) return;
+    b = cursor.b, len = cursor.length();
   }
 
   while (true) {
     const int32_t n = tiles_of<WAVES>(len);
-    const int32_t t0 = static_cast<int32_t>(at), t1 = static_cast<int32_t>(stop < n ? stop : n);
+    const int32_t t0 = static_cast<int32_t>(at > 0 ? at : 0), t1 = static_cast<int32_t>(stop < n ? stop : n);
     const int32_t end = t1 * kTile < len ? t1 * kTile : len;
 
     X8 qf[KS];
@@ -237,11 +239,12 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? 2 : WAVES / 
 #pragma unroll
       for (int i = 0; i < 4; ++i) sh_o[wave][r][EV * (4 * g + i) + t] = o[t][i];
     finish_block<T, WAVES, DP>(a, sh_o, sh_m, sh_l, worker, b, t0, t1, n, head0, heads);
-    if (!shared || stop <= n) return;  // a block per sequence never leaves its own
+    if (!shared || stop <= n + a.lead) return;  // a block per sequence never leaves its own
     // The next sequence that has tokens.
-    stop -= n;
+    stop -= n + a.lead;
     at = 0;
-    if (!next_sequence(a, &b, &len)) return;
+    if (!cursor.next(a)) return;
+    b = cursor.b, len = cursor.length();
     __syncthreads();
   }
 }
@@ -392,7 +395,7 @@ extern "C" int mx_paged_cache_attention(const mx_paged_cache* cache, int32_t dty
   a.lengths = lengths, a.lengths_bytes = lengths_bytes;
   a.B = static_cast<int32_t>(B), a.H = H, a.Hkv = Hkv, a.G = H / Hkv, a.D = D;
   a.head_blocks = head_blocks_of(H, Hkv);
-  a.scale = scale;
+  a.scale = scale, a.units = scale * kLog2e;
   a.out = out;
   const Plan plan = plan_step(B, Hkv * a.head_blocks, D, cache->table_width * cache->page_size);
   a.workers = plan.workers, a.wide = plan.wide;

@@ -19,27 +19,34 @@ namespace {
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 
-__device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+__device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// 128 + c as bf16 (exponent 7, seven bits of mantissa): a code in the low bits of
-// each half of a word, in one instruction for two (the compiler knows neither
-// constant, or it would take two instructions with a literal each).
+// Codes as fp16, two to an instruction: with the exponent of 1024 (ulp 1) set above
+// it, a code in bits 0..3 of a half reads 1024 + c, one in bits 4..7 1024 + 16 c.
+// The compiler knows none of the constants, or it would take two instructions with
+// a literal each.
 struct Codes {
-  uint32_t mask, one28;
+  uint32_t low, high, base;
   __device__ __forceinline__ Codes() {
-    asm("s_mov_b32 %0, 0x000f000f" : "=s"(mask));
-    asm("v_mov_b32 %0, 0x43004300" : "=v"(one28));
+    asm("s_mov_b32 %0, 0x000f000f" : "=s"(low));
+    asm("s_mov_b32 %0, 0x00f000f0" : "=s"(high));
+    asm("v_mov_b32 %0, 0x64006400" : "=v"(base));
   }
-  __device__ __forceinline__ int two(uint32_t w) const { return static_cast<int>((w & mask) | one28); }
+  __device__ __forceinline__ int two(uint32_t w) const { return static_cast<int>((w & low) | base); }
+  __device__ __forceinline__ int two16(uint32_t w) const { return static_cast<int>((w & high) | base); }
 };
-constexpr float kOffset = 136.0f;  // 128 + c - 136 = c - 8
+constexpr float kOffset = 1032.0f;    // 1024 + c - 1032 = c - 8
+constexpr float kOffset16 = 1152.0f;  // 1024 + 16 c - 1152 = 16 (c - 8)
 
-__device__ __forceinline__ bf16x8 splat(float v) {
-  const __bf16 x = static_cast<__bf16>(v);
-  return bf16x8{x, x, x, x, x, x, x, x};
+// Of a word's eight codes, in the order of the operands (0 4, 1 5, 2 6, 3 7), those
+// that read 16 c: the third, fourth, seventh and eighth.
+__device__ __forceinline__ f16x8 pattern(float c, float c16) {
+  const _Float16 x = static_cast<_Float16>(c), y = static_cast<_Float16>(c16);
+  return f16x8{x, x, y, y, x, x, y, y};
 }
+__device__ __forceinline__ f16x8 splat(float v) { return pattern(v, v); }
 
 // N values (2, 4, 8) of a row's codes, in a word's low bits.
 template <int EV>
@@ -69,19 +76,31 @@ struct Tile4 {
   uint32_t k[2][KS], v[8], tail, seen;
 };
 
+// The tail of a head's range: a power of two by which its queries are scaled where
+// fp16 would not hold them (their sixteenths, too).
+__device__ __forceinline__ float query_scale(float largest) {
+  if (!(largest > 0.0f) || (largest >= 0.0625f && largest < 8192.0f)) return 1.0f;
+  const int e = static_cast<int>(__float_as_uint(largest) >> 23) - 127;  // subnormals: -127
+  return ldexpf(1.0f, e > 120 ? -120 : -e);
+}
+
 // One block: up to 16 query heads of one key-value head, and a share of its
 // tiles (or one sequence), as attention over a 16-bit cache; its waves take 32
-// of a tile's keys each.  Codes go straight into registers and become bf16
+// of a tile's keys each.  Codes go straight into registers and become fp16
 // integers there (r = lane % 16, g = lane / 16): for the scores the lane has key
 // r's g-th quarter of the row, for the second product DP / 16 columns of 8 keys,
 // which come out as one operand each of DP / 16 products.  The integers are
-// 128 + c; -136 times the other operand's sum starts each product off, so that
-// what is summed is c - 8 and no more than a tile's offset ever stands in a sum.
-// fp16 queries, and p_j s_j, are split into two bf16 parts.
+// 1024 + c or 1024 + 16 c; minus that many times the other operand's sum starts
+// each product off, so that what is summed is e or 16 e, and no more than a tile's
+// offset ever stands in a sum.
+//
+// Queries are exact in fp16, by a power of two per head where they are large or
+// small (bf16 ones 2^25 below the head's largest are rounded).  p_j s_j is rounded
+// to fp16 (2^-11), times a power of two that keeps the largest s seen below 128
+// (p stays below 256): those of an s 2^21 times smaller than the largest lose bits.
 template <typename T, int DP, int WAVES, bool P16>
-__global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? 2 : WAVES / 4) step4_kernel(const StepArgs a) {
+__global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? (DP <= 64 ? 3 : 2) : WAVES / 4) step4_kernel(const StepArgs a) {
   using E = Elem<T>;
-  constexpr bool kSplit = E::kNarrow;
   constexpr int kTile = WAVES * kStepKeys;
   constexpr int KS = DP / 32;  // products along D of a score; words of codes per lane
   constexpr int EV = DP / 16;  // columns of V per lane
@@ -102,81 +121,81 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? 2 : WAVES / 
   const char* vb = a.c.v + kvh * a.c.v_head;
   const int words = a.D / 8, tail = a.D / 2;
   const Codes codes;
+  // Strides inside a page, and of a page, are below 2^31 bytes (checked by the host).
+  const int32_t pages = static_cast<int32_t>(a.c.pages < 0x7fffffff ? a.c.pages : 0x7fffffff);
+  const uint32_t k_page = static_cast<uint32_t>(a.c.k_page), v_page = static_cast<uint32_t>(a.c.v_page);
+  const uint32_t k_slot = static_cast<uint32_t>(a.c.k_slot), v_slot = static_cast<uint32_t>(a.c.v_slot);
   // The lane's place in a row of codes: words word0.. of a key, the byte of its
   // first column of a value (past the row's end: the first, of a column unused).
   const int word0 = KS * g < words - KS ? KS * g : words - KS;
   const int column = EV * r < a.D ? EV * r / 2 : 0;
   // And among 16 rows of a page.
-  const int64_t k_at = r * a.c.k_slot + word0 * 4, tail_at = r * (g < 2 ? a.c.k_slot : a.c.v_slot) + tail;
-  int64_t v_at[4];
+  const uint32_t k_at = r * k_slot + word0 * 4, tail_at = r * (g < 2 ? k_slot : v_slot) + tail;
+  uint32_t v_at[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v_at[i] = (4 * g + i) * a.c.v_slot + column;
+  for (int i = 0; i < 4; ++i) v_at[i] = (4 * g + i) * v_slot + column;
 
   // The share: tiles [at, stop) counted from sequence b's first one.
   const bool shared = WAVES == kStepWaves && a.workers > 0;
+  Cursor cursor;
   int32_t b = worker, len;
   int64_t at = 0, stop = 0;
   if (!shared) {
     len = __builtin_amdgcn_readfirstlane(tokens_of(a, b));
     stop = tiles_of<WAVES>(len);  // 0 for an empty one: its one pass writes the zeros
-  } else if (!find_share(a, worker, &b, &len, &at, &stop)) {
-    return;
+  } else {
+    if (!find_share(a, worker, &cursor, &at, &stop)) return;
+    b = cursor.b, len = cursor.length();
   }
 
   while (true) {
     const int32_t n = tiles_of<WAVES>(len);
-    const int32_t t0 = static_cast<int32_t>(at), t1 = static_cast<int32_t>(stop < n ? stop : n);
+    const int32_t t0 = static_cast<int32_t>(at > 0 ? at : 0), t1 = static_cast<int32_t>(stop < n ? stop : n);
     const int32_t end = t1 * kTile < len ? t1 * kTile : len;
 
-    // Queries in the codes' order: a word's halves hold codes 0 4, 1 5, 2 6, 3 7.
-    // A row's end may cut its quarters short: they begin early enough then, and
-    // what another quarter has too meets zeros.
-    bf16x8 qf[KS], ql[KS];
-    f32x4 total{};
+    i32x4 qw[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const int word = word0 + s;
-      i32x4 w{};
+      qw[s] = i32x4{};
       if (r < heads && word >= KS * g)
-        w = *reinterpret_cast<const i32x4*>(a.q + b * a.q_row + (head0 + r) * a.q_head + word * 16);
-      const typename E::x8 x = __builtin_bit_cast(typename E::x8, w);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const T v = x[(i >> 1) + 4 * (i & 1)];
-        qf[s][i] = static_cast<__bf16>(static_cast<float>(v));
-        if constexpr (kSplit) ql[s][i] = static_cast<__bf16>(static_cast<float>(v) - static_cast<float>(qf[s][i]));
-      }
-      total = mfma(splat(1.0f), qf[s], total);
-      if constexpr (kSplit) total = mfma(splat(1.0f), ql[s], total);
+        qw[s] = *reinterpret_cast<const i32x4*>(a.q + b * a.q_row + (head0 + r) * a.q_head + word * 16);
     }
-    const float qsum = total[0];  // of head r
-    const float start = -kOffset * qsum;
-    float m = -INFINITY, sum = 0.0f, add = 0.0f;
-    f32x4 o[EV];
-#pragma unroll
-    for (int t = 0; t < EV; ++t) o[t] = f32x4{};
-
     const int32_t* row = a.c.table + b * a.c.table_row;
-    // Asks for the rows of 32 keys from k0 on.  Those of no token are read from
-    // wherever is safe: what they hold never shows.
-    auto load = [&](int32_t k0, Tile4<KS>* x) {
+    // Where the pages of 32 keys from k0 on are (P16: of 16 keys and of the next 16).
+    struct Pages {
+      int32_t page[2], slot[2];
+    };
+    auto find = [&](int32_t k0) {
+      Pages x;
+#pragma unroll
+      for (int u = 0; u < (P16 ? 2 : 1); ++u) {
+        const uint32_t key = P16 ? k0 + 16 * u : k0 + (lane & 31), size = a.c.page_size;
+        const uint32_t e = a.c.page_shift >= 0 ? key >> a.c.page_shift : key / size;
+        x.slot[u] = static_cast<int32_t>(key - e * size);
+        x.page[u] = -1;
+        if (key < static_cast<uint32_t>(end)) {
+          if constexpr (P16) x.page[u] = load_scalar(row + e);
+          else x.page[u] = row[e];
+        }
+      }
+      return x;
+    };
+    // Asks for the rows of 32 keys.  Those of no token are read from wherever is
+    // safe: what they hold never shows.
+    auto load = [&](int32_t k0, const Pages& at, Tile4<KS>* x) {
       if constexpr (P16) {
         // 16 keys from a multiple of 16 are in one page: addresses are the wave's.
         const char *ka[2], *va[2];
         x->seen = 0;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const int32_t key = k0 + 16 * u;
-          const uint32_t size = a.c.page_size;
-          const uint32_t e = a.c.page_shift >= 0 ? static_cast<uint32_t>(key) >> a.c.page_shift : key / size;
-          const int32_t slot = key - e * size;
-          int32_t page = key < end ? load_scalar(row + e) : -1;
-          const bool there = page >= 0 && page < a.c.pages;
-          page = there ? page : 0;
-          const int left = end - key;
+          const bool there = at.page[u] >= 0 && at.page[u] < pages;
+          const uint32_t page = there ? at.page[u] : 0, slot = there ? at.slot[u] : 0;
+          const int left = end - (k0 + 16 * u);
           x->seen |= there ? (left >= 16 ? 0xffffu : (1u << left) - 1u) << (16 * u) : 0u;
-          ka[u] = kb + page * a.c.k_page + (there ? slot : 0) * a.c.k_slot;
-          va[u] = vb + page * a.c.v_page + (there ? slot : 0) * a.c.v_slot;
+          ka[u] = kb + static_cast<uint64_t>(page) * k_page + slot * k_slot;
+          va[u] = vb + static_cast<uint64_t>(page) * v_page + slot * v_slot;
         }
         const char* t = g == 0 ? ka[0] : g == 1 ? ka[1] : g == 2 ? va[0] : va[1];
         x->tail = *reinterpret_cast<const uint32_t*>(t + tail_at);
@@ -187,14 +206,11 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? 2 : WAVES / 
           for (int i = 0; i < 4; ++i) x->v[4 * u + i] = load_codes<EV>(va[u] + v_at[i]);
         }
       } else {
-        const uint32_t key = k0 + (lane & 31), size = a.c.page_size;
-        const uint32_t e = a.c.page_shift >= 0 ? key >> a.c.page_shift : key / size;
-        const int64_t page = key < static_cast<uint32_t>(end) ? row[e] : -1;
-        const bool there = page >= 0 && page < a.c.pages;
+        const bool there = at.page[0] >= 0 && at.page[0] < pages;
         x->seen = static_cast<uint32_t>(__ballot(there));
-        const int32_t slot = key - e * size;
-        const int64_t koff = there ? page * a.c.k_page + slot * a.c.k_slot : 0;
-        const int64_t voff = there ? page * a.c.v_page + slot * a.c.v_slot : 0;
+        const uint32_t page = there ? at.page[0] : 0, slot = there ? at.slot[0] : 0;
+        const int64_t koff = static_cast<uint64_t>(page) * k_page + slot * k_slot;
+        const int64_t voff = static_cast<uint64_t>(page) * v_page + slot * v_slot;
         x->tail = *reinterpret_cast<const uint32_t*>((lane < 32 ? kb + koff : vb + voff) + tail);
 #pragma unroll
         for (int u = 0; u < 2; ++u) load_words<KS>(kb + shfl64(koff, 16 * u + r) + word0 * 4, x->k[u]);
@@ -203,42 +219,93 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? 2 : WAVES / 
           x->v[i] = load_codes<EV>(vb + shfl64(voff, 16 * (i / 4) + 4 * g + i % 4) + column);
       }
     };
+    // A tile's rows are asked for one tile ahead, their pages two.
+    int32_t k0 = t0 * kTile + wave * kStepKeys;
+    Tile4<KS> x0, x1;
+    Pages at_page = find(k0);
+    if (k0 < end) load(k0, at_page, &x0);
+    at_page = find(k0 + kTile);
+
+    // Queries in the codes' order.  A row's end may cut its quarters short: they
+    // begin early enough then, and what another quarter has too meets zeros.
+    f16x8 qf[KS];
+    f32x4 total{}, offset{};
+    float qx[KS][8], largest = 0.0f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const typename E::x8 x = __builtin_bit_cast(typename E::x8, qw[s]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        qx[s][i] = static_cast<float>(x[(i >> 1) + 4 * (i & 1)]);
+        largest = fmaxf(largest, fabsf(qx[s][i]));
+      }
+    }
+    largest = fmaxf(largest, __shfl_xor(largest, 16, 64));
+    largest = fmaxf(largest, other_half(largest));
+    const float up = query_scale(largest), down = 1.0f / up;
+    const bool scaled = __any(up != 1.0f);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) qf[s][i] = static_cast<_Float16>(qx[s][i] * up * (i & 2 ? 0.0625f : 1.0f));
+      total = mfma(pattern(1.0f, 16.0f), qf[s], total);
+      offset = mfma(pattern(-kOffset, -kOffset16), qf[s], offset);
+    }
+    const float qsum = total[0] * down;  // of head r
+    float most_s = 0.0f;  // the largest |s| that p s may meet, times 2^es
+    int es = 0;
+    float m = -INFINITY, sum = 0.0f, add = 0.0f;
+    f32x4 o[EV];
+#pragma unroll
+    for (int t = 0; t < EV; ++t) o[t] = f32x4{};
+
     auto sum_up = [&](const Tile4<KS>& x) {
       const uint32_t seen = x.seen;
       {
         RowCodec<4, false> codec;
         codec.load(reinterpret_cast<const uint8_t*>(&x.tail));
+        const bool here = (seen >> (lane & 31)) & 1;
+        if (__any(here && lane >= 32 && fabsf(codec.scale) > most_s)) {
+          float big = here && lane >= 32 ? fabsf(codec.scale) : 0.0f;
+#pragma unroll
+          for (int d = 1; d < 64; d *= 2) big = fmaxf(big, __shfl_xor(big, d, 64));
+          // s < 2^(e + 1), and s 2^es < 128.  (A scale in fp16 is no subnormal here.)
+          const int e = static_cast<int>(__float_as_uint(big) >> 23) - 127;
+          most_s = ldexpf(1.0f, e + 1);
+          const float f = ldexpf(1.0f, 6 - e - es);
+#pragma unroll
+          for (int t = 0; t < EV; ++t) o[t] *= f;
+          es = 6 - e;
+        }
         const float f = __builtin_fmaf(8.0f, codec.scale, codec.bias);
-        sh_tail[wave][lane >> 5][lane & 31] = (seen >> (lane & 31)) & 1 ? f32x2{codec.scale, f} : f32x2{};
+        const f32x2 tail = lane < 32 ? f32x2{codec.scale * c2, f * c2} : f32x2{ldexpf(codec.scale, es), f};
+        sh_tail[wave][lane >> 5][lane & 31] = here ? tail : f32x2{};
       }
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
       f32x2 kt[8], vt[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int nk = 16 * (i / 4) + 4 * g + i % 4;
-        kt[i] = sh_tail[wave][0][nk];
-        vt[i] = sh_tail[wave][1][nk];
-      }
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-
-      f32x4 s[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) s[u] = f32x4{start, start, start, start};
+      for (int i = 0; i < 8; ++i) kt[i] = sh_tail[wave][0][16 * (i / 4) + 4 * g + i % 4];
+      f32x4 s[2] = {offset, offset};
 #pragma unroll
       for (int i = 0; i < KS; ++i)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const uint32_t w = x.k[u][i];
-          const bf16x8 c = __builtin_bit_cast(
-              bf16x8, i32x4{codes.two(w), codes.two(w >> 4), codes.two(w >> 8), codes.two(w >> 12)});
-          s[u] = mfma(c, qf[i], s[u]);
-          if constexpr (kSplit) s[u] = mfma(c, ql[i], s[u]);
+          const uint32_t w = x.k[u][i], w8 = w >> 8;
+          s[u] = mfma(__builtin_bit_cast(f16x8, i32x4{codes.two(w), codes.two16(w), codes.two(w8), codes.two16(w8)}),
+                      qf[i], s[u]);
         }
+      if (scaled) {
+        asm volatile("" ::: "memory");  // a branch
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s[i / 4][i % 4] = __builtin_fmaf(kt[i][0], s[i / 4][i % 4], kt[i][1] * qsum);
+        for (int u = 0; u < 2; ++u) s[u] *= down;
+      }
+      // Scores in base 2, less the maximum that runs along.
+      const float mc = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        s[i / 4][i % 4] = __builtin_fmaf(kt[i][0], s[i / 4][i % 4], __builtin_fmaf(kt[i][1], qsum, -mc));
       if (seen != 0xffffffffu) {
         asm volatile("" ::: "memory");  // a branch: hardly any tile comes here
 #pragma unroll
@@ -249,35 +316,37 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? 2 : WAVES / 
       }
       float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                         fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-      if (__any((top - m) * c2 > 8.0f)) {
+      if (__any(top > (m == -INFINITY ? -INFINITY : 8.0f))) {
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, other_half(top));
-        const float m2 = fmaxf(m, top);
-        const float f = m2 == -INFINITY ? 1.0f : exp2_hw((m - m2) * c2);
+        const float m2 = fmaxf(m, top + mc);
+        const float f = m2 == -INFINITY ? 1.0f : exp2_hw(m - m2), less = m2 == -INFINITY ? 0.0f : mc - m2;
         sum *= f;
         add *= f;
 #pragma unroll
         for (int t = 0; t < EV; ++t) o[t] *= f;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) s[u] += less;
         m = m2;
       }
-      const float mc = m == -INFINITY ? 0.0f : m * c2;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) vt[i] = sh_tail[wave][1][16 * (i / 4) + 4 * g + i % 4];
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
       f32x8 ps;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float e = exp2_hw(__builtin_fmaf(s[i / 4][i % 4], c2, -mc));
+        const float e = exp2_hw(s[i / 4][i % 4]);
         sum += e;
         add = __builtin_fmaf(e, vt[i][1], add);
         ps[i] = e * vt[i][0];
       }
-      const bf16x8 p = __builtin_convertvector(ps, bf16x8);
-      const bf16x8 pl = __builtin_convertvector(ps - __builtin_convertvector(p, f32x8), bf16x8);
-      const bf16x8 minus = splat(-kOffset);
+      const f16x8 p = __builtin_convertvector(ps, f16x8);
+      const f16x8 minus = splat(-kOffset), minus16 = splat(-kOffset16);
 #pragma unroll
-      for (int t = 0; t < EV; ++t) o[t] = mfma(minus, p, o[t]);
-#pragma unroll
-      for (int t = 0; t < EV; ++t) o[t] = mfma(minus, pl, o[t]);
+      for (int t = 0; t < EV; ++t) o[t] = mfma(t & 1 ? minus16 : minus, p, o[t]);
       // Columns EV r + t of the eight keys, two to a word.
-      constexpr int kHalves = EV == 8 ? 2 : 1, kColumns = EV == 8 ? 4 : EV;
+      constexpr int kHalves = EV == 8 ? 2 : 1, kPairs = EV == 2 ? 1 : 2;
 #pragma unroll
       for (int h = 0; h < kHalves; ++h) {
         uint32_t w[4];
@@ -285,31 +354,30 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? 2 : WAVES / 
         for (int i = 0; i < 4; ++i)
           w[i] = __builtin_amdgcn_perm(x.v[2 * i + 1], x.v[2 * i], h == 0 ? 0x05040100u : 0x07060302u);
 #pragma unroll
-        for (int t = 0; t < kColumns; ++t) {
-          i32x4 c;
+        for (int t = 0; t < kPairs; ++t) {
+          i32x4 c, c16;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) c[i] = codes.two(w[i] >> (4 * t));
-          const bf16x8 y = __builtin_bit_cast(bf16x8, c);
-          o[4 * h + t] = mfma(y, p, o[4 * h + t]);
-          o[4 * h + t] = mfma(y, pl, o[4 * h + t]);
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t y = w[i] >> (8 * t);
+            c[i] = codes.two(y);
+            c16[i] = codes.two16(y);
+          }
+          f32x4 &even = o[4 * h + 2 * t], &odd = o[4 * h + 2 * t + 1];
+          even = mfma(__builtin_bit_cast(f16x8, c), p, even);
+          odd = mfma(__builtin_bit_cast(f16x8, c16), p, odd);
         }
       }
     };
-    // A tile's rows are asked for one tile ahead.
-    int32_t k0 = t0 * kTile + wave * kStepKeys;
-    if (k0 < end) {
-      Tile4<KS> x0, x1;
-      load(k0, &x0);
-      while (true) {
-        if (k0 + kTile < end) load(k0 + kTile, &x1);
-        sum_up(x0);
-        k0 += kTile;
-        if (k0 >= end) break;
-        if (k0 + kTile < end) load(k0 + kTile, &x0);
-        sum_up(x1);
-        k0 += kTile;
-        if (k0 >= end) break;
-      }
+    while (k0 < end) {
+      if (k0 + kTile < end) load(k0 + kTile, at_page, &x1);
+      at_page = find(k0 + 2 * kTile);
+      sum_up(x0);
+      k0 += kTile;
+      if (k0 >= end) break;
+      if (k0 + kTile < end) load(k0 + kTile, at_page, &x0);
+      at_page = find(k0 + 2 * kTile);
+      sum_up(x1);
+      k0 += kTile;
     }
 
     // The waves' sums: lane (r, g) holds head r, columns EV (4 g + i) + t.
@@ -321,31 +389,55 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? 2 : WAVES / 
       sh_m[wave][r] = m;
       sh_l[wave][r] = sum;
     }
+    const float even = ldexpf(1.0f, -es), odd = ldexpf(1.0f, -es - 4);
 #pragma unroll
     for (int t = 0; t < EV; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sh_o[wave][r][EV * (4 * g + i) + t] = o[t][i] + add;
+      for (int i = 0; i < 4; ++i)
+        sh_o[wave][r][EV * (4 * g + i) + t] = __builtin_fmaf(o[t][i], t & 1 ? odd : even, add);
     finish_block<T, WAVES, DP>(a, sh_o, sh_m, sh_l, worker, b, t0, t1, n, head0, heads);
-    if (!shared || stop <= n) return;  // a block per sequence never leaves its own
+    if (!shared || stop <= n + a.lead) return;  // a block per sequence never leaves its own
     // The next sequence that has tokens.
-    stop -= n;
+    stop -= n + a.lead;
     at = 0;
-    if (!next_sequence(a, &b, &len)) return;
+    if (!cursor.next(a)) return;
+    b = cursor.b, len = cursor.length();
     __syncthreads();
   }
 }
 
-// How a call's sequences are cut: as for the 16-bit cache.
+constexpr int wide_waves4(int D) { return D <= 32 ? 16 : 8; }  // by the registers
+
+// How a call's sequences are cut.  Times in us, of back-to-back calls.
+// - A block of four waves per sequence and head where no sequence has more than
+//   eight tiles (64 of up to 1024, 8 heads of 64: 14, wide blocks 15, shares 18; of 128: 18, 22, 23),
+//   or blocks are many and even out by themselves (1024 of up to 2048, 2 x 128: 86, in shares 97; 2048 of up
+//   to 1000, 4 x 64: 75, in shares 133).
+// - A wide block per sequence and head where blocks are too few to fill the chip
+//   and sequences short (16 of 1024, 8 x 64: 9.1, blocks of four waves 12.7, shares 14.1).
+// - Else equal shares of all tiles, two blocks for every CU (three up to D 64, where
+//   the registers allow it), and a second launch that joins them (256 of up to 8192
+//   by their logarithm, 8 x 128: 78, a block per sequence 122; 256 of 8192 each, 8 x 64: 271, a block per
+//   sequence 259: the host does not know lengths).
 struct Plan {
   int32_t workers;  // 0: a block per sequence and head
   bool wide;
 };
 
+// What a sequence's beginning costs a share, in tiles: us for 64 sequences of 64 to 4096
+// (32 heads of 128 over 8) with none, 1, 2, 3, 4 and 6: 48.3, 45.8, 44.3, 43.9, 44.7, 46.7; for 256 of up
+// to 8192 by their logarithm (16 over 8) 98, 84, 78, 79, 83, 89.
+constexpr int32_t kLead = 2;
+
 Plan plan_step(int64_t B, int32_t heads, int32_t D, int64_t most) {
   const int64_t tiles = ceil_div(most, kTileKeys), blocks = B * heads, cus = num_cus();
-  if (tiles <= 1 || blocks >= 8 * cus) return {0, false};
-  if (most <= 2 * wide_waves(D) * kStepKeys && blocks <= 4 * cus) return {0, true};
-  const int64_t w = ceil_div(cus * 2, heads);
+  if (tiles <= 1) return {0, false};
+  if (blocks > cus) {
+    if (tiles <= 8 || (blocks >= 8 * cus && (tiles < 32 || B > 512))) return {0, false};
+  } else if (most <= 4 * wide_waves4(D) * kStepKeys) {
+    return {0, true};
+  }
+  const int64_t w = ceil_div(cus * (D <= 64 ? 3 : 2), heads);
   return {static_cast<int32_t>(w < B * tiles ? w : B * tiles), false};
 }
 
@@ -357,7 +449,7 @@ int launch_step(const StepArgs& a, hipStream_t s) {
   auto launch = [&](auto p16) {
     constexpr bool P16 = decltype(p16)::value;
     const dim3 grid(static_cast<unsigned>(blocks));
-    if (a.wide) step4_kernel<T, DP, wide_waves(DP), P16><<<grid, wide_waves(DP) * 64, 0, s>>>(a);
+    if (a.wide) step4_kernel<T, DP, wide_waves4(DP), P16><<<grid, wide_waves4(DP) * 64, 0, s>>>(a);
     else step4_kernel<T, DP, kStepWaves, P16><<<grid, kStepWaves * 64, 0, s>>>(a);
   };
   if (a.c.page_size % 16 == 0) launch(std::true_type{});
@@ -404,6 +496,10 @@ extern "C" int mx_paged_cache_attention_int4(const mx_paged_cache* cache, int32_
   MX_REQUIRE(H > 0 && H % Hkv == 0, "%d query heads are no multiple of %d key-value heads", H, Hkv);
   MX_REQUIRE(std::isfinite(scale) && scale > 0.0f, "scale must be positive and finite");
   MX_REQUIRE(lengths_bytes == 4 || lengths_bytes == 8, "lengths_bytes %d", lengths_bytes);
+  for (int64_t page : {cache->k_page_stride, cache->v_page_stride})
+    MX_REQUIRE(page < (1ll << 31), "a page's stride is %lld bytes, 2^31 or more", (long long)page);
+  for (int64_t slot : {cache->k_slot_stride, cache->v_slot_stride})
+    MX_REQUIRE(slot <= ((1ll << 31) - 1) / cache->page_size, "a page's slots reach 2^31 bytes or further");
   if (B == 0) return MX_OK;
   MX_REQUIRE(q != nullptr && q->data != nullptr && out != nullptr && lengths != nullptr &&
                  (cache->table != nullptr || cache->table_width == 0),
@@ -418,10 +514,10 @@ extern "C" int mx_paged_cache_attention_int4(const mx_paged_cache* cache, int32_
   a.lengths = lengths, a.lengths_bytes = lengths_bytes;
   a.B = static_cast<int32_t>(B), a.H = H, a.Hkv = Hkv, a.G = H / Hkv, a.D = D;
   a.head_blocks = head_blocks_of(H, Hkv);
-  a.scale = scale;
+  a.scale = scale, a.units = 1.0f;
   a.out = out;
   const Plan plan = plan_step(B, Hkv * a.head_blocks, D, cache->table_width * cache->page_size);
-  a.workers = plan.workers, a.wide = plan.wide;
+  a.workers = plan.workers, a.wide = plan.wide, a.lead = kLead;
   const size_t need = mx_paged_cache_attention_int4_workspace_bytes(cache, B, H, Hkv, D);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return mx::set_error(MX_EWORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);

@@ -67,7 +67,9 @@ struct StepArgs {
   int32_t head_blocks;     // of 16 query heads of a key-value head
   int32_t workers;         // per head block: they share all tiles; 0: a block per sequence
   int32_t wide;            // a block of 8 or 16 waves per sequence
+  int32_t lead;            // of a share: what beginning a sequence costs, in tiles
   float scale;
+  float units;             // of the running maximum, in base 2: scale log2(e), or 1
   void* out;               // [B, H, D]
   float* part;             // [workers, 2, H, D + 2]: sums, then maximum and sum of weights
 };
@@ -88,24 +90,28 @@ __device__ __forceinline__ int32_t tiles_of(int32_t tokens) {
   return (tokens + WAVES * kStepKeys - 1) / (WAVES * kStepKeys);
 }
 
-// The sequences' tiles end to end are cut into equal shares, one for a worker
-// (and no more than tiles): share w begins at tile w total / shares.  A sequence's tiles may be cut anywhere;
+// The sequences' tiles end to end, each sequence's after `lead` units for its
+// beginning, are cut into equal shares, one for a worker (and no more than units):
+// share w begins at unit w total / shares.  A sequence's tiles may be cut anywhere;
 // what a share has of one that it does not have whole is joined later.  Shares
 // are equal whatever the lengths (a block per sequence waits for the longest).
 __device__ __forceinline__ int64_t share_begin(int64_t w, int64_t total, int64_t shares) {
   return w * total / shares;
 }
-__device__ __forceinline__ int64_t share_of(int64_t tile, int64_t total, int64_t shares) {
-  return ((tile + 1) * shares - 1) / total;
+__device__ __forceinline__ int64_t share_of(int64_t unit, int64_t total, int64_t shares) {
+  return ((unit + 1) * shares - 1) / total;
+}
+__device__ __forceinline__ int32_t units_of(const StepArgs& a, int32_t tokens) {
+  return tokens > 0 ? tiles_of(tokens) + a.lead : 0;
 }
 
-// Tiles of all sequences, and of those before `b`.
-__device__ __forceinline__ int64_t count_tiles(const StepArgs& a, int32_t b, int64_t* before) {
+// Units of all sequences, and of those before `b`.
+__device__ __forceinline__ int64_t count_units(const StepArgs& a, int32_t b, int64_t* before) {
   int64_t all = 0, prior = 0;
   for (int32_t i0 = 0; i0 < a.B; i0 += 64) {
     const int32_t i = i0 + lane_id();
-    const int32_t n = i < a.B ? tiles_of(tokens_of(a, i)) : 0;
-    // 64 sequences of less than 2^24 tiles each.
+    const int32_t n = i < a.B ? units_of(a, tokens_of(a, i)) : 0;
+    // 64 sequences of less than 2^24 units each.
     all += readlane_i32(wave_prefix(n), 63);
     if (i0 < b) prior += readlane_i32(wave_prefix(i < b ? n : 0), 63);
   }
@@ -113,20 +119,48 @@ __device__ __forceinline__ int64_t count_tiles(const StepArgs& a, int32_t b, int
   return all;
 }
 
-// The share of `worker`: tiles [at, stop) counted from the first one of sequence b,
-// which has `len` tokens.  False if there are fewer shares.
-__device__ __forceinline__ bool find_share(const StepArgs& a, int worker, int32_t* b, int32_t* len, int64_t* at,
-                                           int64_t* stop) {
+// A wave's place among the sequences: sequence b, and in lane i the tokens of
+// sequence base + i (so that the next one costs no trip to memory).
+struct Cursor {
+  int32_t b, base, tokens;
+
+  __device__ __forceinline__ void read(const StepArgs& a, int32_t from) {
+    base = from;
+    const int32_t i = base + lane_id();
+    tokens = i < a.B ? tokens_of(a, i) : 0;
+  }
+  __device__ __forceinline__ int32_t length() const { return readlane_i32(tokens, b - base); }
+
+  // On to the next sequence that has tokens; false if there is none.
+  __device__ __forceinline__ bool next(const StepArgs& a) {
+    int32_t from = b + 1;
+    while (true) {
+      const uint64_t left = from - base < 64 ? __ballot(tokens > 0) >> (from - base) << (from - base) : 0;
+      if (left != 0) {
+        b = base + __builtin_ctzll(left);
+        return true;
+      }
+      from = base + 64;
+      if (from >= a.B) return false;
+      read(a, from);
+    }
+  }
+};
+
+// The share of `worker`: tiles [at, stop) counted from the first one of the cursor's
+// sequence (`at` may lie before it).  False if there are fewer shares, or this one
+// ends before a tile.
+__device__ __forceinline__ bool find_share(const StepArgs& a, int worker, Cursor* c, int64_t* at, int64_t* stop) {
   int64_t prior;
-  const int64_t total = count_tiles(a, 0, &prior);
+  c->read(a, 0);
+  const int64_t total = a.B <= 64 ? readlane_i32(wave_prefix(units_of(a, c->tokens)), 63) : count_units(a, 0, &prior);
   const int64_t shares = total < a.workers ? total : a.workers;  // none is empty
   if (worker >= shares) return false;
   int64_t from = share_begin(worker, total, shares), to = share_begin(worker + 1, total, shares);
-  *len = 0;
+  c->b = 0;
   for (int32_t i0 = 0; i0 < a.B; i0 += 64) {
-    const int32_t i = i0 + lane_id();
-    const int32_t tokens = i < a.B ? tokens_of(a, i) : 0;
-    const int32_t upto = wave_prefix(tiles_of(tokens));
+    if (i0 > 0) c->read(a, i0);
+    const int32_t upto = wave_prefix(units_of(a, c->tokens));
     const int32_t here = readlane_i32(upto, 63);
     if (from >= here) {
       from -= here;
@@ -134,25 +168,15 @@ __device__ __forceinline__ bool find_share(const StepArgs& a, int worker, int32_
       continue;
     }
     const int l = __builtin_ctzll(__ballot(from < upto));
-    *b = i0 + l;
-    *len = readlane_i32(tokens, l);
-    const int32_t skip = readlane_i32(upto, l) - tiles_of(*len);
+    c->b = i0 + l;
+    const int32_t skip = readlane_i32(upto, l) - tiles_of(readlane_i32(c->tokens, l));  // its lead is behind it
     from -= skip;
     to -= skip;
     break;
   }
   *at = from;
   *stop = to;
-  return true;
-}
-
-// The next sequence that has tokens; false if there is none.
-__device__ __forceinline__ bool next_sequence(const StepArgs& a, int32_t* b, int32_t* len) {
-  do {
-    ++*b;
-    *len = __builtin_amdgcn_readfirstlane(tokens_of(a, *b));
-  } while (*len == 0 && *b + 1 < a.B);
-  return *len != 0;
+  return to > 0;
 }
 
 // Joins what the block's waves have of sequence b's tiles [t0, t1) of n: the
@@ -162,7 +186,7 @@ __device__ __forceinline__ void finish_block(const StepArgs& a, const float (&sh
                                              const float (&sh_m)[WAVES][16], const float (&sh_l)[WAVES][16],
                                              int worker, int32_t b, int32_t t0, int32_t t1, int32_t n, int head0,
                                              int heads) {
-  const float c2 = a.scale * kLog2e;
+  const float c2 = a.units;
   __syncthreads();
   const bool whole = t0 == 0 && t1 == n;
   for (int u = threadIdx.x; u < heads * a.D; u += WAVES * 64) {
@@ -211,15 +235,16 @@ __global__ void __launch_bounds__(kJoinMost * 64) join_kernel(const StepArgs a) 
     return;
   }
   int64_t before;
-  const int64_t total = count_tiles(a, b, &before);
+  const int64_t total = count_units(a, b, &before);
   const int64_t all = total < a.workers ? total : a.workers;
+  before += a.lead;
   const int64_t w0 = share_of(before, total, all), w1 = share_of(before + n - 1, total, all);
   if (w0 == w1) return;
   const int shares = static_cast<int>(w1 - w0 + 1);
   const int waves = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = lane_id();
   const int from = shares * wave / waves, to = shares * (wave + 1) / waves;
-  const float c2 = a.scale * kLog2e;
+  const float c2 = a.units;
   float m = -INFINITY, l = 0.0f, x0 = 0.0f, x1 = 0.0f;
   auto place = [&](int s) {
     return a.part + (((w0 + s) * 2 + (s == 0 ? 1 : 0)) * a.H + head) * (a.D + 2);
