@@ -34,16 +34,16 @@ __device__ __forceinline__ int64_t page_of(const Cache& c, int64_t t, int* slot)
 // The last i of 0..B with offsets[i] <= row, or -1: 64 probes per step.
 __device__ __forceinline__ int64_t list_of_row(const void* offsets, int32_t bytes, int64_t B, int64_t row) {
   int64_t lo = 0, n = B + 1;
-  if (ld_index(offsets, bytes, 0) > row) return -1;
-  while (n > 1) {
+  do {
     const int64_t step = (n + 63) >> 6;
     const int64_t i = lo + lane_id() * step;
     const bool in = i < lo + n && ld_index(offsets, bytes, i) <= row;
     const int c = __popcll(__ballot(in));
-    const int64_t at = (c > 0 ? c - 1 : 0) * step;
+    if (c == 0) return -1;  // offsets[0] > row (a later step's first probe is known not to be)
+    const int64_t at = (c - 1) * step;
     lo += at;
     n = n - at < step ? n - at : step;
-  }
+  } while (n > 1);
   return uniform64(lo);
 }
 

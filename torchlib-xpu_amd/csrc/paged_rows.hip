@@ -172,6 +172,7 @@ __device__ __forceinline__ bool wave_tile(const RowsArgs& a, Tile1* t) {
 template <typename T, int GS, Kind KIND, bool ONE>
 __global__ void __launch_bounds__(kRowsWaves * 64) rows_kernel(const RowsArgs a) {
   using X4 = typename Quad<T>::type;
+  using X8 = typename Elem<T>::x8;
   constexpr int kGroups = 64 / GS;
   Tile1 w;
   if (!wave_tile(a, &w)) return;
@@ -199,7 +200,13 @@ __global__ void __launch_bounds__(kRowsWaves * 64) rows_kernel(const RowsArgs a)
       const char* s = which == 0 ? a.src[0] + (w.r0 + row) * a.src_row[0] + h * a.src_head[0]
                       : which == 1 ? a.src[1] + (w.r0 + row) * a.src_row[1] + h * a.src_head[1]
                                    : a.src[2] + (w.r0 + row) * a.src_row[2] + h * a.src_head[2];
-      const X4 xa = *reinterpret_cast<const X4*>(s + ea * 2), xb = *reinterpret_cast<const X4*>(s + eb * 2);
+      X4 xa, xb;
+      if (split) {
+        xa = *reinterpret_cast<const X4*>(s + ea * 2), xb = *reinterpret_cast<const X4*>(s + eb * 2);
+      } else {
+        const X8 v = *reinterpret_cast<const X8*>(s + u * 16);
+        xa = __builtin_shufflevector(v, v, 0, 1, 2, 3), xb = __builtin_shufflevector(v, v, 4, 5, 6, 7);
+      }
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[e] = static_cast<float>(xa[e]), x[4 + e] = static_cast<float>(xb[e]);
       if (turns) {
@@ -232,8 +239,12 @@ __global__ void __launch_bounds__(kRowsWaves * 64) rows_kernel(const RowsArgs a)
 #pragma unroll
         for (int e = 0; e < 4; ++e) wa |= codec.code(x[e]) << (4 * e), wb |= codec.code(x[4 + e]) << (4 * e);
         char* d = (which == 1 ? a.c.k + to + h * a.c.k_head : a.c.v + to + h * a.c.v_head);
-        *reinterpret_cast<uint16_t*>(d + ea / 2) = static_cast<uint16_t>(wa);
-        *reinterpret_cast<uint16_t*>(d + eb / 2) = static_cast<uint16_t>(wb);
+        if (split) {
+          *reinterpret_cast<uint16_t*>(d + ea / 2) = static_cast<uint16_t>(wa);
+          *reinterpret_cast<uint16_t*>(d + eb / 2) = static_cast<uint16_t>(wb);
+        } else {
+          *reinterpret_cast<uint32_t*>(d + u * 4) = wa | (wb << 16);
+        }
         if (u == 0) codec.store(reinterpret_cast<uint8_t*>(d) + a.D / 2);
       }
     }
@@ -244,8 +255,12 @@ __global__ void __launch_bounds__(kRowsWaves * 64) rows_kernel(const RowsArgs a)
       X4 ya, yb;
 #pragma unroll
       for (int e = 0; e < 4; ++e) ya[e] = static_cast<T>(x[e]), yb[e] = static_cast<T>(x[4 + e]);
-      *reinterpret_cast<X4*>(d + ea * 2) = ya;
-      *reinterpret_cast<X4*>(d + eb * 2) = yb;
+      if (split) {
+        *reinterpret_cast<X4*>(d + ea * 2) = ya;
+        *reinterpret_cast<X4*>(d + eb * 2) = yb;
+      } else {
+        *reinterpret_cast<X8*>(d + u * 16) = __builtin_shufflevector(ya, yb, 0, 1, 2, 3, 4, 5, 6, 7);
+      }
     }
   }
 }
