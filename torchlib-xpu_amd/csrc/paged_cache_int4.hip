@@ -98,9 +98,12 @@ __device__ __forceinline__ float query_scale(float largest) {
 // small (bf16 ones 2^25 below the head's largest are rounded).  p_j s_j is rounded
 // to fp16 (2^-11), times a power of two that keeps the largest s seen below 128
 // (p stays below 256): those of an s 2^21 times smaller than the largest lose bits.
+// For fp16 outputs what the rounding leaves is a second operand (rounded once, they
+// would be half as far off again as their own rounding makes them).
 template <typename T, int DP, int WAVES, bool P16>
 __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? (DP <= 64 ? 3 : 2) : WAVES / 4) step4_kernel(const StepArgs a) {
   using E = Elem<T>;
+  constexpr bool kSplit = E::kNarrow;
   constexpr int kTile = WAVES * kStepKeys;
   constexpr int KS = DP / 32;  // products along D of a score; words of codes per lane
   constexpr int EV = DP / 16;  // columns of V per lane
@@ -254,7 +257,7 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? (DP <= 64 ? 
     const float qsum = total[0] * down;  // of head r
     float most_s = 0.0f;  // the largest |s| that p s may meet, times 2^es
     int es = 0;
-    float m = -INFINITY, sum = 0.0f, add = 0.0f;
+    float m = -INFINITY, sum = 0.0f, add = 0.0f, over = 0.0f;
     f32x4 o[EV];
 #pragma unroll
     for (int t = 0; t < EV; ++t) o[t] = f32x4{};
@@ -273,6 +276,7 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? (DP <= 64 ? 
           const int e = static_cast<int>(__float_as_uint(big) >> 23) - 127;
           most_s = ldexpf(1.0f, e + 1);
           const float f = ldexpf(1.0f, 6 - e - es);
+          over *= f;
 #pragma unroll
           for (int t = 0; t < EV; ++t) o[t] *= f;
           es = 6 - e;
@@ -323,6 +327,7 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? (DP <= 64 ? 
         const float f = m2 == -INFINITY ? 1.0f : exp2_hw(m - m2), less = m2 == -INFINITY ? 0.0f : mc - m2;
         sum *= f;
         add *= f;
+        over *= f;
 #pragma unroll
         for (int t = 0; t < EV; ++t) o[t] *= f;
 #pragma unroll
@@ -342,6 +347,13 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? (DP <= 64 ? 
         ps[i] = e * vt[i][0];
       }
       const f16x8 p = __builtin_convertvector(ps, f16x8);
+      f16x8 rest{};
+      if constexpr (kSplit) {
+        const f32x8 r8 = ps - __builtin_convertvector(p, f32x8);
+        rest = __builtin_convertvector(r8, f16x8);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) over += r8[i];
+      }
       const f16x8 minus = splat(-kOffset), minus16 = splat(-kOffset16);
 #pragma unroll
       for (int t = 0; t < EV; ++t) o[t] = mfma(t & 1 ? minus16 : minus, p, o[t]);
@@ -365,6 +377,10 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? (DP <= 64 ? 
           f32x4 &even = o[4 * h + 2 * t], &odd = o[4 * h + 2 * t + 1];
           even = mfma(__builtin_bit_cast(f16x8, c), p, even);
           odd = mfma(__builtin_bit_cast(f16x8, c16), p, odd);
+          if constexpr (kSplit) {
+            even = mfma(__builtin_bit_cast(f16x8, c), rest, even);
+            odd = mfma(__builtin_bit_cast(f16x8, c16), rest, odd);
+          }
         }
       }
     };
@@ -390,6 +406,12 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? (DP <= 64 ? 
       sh_l[wave][r] = sum;
     }
     const float even = ldexpf(1.0f, -es), odd = ldexpf(1.0f, -es - 4);
+    if constexpr (kSplit) {  // what the second operands' sums hold besides e
+      over += __shfl_xor(over, 16, 64);
+      over += other_half(over);
+#pragma unroll
+      for (int t = 0; t < EV; ++t) o[t] -= over * (t & 1 ? kOffset16 : kOffset);
+    }
 #pragma unroll
     for (int t = 0; t < EV; ++t)
 #pragma unroll

@@ -153,11 +153,11 @@ __device__ __forceinline__ float group_max(float v) {
 constexpr int kRowsWaves = 4;
 
 // The wave's tile and slice; false if it has none.
-struct Tile1 {
+struct WaveTile {
   int64_t r0;
   int rows, slice;
 };
-__device__ __forceinline__ bool wave_tile(const RowsArgs& a, Tile1* t) {
+__device__ __forceinline__ bool wave_tile(const RowsArgs& a, WaveTile* t) {
   const int64_t w = uniform64(static_cast<int64_t>(blockIdx.x) * kRowsWaves + (threadIdx.x >> 6));
   if (w >= a.waves) return false;
   const int64_t tile = w / a.slices;
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(kRowsWaves * 64) rows_kernel(const RowsArgs a)
   using X4 = typename Quad<T>::type;
   using X8 = typename Elem<T>::x8;
   constexpr int kGroups = 64 / GS;
-  Tile1 w;
+  WaveTile w;
   if (!wave_tile(a, &w)) return;
   const Place mine = places<KIND, ONE>(a, w.r0, w.rows);
   const int lane = lane_id(), group = lane / GS, u = lane % GS;
@@ -271,7 +271,7 @@ template <typename T, int GS, Kind KIND, bool ONE>
 __global__ void __launch_bounds__(kRowsWaves * 64) gather_kernel(const RowsArgs a) {
   using X8 = typename Elem<T>::x8;
   constexpr int kGroups = 64 / GS;
-  Tile1 w;
+  WaveTile w;
   if (!wave_tile(a, &w)) return;
   const Place mine = places<KIND, ONE>(a, w.r0, w.rows);
   const int lane = lane_id(), group = lane / GS, u = lane % GS;
