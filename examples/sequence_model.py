@@ -6,9 +6,11 @@ user's list, and a loss on a vector of the next event; the backward updates the
 projection and, by the fused rowwise Adagrad, the table.  Serving: the users'
 histories fill a paged cache, then every new event costs one appended row and
 one pass over the user's own cache; the results are those of the attention over
-the whole lists.
+the whole lists.  With --positions queries and keys turn by their events'
+positions, in training and on the way into the cache; with --bits 4 the cache
+holds rows of 4 bits.
 
-    python examples/sequence_model.py [--users 64] [--events 200] [--steps 20]
+    python examples/sequence_model.py [--users 64] [--events 200] [--steps 20] [--positions] [--bits 4]
 """
 
 from __future__ import annotations
@@ -23,7 +25,7 @@ sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "torchlib-xpu_amd")
 
 import mx_fbgemm  # noqa: E402,F401  (registers torch.ops.fbgemm.* and torch.ops.mx_fbgemm.*)
 from mx_fbgemm import ComputeDevice, EmbeddingLocation, PoolingMode  # noqa: E402
-from mx_fbgemm.sequence_attention import PagedSequenceCache  # noqa: E402
+from mx_fbgemm.sequence_attention import PagedSequenceCache, rotary_table  # noqa: E402
 from mx_fbgemm.split_table_batched_embeddings_ops_training import (  # noqa: E402
     SplitTableBatchedEmbeddingBagsCodegen,
 )
@@ -32,7 +34,8 @@ from mx_fbgemm.split_table_batched_embeddings_ops_training import (  # noqa: E40
 class SequenceModel(torch.nn.Module):
     """One attention layer over one sequence feature's rows."""
 
-    def __init__(self, rows: int, dim: int = 64, heads: int = 4, kv_heads: int = 2, device="cuda"):
+    def __init__(self, rows: int, dim: int = 64, heads: int = 4, kv_heads: int = 2, device="cuda",
+                 positions: int = 0):
         super().__init__()
         self.heads, self.kv_heads, self.head_dim = heads, kv_heads, dim // heads * 2
         self.table = SplitTableBatchedEmbeddingBagsCodegen(
@@ -43,6 +46,8 @@ class SequenceModel(torch.nn.Module):
         width = (heads + 2 * kv_heads) * self.head_dim
         self.project = torch.nn.Linear(dim, width, bias=False, device=device)
         self.out = torch.nn.Linear(heads * self.head_dim, dim, bias=False, device=device)
+        # Angles of up to `positions` events (0: the model knows no positions).
+        self.register_buffer("rotary", rotary_table(positions, self.head_dim, device=device) if positions else None)
         self.register_buffer("targets", torch.randn(rows, dim, device=device))  # of each event
 
     def qkv(self, rows: torch.Tensor):
@@ -50,10 +55,14 @@ class SequenceModel(torch.nn.Module):
         x = self.project(rows).to(torch.bfloat16).view(rows.size(0), -1, self.head_dim)
         return x.split([self.heads, self.kv_heads, self.kv_heads], dim=1)
 
+    def attend(self, rows: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+        q, k, v = self.qkv(rows)
+        if self.rotary is not None:
+            q, k = (torch.ops.mx_fbgemm.jagged_rotary(x, offsets, self.rotary) for x in (q, k))
+        return torch.ops.mx_fbgemm.jagged_attention(q, k, v, offsets)
+
     def forward(self, ids: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
-        q, k, v = self.qkv(self.table(ids, offsets))
-        y = torch.ops.mx_fbgemm.jagged_attention(q, k, v, offsets)
-        return self.out(y.flatten(1).float())
+        return self.out(self.attend(self.table(ids, offsets), offsets).flatten(1).float())
 
 
 def synthetic_batch(users: int, events: int, rows: int, seed: int):
@@ -85,7 +94,7 @@ def train(model: SequenceModel, users: int, events: int, rows: int, steps: int) 
 
 
 @torch.no_grad()
-def serve(model: SequenceModel, users: int, events: int, rows: int, new: int):
+def serve(model: SequenceModel, users: int, events: int, rows: int, new: int, bits: int = 16):
     """Histories into the cache, then `new` events per user one at a time; the
     outputs of the new events, and those of attention over the whole lists."""
     ids, offsets = (x.cuda() for x in synthetic_batch(users, events, rows, 1))
@@ -93,7 +102,7 @@ def serve(model: SequenceModel, users: int, events: int, rows: int, new: int):
     counts = offsets.diff().tolist()
     cache = PagedSequenceCache(pages=sum(-(-(n + new) // 16) for n in counts), page_size=16,
                                heads=model.kv_heads, head_dim=model.head_dim, max_sequences=users,
-                               max_length=max(counts) + new)
+                               max_length=max(counts) + new, bits=bits, rotary=model.rotary)
     names = [cache.add() for _ in range(users)]
     q, k, v = model.qkv(model.table(ids, offsets))
     cache.append(names, counts, k, v)
@@ -101,13 +110,12 @@ def serve(model: SequenceModel, users: int, events: int, rows: int, new: int):
     steps = []
     for t in range(new):
         q, k, v = model.qkv(model.table(more[t], one_each))
-        cache.append(names, [1] * users, k, v)
+        q = cache.append(names, [1] * users, k, v, q)  # (turned, if the cache turns keys)
         steps.append(cache.attend(names, q).clone())
     # The same from the whole lists.
     lists = [torch.cat([ids[offsets[u]:offsets[u + 1]], more[:, u]]) for u in range(users)]
     whole = torch.tensor([0, *counts]).cumsum(0).cuda() + torch.arange(users + 1, device="cuda") * new
-    q, k, v = model.qkv(model.table(torch.cat(lists), whole))
-    y = torch.ops.mx_fbgemm.jagged_attention(q, k, v, whole)
+    y = model.attend(model.table(torch.cat(lists), whole), whole)
     at = whole[1:, None] - new + torch.arange(new, device="cuda")[None, :]
     return torch.stack(steps, 1), y[at]
 
@@ -119,12 +127,14 @@ def main() -> None:
     ap.add_argument("--rows", type=int, default=1000)
     ap.add_argument("--steps", type=int, default=20)
     ap.add_argument("--new", type=int, default=8)
+    ap.add_argument("--positions", action="store_true", help="rotate queries and keys by position")
+    ap.add_argument("--bits", type=int, choices=(16, 4), default=16, help="of the cache")
     a = ap.parse_args()
     torch.manual_seed(0)
-    model = SequenceModel(a.rows)
+    model = SequenceModel(a.rows, positions=a.events + a.new if a.positions else 0)
     losses = train(model, a.users, a.events, a.rows, a.steps)
     print(f"training loss {losses[0]:.4f} -> {losses[-1]:.4f} in {a.steps} steps")
-    got, want = serve(model, a.users, a.events, a.rows, a.new)
+    got, want = serve(model, a.users, a.events, a.rows, a.new, a.bits)
     off = float((got - want).float().norm() / want.float().norm())
     print(f"{a.new} served events of {a.users} users against the whole lists: {off:.1e} apart")
 

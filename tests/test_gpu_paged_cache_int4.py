@@ -215,3 +215,81 @@ def test_refusals(dev):
                  (q, kc, kc, table, n, 0.0), (q, kc, kc, table, n.float()), (q, kc[0], kc[0], table, n)]:
         with pytest.raises((RuntimeError, NotImplementedError)):
             OPS.paged_cache_attention(*args)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("lengths", [[90, 5], [2000, 33]])
+def test_rows_of_very_different_sizes_in_one_sequence(dev, dtype, lengths):
+    """Scales 2^-8 to 2^8 of each other among a sequence's values, the largest in the
+    middle: p s keeps its bits whichever comes first, and small values are not lost
+    where large ones get no weight."""
+    def values(which, b, n):
+        x = make((n, 2, 64), torch.float32, 3 * b + which)
+        if which == 0:
+            return x
+        size = 2.0 ** (16 * torch.rand(n, generator=torch.Generator().manual_seed(b)) - 8)
+        size[n // 2] = 2.0 ** 8
+        return x * size[:, None, None]
+    run(dev, lengths, 16, 4, 2, 64, dtype, values=values)
+    run(dev, lengths, 16, 4, 2, 64, dtype, values=values, scale=4.0)
+
+
+@pytest.mark.parametrize("dtype,large", [("float16", 60000.0), ("bfloat16", 1e20)])
+def test_heads_of_very_different_sizes(dev, dtype, large):
+    """A head whose queries do not fit beside its neighbours' (each has a power of two
+    of its own); its one winning token, the others' ordinary weights."""
+    q = make((2, 4, 64), torch.float32, 5)
+    q[:, 1] *= large / 4
+    q[:, 2] *= 1e-4
+    run(dev, [70, 600], 16, 4, 2, 64, dtype, q=q.clamp(-65000, 65000).to(getattr(torch, dtype)) if dtype == "float16"
+        else q.to(torch.bfloat16))
+
+
+def test_wide_pages_and_pages_that_no_multiple_of_16_has(dev):
+    """The same rows in pages of 16 (addresses by the wave) and of 24 (by the lanes):
+    the same bits."""
+    D, n = 128, [300, 77]
+    outs = []
+    rows = [[rows4(make((m, 2, D), torch.float32, 7 * w + m)) for m in n] for w in range(2)]
+    q = make((2, 4, D), "bfloat16", 3).to(dev)
+    for page in (16, 24, 48):
+        table, pages = page_table(n, page, width=-(-320 // page))
+        caches = [torch.zeros((pages, page, 2, D // 2 + 4), dtype=torch.uint8) for _ in range(2)]
+        for c, lists in zip(caches, rows):
+            for b, m in enumerate(n):
+                t = torch.arange(m)
+                c[table[b, t // page].long(), t % page] = lists[b]
+        outs.append(OPS.paged_cache_attention(q, caches[0].to(dev), caches[1].to(dev), table.to(dev),
+                                              torch.tensor(n, device=dev)))
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+def test_page_strides_past_31_bits_are_refused(dev):
+    """Strides are 32-bit numbers in the kernel: larger ones end at the host."""
+    kc = torch.zeros(1 << 10, dtype=torch.uint8, device=dev).as_strided((1, 2, 1, 20), (1 << 31, 20, 20, 1))
+    q = torch.zeros((1, 1, 32), dtype=torch.float16, device=dev)
+    table, n = torch.zeros((1, 1), dtype=torch.int32, device=dev), torch.ones(1, dtype=torch.int64, device=dev)
+    with pytest.raises(RuntimeError, match="2\\^31"):
+        OPS.paged_cache_attention(q, kc, kc, table, n)
+    kc = torch.zeros(1 << 10, dtype=torch.uint8, device=dev).as_strided((1, 1, 1, 20), (20, 1 << 31, 20, 1))
+    with pytest.raises(RuntimeError, match="2\\^31"):
+        OPS.paged_cache_attention(q, kc, kc, table, n)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lengths", [[70, 40], [3000, 40]])
+@pytest.mark.parametrize("where", ["k", "v", "q"])
+def test_nan_of_a_token_shows_in_its_sequence_alone(dev, D, lengths, where):
+    for at in (0, 33, lengths[0] - 1):
+        kc, vc, table, ks, vs = make_cache(lengths, 16, 2, D)
+        q = make((2, 4, D), "bfloat16", 1)
+        if where == "q":
+            q[0, 1, 5] = float("nan")
+        else:
+            c = kc if where == "k" else vc
+            c[int(table[0, at // 16]), at % 16, 0, -4:-2] = torch.tensor([float("nan")], dtype=torch.float16).view(torch.uint8)
+        out = OPS.paged_cache_attention(q.to(dev), kc.to(dev), vc.to(dev), table.to(dev), torch.tensor(lengths, device=dev)).cpu()
+        bad = torch.isnan(out[0]).all(-1)
+        assert bad.tolist() == ([False, True, False, False] if where == "q" else [True, True, False, False]), at
+        want, tol = attention4(q[1:].double().numpy(), ks[1:], vs[1:], D ** -0.5, "bfloat16")
+        check(out[1:].double().numpy(), want, tol, "the other sequence")

@@ -100,6 +100,16 @@ __device__ __forceinline__ float query_scale(float largest) {
 // (p stays below 256): those of an s 2^21 times smaller than the largest lose bits.
 // For fp16 outputs what the rounding leaves is a second operand (rounded once, they
 // would be half as far off again as their own rounding makes them).
+//
+// Bound: reading the cache (256 sequences of 8192, 16 heads of 128 over 4: 231 us, 4.9
+// TB/s, in bf16 220; the 16-bit cache 745); the issue of its instructions is close
+// behind (two waves a SIMD, 150 vector and 24 matrix instructions, in fp16 32, for 32 keys).  64 sequences
+// of 64 to 4096, 32 heads over 8: 44 us, 3.2 TB/s: 5 the join, the rest beginnings and ends
+// of sequences, 4 us each.  P16 (pages of a multiple of 16 tokens): the wave finds
+// addresses, else lanes do and pass them on.  Loads past the
+// caches are slower here (266 for 224): rows of 68 bytes share lines.
+// Three blocks a CU up to D 64; at 128 the registers would not hold it (spilled, 279
+// for 223 us).
 template <typename T, int DP, int WAVES, bool P16>
 __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? (DP <= 64 ? 3 : 2) : WAVES / 4) step4_kernel(const StepArgs a) {
   using E = Elem<T>;
@@ -330,8 +340,12 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? (DP <= 64 ? 
         over *= f;
 #pragma unroll
         for (int t = 0; t < EV; ++t) o[t] *= f;
+        // (At most 0, also where scores are so large that fp32 rounds the difference up.)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) s[u] += less;
+        for (int i = 0; i < 8; ++i) {
+          const float x = s[i / 4][i % 4] + less;
+          s[i / 4][i % 4] = x > 0.0f ? 0.0f : x;  // NaN stays
+        }
         m = m2;
       }
 #pragma unroll
