@@ -293,3 +293,36 @@ def test_nan_of_a_token_shows_in_its_sequence_alone(dev, D, lengths, where):
         assert bad.tolist() == ([False, True, False, False] if where == "q" else [True, True, False, False]), at
         want, tol = attention4(q[1:].double().numpy(), ks[1:], vs[1:], D ** -0.5, "bfloat16")
         check(out[1:].double().numpy(), want, tol, "the other sequence")
+
+
+@pytest.mark.parametrize("pattern", ["ragged", "empty first", "empty last", "one long", "alternating"])
+def test_shares_over_more_sequences_than_lanes(dev, pattern):
+    """Tables long enough for shares, sequences in several groups of 64: shares that
+    begin or end before a sequence's first tile, and sequences without tokens
+    wherever a share begins."""
+    B, long = 170, 2300
+    rng = np.random.default_rng(len(pattern))
+    n = rng.integers(1, 400, B)
+    if pattern == "empty first":
+        n[:70] = 0
+    elif pattern == "empty last":
+        n[-75:] = 0
+    elif pattern == "one long":
+        n[:] = 1
+    elif pattern == "alternating":
+        n[::2] = 0
+    n[100 if pattern != "empty last" else 20] = long
+    run(dev, [int(x) for x in n], 16, 2, 1, 32, "float16")
+
+
+@pytest.mark.parametrize("pattern", ["ragged", "ones", "empty around"])
+def test_shares_of_many_heads(dev, pattern):
+    """Fewer workers than sequences, and shares of a unit each."""
+    n = {"ragged": [1, 1500, 3, 0, 1100, 129, 128, 127], "ones": [1, 1, 1, 1],
+         "empty around": [0, 0, 1200, 0, 0, 7, 0]}[pattern]
+    run(dev, n, 16, 16, 8, 64, "bfloat16")
+    kc, vc, table, ks, vs = make_cache(n, 16, 8, 64, width=160)
+    q = make((len(n), 16, 64), "bfloat16", 3)
+    out = OPS.paged_cache_attention(q.to(dev), kc.to(dev), vc.to(dev), table.to(dev), torch.tensor(n, device=dev))
+    want, tol = attention4(q.double().numpy(), ks, vs, 64 ** -0.5, "bfloat16")
+    check(out.double().cpu().numpy(), want, tol, "out")
