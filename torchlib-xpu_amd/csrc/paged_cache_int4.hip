@@ -76,8 +76,8 @@ struct Tile4 {
   uint32_t k[2][KS], v[8], tail, seen;
 };
 
-// The tail of a head's range: a power of two by which its queries are scaled where
-// fp16 would not hold them (their sixteenths, too).
+// A power of two by which a head's queries are scaled where fp16 would not hold them
+// and their sixteenths (operands of the codes that read 16 c).
 __device__ __forceinline__ float query_scale(float largest) {
   if (!(largest > 0.0f) || (largest >= 0.0625f && largest < 8192.0f)) return 1.0f;
   const int e = static_cast<int>(__float_as_uint(largest) >> 23) - 127;  // subnormals: -127
@@ -102,16 +102,17 @@ __device__ __forceinline__ float query_scale(float largest) {
 // would be half as far off again as their own rounding makes them).
 //
 // Bound: reading the cache (256 sequences of 8192, 16 heads of 128 over 4: 231 us, 4.9
-// TB/s, in bf16 220; the 16-bit cache 745); the issue of its instructions is close
-// behind (two waves a SIMD, 150 vector and 24 matrix instructions, in fp16 32, for 32 keys).  64 sequences
-// of 64 to 4096, 32 heads over 8: 44 us, 3.2 TB/s: 5 the join, the rest beginnings and ends
-// of sequences, 4 us each.  P16 (pages of a multiple of 16 tokens): the wave finds
-// addresses, else lanes do and pass them on.  Loads past the
-// caches are slower here (266 for 224): rows of 68 bytes share lines.
-// Three blocks a CU up to D 64; at 128 the registers would not hold it (spilled, 279
-// for 223 us).
+// TB/s, in bf16 220; the 16-bit cache 742), the issue of instructions half of the
+// time (in fp16 230 vector and 32 matrix ones for 32 keys; in bf16 24 matrix ones).  64
+// sequences of 64 to 4096, 32 heads over 8: 44 us, 3.2 TB/s, of which 5 the join and
+// much of the rest beginnings and ends of sequences, 4 us each.  P16 (pages of a
+// multiple of 16 tokens): the wave finds addresses, else lanes do and pass them on.
+// Loads past the caches are slower here (266 for 224): rows of 68 bytes share lines.
+// Three blocks a CU up to D 64 (272 for 315 us, 256 of 8192, 8 heads); at 128 the
+// registers would not hold it (spilled, 279 for 223 us).
 template <typename T, int DP, int WAVES, bool P16>
-__global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? (DP <= 64 ? 3 : 2) : WAVES / 4) step4_kernel(const StepArgs a) {
+__global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? (DP <= 64 ? 3 : 2) : WAVES / 4)
+    step4_kernel(const StepArgs a) {
   using E = Elem<T>;
   constexpr bool kSplit = E::kNarrow;
   constexpr int kTile = WAVES * kStepKeys;
