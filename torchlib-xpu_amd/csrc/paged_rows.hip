@@ -16,6 +16,7 @@
 // writes rows.
 #include "paged_common.h"
 #include "row_codec.h"
+#include "token_of_row.h"
 
 namespace mx {
 namespace attn {
@@ -89,12 +90,11 @@ __device__ __forceinline__ Place place_of(const RowsArgs& a, int64_t b, int64_t 
   Place p{kNoList, -1, -1};
   if (b < 0 || b >= a.B || row >= a.N) return p;
   const int64_t start = a.starts != nullptr ? ld_index(a.starts, a.starts_bytes, b) : 0;
-  const int64_t i = row - ld_index(a.offsets, a.offsets_bytes, b), t = start + i;
-  const bool fine = start >= 0 && i >= 0 && t >= 0;
-  p.pos = fine && t < a.positions ? static_cast<int32_t>(t) : kNoAngle;
+  const int64_t t = token_of_row(start, row, ld_index(a.offsets, a.offsets_bytes, b));
+  p.pos = t >= 0 && t < a.positions ? static_cast<int32_t>(t) : kNoAngle;
   if constexpr (KIND != kRotate) {
     int slot;
-    const int64_t e = fine ? page_of(a.c, t, &slot) : a.c.width;
+    const int64_t e = t >= 0 ? page_of(a.c, t, &slot) : a.c.width;
     if (e < a.c.width && (a.pairs == 0 || p.pos >= 0)) {
       const int64_t page = a.c.table[b * a.c.table_row + e];
       if (page >= 0 && page < a.c.pages) {
