@@ -18,35 +18,39 @@ namespace {
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// Codes as fp16, two to an instruction: with the exponent of 1024 (ulp 1) set above
-// it, a code in bits 0..3 of a half reads 1024 + c, one in bits 4..7 1024 + 16 c.
+// e = c - 8 in fp16, two at a time and exact: with the exponent of 1024 (ulp 1) set
+// above it, a code in bits 0..3 of a half reads 1024 + c, one in bits 4..7 1024 + 16 c.
 // The compiler knows none of the constants, or it would take two instructions with
-// a literal each.
+// a literal each.  (Products on the codes as they stand, their offset taken off by
+// another product, save an instruction of two but leave the offset in the sums: on
+// 1024 + c, scores were off by 5e-4 and more for queries of mean 1; and on c as a subnormal number,
+// of which the matrix unit keeps fewer bits, small outputs by 2^-16 of the values.)
 struct Codes {
   uint32_t low, high, base;
+  f16x2 sixteenth;
   __device__ __forceinline__ Codes() {
     asm("s_mov_b32 %0, 0x000f000f" : "=s"(low));
     asm("s_mov_b32 %0, 0x00f000f0" : "=s"(high));
     asm("v_mov_b32 %0, 0x64006400" : "=v"(base));
+    uint32_t x;
+    asm("v_mov_b32 %0, 0x2c002c00" : "=v"(x));
+    sixteenth = __builtin_bit_cast(f16x2, x);
   }
-  __device__ __forceinline__ int two(uint32_t w) const { return static_cast<int>((w & low) | base); }
-  __device__ __forceinline__ int two16(uint32_t w) const { return static_cast<int>((w & high) | base); }
+  __device__ __forceinline__ int two(uint32_t w) const {
+    const f16x2 off = {-1032, -1032};
+    return __builtin_bit_cast(int, __builtin_bit_cast(f16x2, (w & low) | base) + off);
+  }
+  __device__ __forceinline__ int two16(uint32_t w) const {
+    const f16x2 off = {-72, -72};
+    return __builtin_bit_cast(int, __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (w & high) | base), sixteenth, off));
+  }
 };
-constexpr float kOffset = 1032.0f;    // 1024 + c - 1032 = c - 8
-constexpr float kOffset16 = 1152.0f;  // 1024 + 16 c - 1152 = 16 (c - 8)
-
-// Of a word's eight codes, in the order of the operands (0 4, 1 5, 2 6, 3 7), those
-// that read 16 c: the third, fourth, seventh and eighth.
-__device__ __forceinline__ f16x8 pattern(float c, float c16) {
-  const _Float16 x = static_cast<_Float16>(c), y = static_cast<_Float16>(c16);
-  return f16x8{x, x, y, y, x, x, y, y};
-}
-__device__ __forceinline__ f16x8 splat(float v) { return pattern(v, v); }
 
 // N values (2, 4, 8) of a row's codes, in a word's low bits.
 template <int EV>
@@ -76,40 +80,40 @@ struct Tile4 {
   uint32_t k[2][KS], v[8], tail, seen;
 };
 
-// A power of two by which a head's queries are scaled where fp16 would not hold them
-// and their sixteenths (operands of the codes that read 16 c).
-__device__ __forceinline__ float query_scale(float largest) {
-  if (!(largest > 0.0f) || (largest >= 0.0625f && largest < 8192.0f)) return 1.0f;
+// A power of two that brings a head's queries to where fp16 holds them with all their
+// bits, and the matrix unit too (of subnormal numbers it keeps fewer).  From 1 to 2^15
+// for the largest nothing is needed: what is rounded or cut then, below 2^-14, is off by
+// 2^-25 of the largest at most, less than fp32 sums keep beside its product.
+__device__ __forceinline__ int query_shift(float largest) {
+  if (!(largest > 0.0f) || (largest >= 1.0f && largest < 32768.0f)) return 0;
   const int e = static_cast<int>(__float_as_uint(largest) >> 23) - 127;  // subnormals: -127
-  return ldexpf(1.0f, e > 120 ? -120 : -e);
+  return 14 - e;
 }
 
 // One block: up to 16 query heads of one key-value head, and a share of its
 // tiles (or one sequence), as attention over a 16-bit cache; its waves take 32
 // of a tile's keys each.  Codes go straight into registers and become fp16
-// integers there (r = lane % 16, g = lane / 16): for the scores the lane has key
+// integers e there (r = lane % 16, g = lane / 16): for the scores the lane has key
 // r's g-th quarter of the row, for the second product DP / 16 columns of 8 keys,
-// which come out as one operand each of DP / 16 products.  The integers are
-// 1024 + c or 1024 + 16 c; minus that many times the other operand's sum starts
-// each product off, so that what is summed is e or 16 e, and no more than a tile's
-// offset ever stands in a sum.
+// which come out as one operand each of DP / 16 products.
 //
-// Queries are exact in fp16, by a power of two per head where they are large or
-// small (bf16 ones 2^25 below the head's largest are rounded).  p_j s_j is rounded
-// to fp16 (2^-11), times a power of two that keeps the largest s seen below 128
-// (p stays below 256): those of an s 2^21 times smaller than the largest lose bits.
-// For fp16 outputs what the rounding leaves is a second operand (rounded once, they
-// would be half as far off again as their own rounding makes them).
+// Queries are exact in fp16, by a power of two per head where they are large or small
+// (query_shift).  p_j s_j is rounded to fp16 (2^-11), times a power of two that
+// keeps the largest s seen below 128 (p stays below 256): those of an s 2^21 times
+// smaller than the largest lose bits.  For fp16 outputs what the rounding leaves is a
+// second operand (rounded once, they would be half as far off again as their own
+// rounding makes them).
 //
-// Bound: reading the cache (256 sequences of 8192, 16 heads of 128 over 4: 231 us, 4.9
-// TB/s, in bf16 220; the 16-bit cache 742), the issue of instructions half of the
-// time (in fp16 230 vector and 32 matrix ones for 32 keys; in bf16 24 matrix ones).  64
-// sequences of 64 to 4096, 32 heads over 8: 44 us, 3.2 TB/s, of which 5 the join and
+// Bound: reading the cache (256 sequences of 8192, 16 heads of 128 over 4: 245 us, 4.7
+// TB/s, in bf16 234; the 16-bit cache 742), the issue of instructions more than half of
+// the time (about 300 vector ones for 32 keys, 64 of them for e instead of codes, which
+// cost 10 of the 245 us; in fp16 24 matrix ones, in bf16 16).  64 sequences of 64 to
+// 4096, 32 heads over 8: 46 us, 3.1 TB/s, of which 5 the join and
 // much of the rest beginnings and ends of sequences, 4 us each.  P16 (pages of a
 // multiple of 16 tokens): the wave finds addresses, else lanes do and pass them on.
-// Loads past the caches are slower here (266 for 224): rows of 68 bytes share lines.
-// Three blocks a CU up to D 64 (272 for 315 us, 256 of 8192, 8 heads); at 128 the
-// registers would not hold it (spilled, 279 for 223 us).
+// Loads past the caches are slower here (by a fifth): rows of 68 bytes share lines.
+// Three blocks a CU up to D 64 (285 us for 256 of 8192, 8 heads; two took 315 and more);
+// at 128 the registers would not hold it (spilled, by a quarter slower).
 template <typename T, int DP, int WAVES, bool P16>
 __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? (DP <= 64 ? 3 : 2) : WAVES / 4)
     step4_kernel(const StepArgs a) {
@@ -135,6 +139,7 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? (DP <= 64 ? 
   const char* vb = a.c.v + kvh * a.c.v_head;
   const int words = a.D / 8, tail = a.D / 2;
   const Codes codes;
+  const f16x8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
   // Strides inside a page, and of a page, are below 2^31 bytes (checked by the host).
   const int32_t pages = static_cast<int32_t>(a.c.pages < 0x7fffffff ? a.c.pages : 0x7fffffff);
   const uint32_t k_page = static_cast<uint32_t>(a.c.k_page), v_page = static_cast<uint32_t>(a.c.v_page);
@@ -243,7 +248,7 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? (DP <= 64 ? 
     // Queries in the codes' order.  A row's end may cut its quarters short: they
     // begin early enough then, and what another quarter has too meets zeros.
     f16x8 qf[KS];
-    f32x4 total{}, offset{};
+    f32x4 total{};
     float qx[KS][8], largest = 0.0f;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
@@ -256,19 +261,18 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? (DP <= 64 ? 
     }
     largest = fmaxf(largest, __shfl_xor(largest, 16, 64));
     largest = fmaxf(largest, other_half(largest));
-    const float up = query_scale(largest), down = 1.0f / up;
-    const bool scaled = __any(up != 1.0f);
+    const int shift = query_shift(largest);
+    const bool scaled = __any(shift != 0);
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) qf[s][i] = static_cast<_Float16>(qx[s][i] * up * (i & 2 ? 0.0625f : 1.0f));
-      total = mfma(pattern(1.0f, 16.0f), qf[s], total);
-      offset = mfma(pattern(-kOffset, -kOffset16), qf[s], offset);
+      for (int i = 0; i < 8; ++i) qf[s][i] = static_cast<_Float16>(ldexpf(qx[s][i], shift));
+      total = mfma(ones, qf[s], total);
     }
-    const float qsum = total[0] * down;  // of head r
+    const float qsum = ldexpf(total[0], -shift);  // of head r
     float most_s = 0.0f;  // the largest |s| that p s may meet, times 2^es
     int es = 0;
-    float m = -INFINITY, sum = 0.0f, add = 0.0f, over = 0.0f;
+    float m = -INFINITY, sum = 0.0f, add = 0.0f;
     f32x4 o[EV];
 #pragma unroll
     for (int t = 0; t < EV; ++t) o[t] = f32x4{};
@@ -287,7 +291,6 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? (DP <= 64 ? 
           const int e = static_cast<int>(__float_as_uint(big) >> 23) - 127;
           most_s = ldexpf(1.0f, e + 1);
           const float f = ldexpf(1.0f, 6 - e - es);
-          over *= f;
 #pragma unroll
           for (int t = 0; t < EV; ++t) o[t] *= f;
           es = 6 - e;
@@ -302,7 +305,7 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? (DP <= 64 ? 
       f32x2 kt[8], vt[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) kt[i] = sh_tail[wave][0][16 * (i / 4) + 4 * g + i % 4];
-      f32x4 s[2] = {offset, offset};
+      f32x4 s[2] = {};
 #pragma unroll
       for (int i = 0; i < KS; ++i)
 #pragma unroll
@@ -314,7 +317,7 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? (DP <= 64 ? 
       if (scaled) {
         asm volatile("" ::: "memory");  // a branch
 #pragma unroll
-        for (int u = 0; u < 2; ++u) s[u] *= down;
+        for (int i = 0; i < 8; ++i) s[i / 4][i % 4] = ldexpf(s[i / 4][i % 4], -shift);
       }
       // Scores in base 2, less the maximum that runs along.
       const float mc = m == -INFINITY ? 0.0f : m;
@@ -338,7 +341,6 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? (DP <= 64 ? 
         const float f = m2 == -INFINITY ? 1.0f : exp2_hw(m - m2), less = m2 == -INFINITY ? 0.0f : mc - m2;
         sum *= f;
         add *= f;
-        over *= f;
 #pragma unroll
         for (int t = 0; t < EV; ++t) o[t] *= f;
         // (At most 0, also where scores are so large that fp32 rounds the difference up.)
@@ -366,12 +368,7 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? (DP <= 64 ? 
       if constexpr (kSplit) {
         const f32x8 r8 = ps - __builtin_convertvector(p, f32x8);
         rest = __builtin_convertvector(r8, f16x8);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) over += r8[i];
       }
-      const f16x8 minus = splat(-kOffset), minus16 = splat(-kOffset16);
-#pragma unroll
-      for (int t = 0; t < EV; ++t) o[t] = mfma(t & 1 ? minus16 : minus, p, o[t]);
       // Columns EV r + t of the eight keys, two to a word.
       constexpr int kHalves = EV == 8 ? 2 : 1, kPairs = EV == 2 ? 1 : 2;
 #pragma unroll
@@ -420,18 +417,11 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? (DP <= 64 ? 
       sh_m[wave][r] = m;
       sh_l[wave][r] = sum;
     }
-    const float even = ldexpf(1.0f, -es), odd = ldexpf(1.0f, -es - 4);
-    if constexpr (kSplit) {  // what the second operands' sums hold besides e
-      over += __shfl_xor(over, 16, 64);
-      over += other_half(over);
-#pragma unroll
-      for (int t = 0; t < EV; ++t) o[t] -= over * (t & 1 ? kOffset16 : kOffset);
-    }
+    const float unit = ldexpf(1.0f, -es);
 #pragma unroll
     for (int t = 0; t < EV; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        sh_o[wave][r][EV * (4 * g + i) + t] = __builtin_fmaf(o[t][i], t & 1 ? odd : even, add);
+      for (int i = 0; i < 4; ++i) sh_o[wave][r][EV * (4 * g + i) + t] = __builtin_fmaf(o[t][i], unit, add);
     finish_block<T, WAVES, DP>(a, sh_o, sh_m, sh_l, worker, b, t0, t1, n, head0, heads);
     if (!shared || stop <= n + a.lead) return;  // a block per sequence never leaves its own
     // The next sequence that has tokens.
