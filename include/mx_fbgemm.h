@@ -695,6 +695,9 @@ int mx_paged_cache_attention(const mx_paged_cache* cache, int32_t dtype,
  * bias in fp16; value = scale * code + bias.  A head's row is quantized as
  * mx_quantize_fused_nbit_rowwise does it: bias the row's smallest value in fp16, scale
  * (largest - bias) / 15 in fp16 (1 where that is 0), codes rounded to nearest.
+ * A row with a NaN among its values has codes 0 and NaN as scale and bias; one with an
+ * infinity, a smallest value below -65504 or a range past 15 times 65504 reads back
+ * as NaN too.
  * mx_paged_cache's strides count bytes then (multiples of 4), and k and v are
  * 4-byte aligned. */
 

@@ -68,3 +68,76 @@ def test_offsets_below_every_row(dev, first):
     kc[..., -4:] = 1
     k, v = OPS.paged_cache_gather(kc, kc, table, off, 6, torch.float16)
     assert torch.count_nonzero(k) == 0 and torch.count_nonzero(v) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [8, 40, 64, 96, 128])
+@pytest.mark.parametrize("rotary", [False, True])
+def test_nan_of_an_element_is_its_heads_row(dev, dtype, D, rotary):
+    """A 4-bit row has no code for NaN: the head's whole row is NaN (scale and bias,
+    codes 0), where a 16-bit cache shows the element.  Other heads' and tokens' rows
+    are those of the same values without it."""
+    n, Hkv = D + 2, 3
+    k, v = (make((n, Hkv, D), dtype, s).to(dev) for s in (1, 2))
+    bad_k, bad_v = k.clone(), v.clone()
+    for i in range(D):
+        bad_k[i, 1, i] = float("nan")
+        bad_v[i, 2, D - 1 - i] = float("nan")
+    bad_k[D, 0] = float("nan")
+    page = 16
+    pages = -(-n // page)
+    table = torch.arange(pages, dtype=torch.int32, device=dev).view(1, pages)
+    off, zero, t = torch.tensor([0, n], device=dev), torch.tensor([0], device=dev), angles(n, D).to(dev)
+
+    def append(k, v):
+        kc, vc = (torch.zeros((pages, page, Hkv, D // 2 + 4), dtype=torch.uint8, device=dev) for _ in range(2))
+        if rotary:
+            OPS.paged_cache_append_rotary(None, k, v, off, zero, t, kc, vc, table)
+        else:
+            OPS.paged_cache_append(k, v, off, zero, kc, vc, table)
+        return kc, vc
+
+    got, want = append(bad_k, bad_v), append(k, v)
+    read = OPS.paged_cache_gather(*got, table, off, n, torch.bfloat16)
+    for c, w, x, r in zip(got, want, (bad_k, bad_v), read):
+        bad = torch.isnan(x).any(-1)
+        c, w = (y.view(-1, Hkv, D // 2 + 4)[:n] for y in (c, w))
+        assert torch.equal(c[~bad], w[~bad])
+        assert torch.count_nonzero(c[bad][:, :-4]) == 0
+        assert torch.isnan(c[bad][:, -4:].contiguous().view(torch.float16)).all()
+        assert torch.equal(torch.isnan(r), bad[..., None].expand_as(r))
+    # And attention shows it, in the heads that read it.
+    q = make((1, 2 * Hkv, D), dtype, 3).to(dev)
+    out = OPS.paged_cache_attention(q, *got, table, torch.tensor([n - 1], device=dev))
+    assert torch.isnan(out).all()
+    out = OPS.paged_cache_attention(q, got[0], want[1], table, torch.tensor([D], device=dev))
+    assert torch.isnan(out[0]).all(-1).tolist() == [False, False, True, True, False, False]
+    assert torch.isnan(out[0]).any(-1).tolist() == [False, False, True, True, False, False]
+
+
+@pytest.mark.parametrize("dtype,value", [(torch.float16, float("inf")), (torch.float16, -float("inf")),
+                                         (torch.bfloat16, float("inf")), (torch.bfloat16, -float("inf")),
+                                         (torch.bfloat16, -70000.0), (torch.bfloat16, 1.5e6), (torch.bfloat16, 3e38)])
+def test_what_fp16_does_not_hold_reads_back_as_nan(dev, dtype, value):
+    """Infinities, a smallest value below fp16's range, and a range whose fifteenth is past it."""
+    D = 32
+    x = make((2, 1, D), dtype, 1).to(dev)
+    x[0, 0, 5] = value
+    kc = torch.zeros((1, 2, 1, D // 2 + 4), dtype=torch.uint8, device=dev)
+    vc, table, off = kc.clone(), torch.zeros((1, 1), dtype=torch.int32, device=dev), torch.tensor([0, 2], device=dev)
+    OPS.paged_cache_append(x, x, off, off[:1], kc, vc, table)
+    k, v = OPS.paged_cache_gather(kc, vc, table, off, 2, torch.bfloat16)
+    assert torch.isnan(k[0]).all() and torch.isnan(v[0]).all() and torch.isfinite(k[1]).all()
+    q = make((1, 1, D), dtype, 2).to(dev)
+    assert torch.isnan(OPS.paged_cache_attention(q, kc, vc, table, torch.tensor([2], device=dev))).all()
+
+
+def test_values_past_fp16_whose_range_it_holds(dev):
+    x = make((1, 1, 32), torch.bfloat16, 1).to(dev)
+    x[0, 0, 5] = 90112.0  # a scale of 6,000: 15 steps reach it
+    kc = torch.zeros((1, 1, 1, 20), dtype=torch.uint8, device=dev)
+    table, off = torch.zeros((1, 1), dtype=torch.int32, device=dev), torch.tensor([0, 1], device=dev)
+    OPS.paged_cache_append(x, x, off, off[:1], kc, kc.clone(), table)
+    k, _ = OPS.paged_cache_gather(kc, kc, table, off, 1, torch.bfloat16)
+    # Scale and bias are rounded to fp16 (2^-11), the value to bf16 (2^-8).
+    assert abs(float(k[0, 0, 5]) - 90112.0) <= 90112.0 * (2 ** -10 + 2 ** -8) and torch.isfinite(k).all()

@@ -13,7 +13,7 @@
 //
 // A row of a 4-bit cache is D / 2 bytes of codes (the even element in the low
 // half), fp16 scale, fp16 bias: value = scale code + bias, as the 4-bit codec op
-// writes rows.
+// writes rows; but for values that hold a NaN, whose row is NaN in scale and bias.
 #include "paged_common.h"
 #include "row_codec.h"
 #include "token_of_row.h"
@@ -232,12 +232,16 @@ __global__ void __launch_bounds__(kRowsWaves * 64) rows_kernel(const RowsArgs a)
     if (KIND == kAppend4) {
       // All lanes of the group hold one head's values (or none do).
       float lo = INFINITY, hi = -INFINITY;
+      bool nan = false;
       if (live) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) lo = fminf(lo, x[e]), hi = fmaxf(hi, x[e]);
+        for (int e = 0; e < 8; ++e) lo = fminf(lo, x[e]), hi = fmaxf(hi, x[e]), nan |= __builtin_isnan(x[e]);
       }
       lo = group_min<GS>(lo);
       hi = group_max<GS>(hi);
+      // A code cannot say NaN, and the minimum and maximum pass over it: the head's whole row
+      // is one, by its scale and bias.
+      if ((__ballot(nan) >> (group * GS)) & ((1ull << GS) - 1)) lo = hi = NAN;
       if (live && which > 0) {
         RowCodec<4, false> codec;
         codec.set(lo, hi);

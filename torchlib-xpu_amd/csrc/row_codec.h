@@ -39,7 +39,7 @@ struct RowCodec {
   __device__ __forceinline__ uint32_t code(float x) const {
     float q = __builtin_rintf(__fmul_rn(x - bias, inv));
     if constexpr (FUSED8) return static_cast<uint8_t>(q);
-    q = q < 0.0f ? 0.0f : (q > static_cast<float>(kMax) ? static_cast<float>(kMax) : q);
+    q = q > 0.0f ? (q > static_cast<float>(kMax) ? static_cast<float>(kMax) : q) : 0.0f;  // NaN: 0
     return static_cast<uint32_t>(q);
   }
   __device__ __forceinline__ void store(uint8_t* o) const {

@@ -47,7 +47,7 @@ class PagedSequenceCache:
     scale and fp16 bias, as the 4-bit codec writes it (uint8 [pages, page_size,
     heads, head_dim / 2 + 4], a page's rows of one head next to each other): 3.8
     times the events in the same memory.  Rows come and queries go in ``dtype`` as
-    before; values past fp16's range do not fit.
+    before; a row with a value below fp16's range, or one that is no number, is NaN whole.
 
     With ``rotary`` (a table as ``rotary_table`` makes it, of ``max_length``
     positions at least) keys turn by their positions on the way in, and so do the
