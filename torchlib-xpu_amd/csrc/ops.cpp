@@ -2242,6 +2242,18 @@ void bump_versions(const Tensor& k_cache, const Tensor& v_cache) {
     if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();  // (inference tensors keep none)
 }
 
+// What goes into a cache or comes out of one has no derivative, of either direction:
+// it would be cut without a word.
+void refuse_derivatives(std::initializer_list<const Tensor*> inputs, const char* op) {
+  const bool forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  for (const Tensor* t : inputs) {
+    if (!t->defined()) continue;
+    TORCH_CHECK_NOT_IMPLEMENTED(!forward || !t->_fw_grad(0).defined(), op, " has no forward-mode derivative");
+    TORCH_CHECK(!at::GradMode::is_enabled() || !t->requires_grad(), op,
+                " has no gradient: call it under torch.no_grad()");
+  }
+}
+
 // The append as autograd sees it.
 void paged_cache_append_inplace(const Tensor& k, const Tensor& v, const Tensor& offsets, const Tensor& starts,
                                 const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table) {
@@ -2390,9 +2402,8 @@ Tensor paged_cache_append_rotary_inplace(const std::optional<Tensor>& q, const T
                                          const Tensor& offsets, const Tensor& starts, const Tensor& table,
                                          const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table,
                                          bool interleaved) {
-  // The rotated queries would come back without their graph.
-  TORCH_CHECK(!at::GradMode::is_enabled() || !(q.has_value() && q->defined() && q->requires_grad()),
-              "paged_cache_append_rotary has no gradient: call it under torch.no_grad(), or jagged_rotary");
+  Tensor none;
+  refuse_derivatives({&(q.has_value() ? *q : none), &k, &v, &table}, "paged_cache_append_rotary");
   Tensor out;
   {
     at::AutoDispatchBelowADInplaceOrView g;
@@ -2456,6 +2467,14 @@ std::tuple<Tensor, Tensor> paged_cache_gather(const Tensor& k_cache, const Tenso
                                 index_bytes_of(offsets, "offsets"), k.data_ptr(), v.data_ptr(),
                                 stream_of(k_cache)));
   return {k, v};
+}
+
+std::tuple<Tensor, Tensor> paged_cache_gather_autograd(const Tensor& k_cache, const Tensor& v_cache,
+                                                       const Tensor& page_table, const Tensor& offsets, int64_t total,
+                                                       std::optional<at::ScalarType> dtype) {
+  refuse_derivatives({&k_cache, &v_cache}, "paged_cache_gather");
+  at::AutoDispatchBelowADInplaceOrView g;
+  return paged_cache_gather(k_cache, v_cache, page_table, offsets, total, dtype);
 }
 
 }  // namespace mx_ops
@@ -2745,4 +2764,5 @@ TORCH_LIBRARY_IMPL(mx_fbgemm, Autograd, m) {
   m.impl("jagged_attention", TORCH_FN(mx_ops::jagged_attention_autograd));
   m.impl("jagged_rotary", TORCH_FN(mx_ops::jagged_rotary_autograd));
   m.impl("jagged_rotary_backward", TORCH_FN(mx_ops::jagged_rotary_backward_autograd));
+  m.impl("paged_cache_gather", TORCH_FN(mx_ops::paged_cache_gather_autograd));
 }
