@@ -83,7 +83,9 @@ class PagedSequenceCache:
             if rotary.size(0) < max_length:
                 raise ValueError(f"rotary has {rotary.size(0)} positions for sequences of {max_length}")
         self.page_size, self.max_length, self.dtype, self.bits = page_size, max_length, dtype, bits
-        self._rotary, self._interleaved = rotary, interleaved
+        # A view along the pairs is laid out here once, not in every call.
+        self._rotary = rotary.contiguous() if rotary is not None else None
+        self._interleaved = interleaved
 
         def tensor() -> torch.Tensor:
             if bits == 16:
