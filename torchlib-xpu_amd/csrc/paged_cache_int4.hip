@@ -5,7 +5,7 @@
 // so that over the tokens j of a sequence
 //   score_j = scale (s_j (q . e_j) + f_j sum(q)),
 //   out = sum_j p_j s_j e_j + sum_j p_j f_j,   p = softmax(score):
-// the matrix products run on the codes themselves, scale and bias enter once per
+// the matrix products run on the small integers e, scale and bias enter once per
 // token.
 #include <type_traits>
 
@@ -28,9 +28,10 @@ __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
 // above it, a code in bits 0..3 of a half reads 1024 + c, one in bits 4..7 1024 + 16 c.
 // The compiler knows none of the constants, or it would take two instructions with
 // a literal each.  (Products on the codes as they stand, their offset taken off by
-// another product, save an instruction of two but leave the offset in the sums: on
-// 1024 + c, scores were off by 5e-4 and more for queries of mean 1; and on c as a subnormal number,
-// of which the matrix unit keeps fewer bits, small outputs by 2^-16 of the values.)
+// another product, save one instruction of two but leave the offset in the sums: on
+// 1024 + c, scores were off by 5e-4 and more for queries of mean 1.  On c as a
+// subnormal number, of which the matrix unit keeps fewer bits, small outputs were off
+// by 2^-16 of the values.)
 struct Codes {
   uint32_t low, high, base;
   f16x2 sixteenth;
@@ -104,15 +105,15 @@ __device__ __forceinline__ int query_shift(float largest) {
 // second operand (rounded once, they would be half as far off again as their own
 // rounding makes them).
 //
-// Bound: reading the cache (256 sequences of 8192, 16 heads of 128 over 4: 245 us, 4.7
-// TB/s, in bf16 234; the 16-bit cache 742), the issue of instructions more than half of
-// the time (about 300 vector ones for 32 keys, 64 of them for e instead of codes, which
-// cost 10 of the 245 us; in fp16 24 matrix ones, in bf16 16).  64 sequences of 64 to
+// Bound: reading the cache (256 sequences of 8192, 16 heads of 128 over 4: 240 us, 4.75
+// TB/s, in bf16 230; the 16-bit cache 742), the issue of instructions more than half of
+// the time (in fp16 281 vector and 24 matrix ones for 32 keys, in bf16 16 matrix ones; 64
+// vector ones are for e instead of codes, which cost 3 to 4 percent).  64 sequences of 64 to
 // 4096, 32 heads over 8: 46 us, 3.1 TB/s, of which 5 the join and
 // much of the rest beginnings and ends of sequences, 4 us each.  P16 (pages of a
 // multiple of 16 tokens): the wave finds addresses, else lanes do and pass them on.
 // Loads past the caches are slower here (by a fifth): rows of 68 bytes share lines.
-// Three blocks a CU up to D 64 (285 us for 256 of 8192, 8 heads; two took 315 and more);
+// Three blocks a CU up to D 64 (280 us for 256 of 8192, 8 heads; two took 315 and more);
 // at 128 the registers would not hold it (spilled, by a quarter slower).
 template <typename T, int DP, int WAVES, bool P16>
 __global__ void __launch_bounds__(WAVES * 64, WAVES == kStepWaves ? (DP <= 64 ? 3 : 2) : WAVES / 4)
@@ -437,23 +438,26 @@ constexpr int wide_waves4(int D) { return D <= 32 ? 16 : 8; }  // by the registe
 
 // How a call's sequences are cut.  Times in us, of back-to-back calls.
 // - A block of four waves per sequence and head where no sequence has more than
-//   eight tiles (64 of up to 1024, 8 heads of 64: 14, wide blocks 15, shares 18; of 128: 18, 22, 23),
-//   or blocks are many and even out by themselves (1024 of up to 2048, 2 x 128: 86, in shares 97; 2048 of up
-//   to 1000, 4 x 64: 75, in shares 133).
+//   eight tiles (64 of up to 1024, 8 heads of 64: 14, wide blocks 16, shares 18; of 128: 17.5, 21, 22),
+//   or blocks are many and even out by themselves (1024 of up to 2048, 2 x 128: 90, in shares 100; 2048 of up
+//   to 1000, 4 x 64: 74, in shares 132).  For more than 512 sequences whatever the table's
+//   length: 8 percent where they are even (1024 of 8192, 8 x 64: 1,055, in shares 1,141),
+//   nothing where they are not (of up to 8192 by their logarithm: 213 and 205), and one very
+//   long one among them is waited for (600 of up to 500 but one of 131,072: 975, in shares 87).
 // - A wide block per sequence and head where blocks are too few to fill the chip
-//   and sequences short (16 of 1024, 8 x 64: 9.1, blocks of four waves 12.7, shares 14.1).
+//   and sequences short (16 of 1024, 8 x 64: 9.2, blocks of four waves 12.2, shares 14.0).
 // - Else equal shares of all tiles, two blocks for every CU (three up to D 64, where
 //   the registers allow it), and a second launch that joins them (256 of up to 8192
-//   by their logarithm, 8 x 128: 78, a block per sequence 122; 256 of 8192 each, 8 x 64: 271, a block per
-//   sequence 259: the host does not know lengths).
+//   by their logarithm, 8 x 128: 81, a block per sequence 129; 256 of 8192 each, 8 x 64: 288, a block per
+//   sequence 270: the host does not know lengths).
 struct Plan {
   int32_t workers;  // 0: a block per sequence and head
   bool wide;
 };
 
 // What a sequence's beginning costs a share, in tiles: us for 64 sequences of 64 to 4096
-// (32 heads of 128 over 8) with none, 1, 2, 3, 4 and 6: 48.3, 45.8, 44.3, 43.9, 44.7, 46.7; for 256 of up
-// to 8192 by their logarithm (16 over 8) 98, 84, 78, 79, 83, 89.
+// (32 heads of 128 over 8) with none, 1, 2, 3, 4 and 6: 50.4, 47.4, 46.0, 45.7, 46.5, 48.5; for 256 of up
+// to 8192 by their logarithm (16 over 8) 100.6, 86.5, 81.0, 83.4, 88.2, 94.0.
 constexpr int32_t kLead = 2;
 
 Plan plan_step(int64_t B, int32_t heads, int32_t D, int64_t most) {

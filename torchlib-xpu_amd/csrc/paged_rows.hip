@@ -169,12 +169,13 @@ __device__ __forceinline__ bool wave_tile(const RowsArgs& a, WaveTile* t) {
 
 // A wave takes tile_rows rows (ONE: one); GS lanes take a head, eight values
 // each: four pairs, or eight values that do not turn (16 bytes at a time where they
-// lie together: 256 lists of up to 512, 16 heads of 96, 69.7 -> 65.6 us).  Bound: the
-// copy, for batches that fill the chip (4 lists of 4096, 20 heads of 128, one way:
-// 39 us, 4.3 TB/s; appends of 32 lists of up to 2000, 32 heads of 128: 105 us, 5.0
-// TB/s); few rows by the loads in turn before them (64 rows of 48 heads: 4.2 us).
-// Many short waves hide these loads best: waves of four or more rows that ask for
-// the next heads beforehand took 74 for 65 us, 120 to 138 for 105.
+// lie together: 256 lists of up to 512, 16 heads of 96, both ways, 69.7 -> 65.6 us in
+// calls one after another).  Bound: the copy, for batches that fill the chip (4 lists
+// of 4096, 20 heads of 128, one way: 39 us, 4.3 TB/s; appends of 32 lists of up to
+// 2000, 32 heads of 128: 108 us, 4.8 TB/s, into 4-bit rows 112, 3.8 TB/s); few rows
+// by the loads in turn before them (64 rows of 48 heads: 4.1 us).  Many short waves
+// hide these loads best: waves of four or more rows that ask for the next heads
+// beforehand took 74 for 65 us, 120 to 138 for 105.
 template <typename T, int GS, Kind KIND, bool ONE>
 __global__ void __launch_bounds__(kRowsWaves * 64) rows_kernel(const RowsArgs a) {
   using X4 = typename Quad<T>::type;
